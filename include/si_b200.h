@@ -444,6 +444,107 @@ SI_API si_status si_attention_prefill_dev(si_ctx *ctx, si_kv *kv, const si_dims 
                                           float *out_dev);
 
 /* ------------------------------------------------------------------------ */
+/* Paged KV cache in 4 bits (no reference counterpart: the reference's cache  */
+/* is one fp16 array).  A row -- one position's K or V of one KV head -- is    */
+/* held as Q4_0 blocks of 32 dims (the weights' rule: d = (value of largest    */
+/* magnitude) / -8, code = min(15, trunc(x * (1/d) + 8.5)), scale fp16(d), a    */
+/* code standing for scale * (code - 8)): 4.5 bits a value, 3.56x fewer bytes   */
+/* than fp16.  Values up to 524,000 keep a finite scale.                        */
+/*                                                                              */
+/* Positions live in pages of page_len positions (a multiple of 16, up to       */
+/* 4096); sequences 0 .. n_seqs-1 each hold the pages of their first positions, */
+/* in order, and several sequences may hold one page.  The pool is              */
+/*   [n_pages][n_kv_heads][page_len / 16] groups of 16 positions, a group being */
+/*   16 rows of K codes (D/2 bytes each), 16 rows of K scales (D/32 fp16 each), */
+/*   then the same for V.                                                       */
+/* Codes lie in 16-bit groups of four neighbouring dims, nibble i = dim i: dims  */
+/* 32b + 4g .. 32b + 4g + 3 are half-word g * (D/32) + b of the row.             */
+/*                                                                              */
+/* The page tables are kept on the host and mirrored on the device; calls that  */
+/* change them are refused (SI_ERR_INVALID) during a graph capture, take their  */
+/* arguments at once, and queue the device's part on the context's stream.  A   */
+/* refused call changes nothing.  Free pages are handed out lowest first.       */
+/* Calls on one cache come from one thread at a time, like all calls of one     */
+/* context.                                                                     */
+/* ------------------------------------------------------------------------ */
+typedef struct si_kv4 si_kv4;
+/* `count` consecutive tokens of sequence `seq`, the first at position `pos`.
+ * Calls take a list of runs; their row-wise tensors hold the runs' tokens one
+ * after the other.  A decode batch is runs of one token, a prompt one long run,
+ * and a list may mix them.  At most 4,194,304 tokens a call. */
+typedef struct {
+    int seq, pos, count;
+} si_kv4_run;
+/* Bytes of one page (0 for bad arguments); host only. */
+SI_API size_t si_kv4_page_bytes(const si_dims *dims, int page_len);
+/* pool_dev NULL: the pool is allocated and zeroed; else n_pages *
+ * si_kv4_page_bytes of the caller's device memory, 16-byte aligned, used as it
+ * is and left to the caller, who keeps it until si_kv4_free. */
+SI_API si_status si_kv4_create(si_ctx *ctx, const si_dims *dims, int n_seqs, int max_ctx,
+                               int n_pages, int page_len, void *pool_dev, si_kv4 **out);
+SI_API void si_kv4_free(si_kv4 *kv);
+/* 0 = the pool, 1 = the device page tables, int [n_seqs][ceil(max_ctx /
+ * page_len)], -1 where a sequence holds no page (read only). */
+SI_API void *si_kv4_device_ptr(si_kv4 *kv, int which);
+SI_API int si_kv4_free_pages(const si_kv4 *kv);
+/* Number of pages that seq holds (-1 for a bad seq), the first `cap` of them
+ * in pages[] (which may be NULL). */
+SI_API int si_kv4_pages(const si_kv4 *kv, int seq, int *pages, int cap);
+/* Pages for writing to the runs: missing ones are taken (from the sequence's
+ * first missing one on, so a gap before pos is filled too, its contents
+ * unspecified), a page that another sequence holds as well is replaced by a
+ * copy.  si_kv4_append_dev and si_step_kv4_dev do this themselves; steps with
+ * device-resident lengths, and captured ones, need it done before. */
+SI_API si_status si_kv4_reserve(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs, int n);
+/* Sequence seqs[i], which holds no pages, gets the next counts[i] of pages[]
+ * (as when a stored cache is put back; pages may be held already). */
+SI_API si_status si_kv4_assign(si_ctx *ctx, si_kv4 *kv, const int *seqs, const int *counts, int n,
+                               const int *pages);
+/* Sequence dst[i], which holds no pages, begins with the first lens[i]
+ * positions of src[i]: whole pages are shared, the page in which lens[i] ends
+ * is copied.  dst holds each sequence once. */
+SI_API si_status si_kv4_fork(si_ctx *ctx, si_kv4 *kv, const int *src, const int *dst,
+                             const int *lens, int n);
+/* Sequence seqs[i] keeps the pages of its first keep[i] positions (keep NULL:
+ * none); a page that no sequence holds any more is free. */
+SI_API si_status si_kv4_release(si_ctx *ctx, si_kv4 *kv, const int *seqs, const int *keep, int n);
+/* The used pages become pages 0 .. *used-1 (used may be NULL): the i-th used
+ * page from *used on moves to the i-th free page below.  The used part of the
+ * pool can then be stored with one copy. */
+SI_API si_status si_kv4_compact(si_ctx *ctx, si_kv4 *kv, int *used);
+/* Quantises rows k, v [T][Hkv][D] (fp32, keys as the attention is to see them)
+ * into the runs' positions, no position twice in a call. */
+SI_API si_status si_kv4_append_dev(si_ctx *ctx, si_kv4 *kv, const float *k_dev, const float *v_dev,
+                                   const si_kv4_run *runs, int n);
+/* The runs' rows as fp32 [T][Hkv][D] (either may be NULL), 16-byte aligned. */
+SI_API si_status si_kv4_read_dev(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs, int n,
+                                 float *k_dev, float *v_dev);
+/* Attention of queries q [T][Hq][D] (RoPE applied; 16-byte aligned, as out)
+ * over the cache: the token at position p attends positions 0 .. p of its
+ * sequence, whose pages must cover it.  A run at pos -1 begins with a token
+ * that attends nothing; its row of out is zeros (padding of a batch).  Runs of
+ * 16 tokens and more go through the prefill kernels over their keys unpacked
+ * once (the kernel follows si_ctx_set_exact_attention), shorter ones read the
+ * packed cache directly.  fp32 in and out; no product's input is rounded to
+ * fewer than 22 bits.  Sums follow the split of the work, so a token's result
+ * may differ in its last bits between calls with other runs. */
+SI_API si_status si_attention_kv4_dev(si_ctx *ctx, si_kv4 *kv, const si_dims *dims,
+                                      const float *q_dev, const si_kv4_run *runs, int n,
+                                      float *out_dev);
+/* Layer steps over such a cache: x and y are [T][H] for the runs' tokens, each
+ * written to the cache at its position and attending positions 0 .. its own.
+ * Modes as si_decode_step. */
+SI_API si_status si_step_kv4_dev(si_ctx *ctx, si_layer *l, si_kv4 *kv, const float *x_dev,
+                                 const si_kv4_run *runs, int n, float *y_dev, int mode);
+/* A decode step of sequences 0 .. batch-1 with the lengths of st (whose
+ * max_ctx must equal the cache's).  The positions must be reserved: a token
+ * whose position has no page of its own is not written and records
+ * SI_ERR_INVALID in the context's error word. */
+SI_API si_status si_decode_step_state_kv4_dev(si_ctx *ctx, si_layer *l, si_kv4 *kv,
+                                              const float *x_dev, si_decode_state *st,
+                                              float *y_dev, int mode);
+
+/* ------------------------------------------------------------------------ */
 /* Reference-shaped entry points (host pointers, implicit context).          */
 /* ------------------------------------------------------------------------ */
 

@@ -7,6 +7,7 @@
 #include <dlfcn.h>
 #include <nccl.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -20,6 +21,7 @@
 
 #include "../../include/si_b200.h"
 #include "si_kernels.cuh"
+#include "si_kv4_pages.hpp"
 
 // ----------------------------------------------------------------------------
 // errors
@@ -78,14 +80,28 @@ extern "C" SI_API const char *si_last_error(void) { return g_last_error.c_str();
 struct DevBuf {
   void *p = nullptr;
   size_t bytes = 0;
+  // Once the context has captured a graph, memory that a captured kernel may
+  // hold stays until the context goes: growth sets it aside.
+  bool keep = false;
+  std::vector<void *> kept;
+  size_t kept_bytes = 0;
   void release() {
     if (p) cudaFree(p);
+    for (void *k : kept) cudaFree(k);
+    kept.clear();
     p = nullptr;
-    bytes = 0;
+    bytes = kept_bytes = 0;
   }
   si_status reserve(size_t n) {
     if (n <= bytes) return SI_OK;
-    release();
+    if (keep && p) {
+      kept.push_back(p);
+      kept_bytes += bytes;
+      p = nullptr;
+      bytes = 0;
+    } else if (!keep) {
+      release();
+    }
     cudaError_t e = cudaMalloc(&p, n);
     if (e != cudaSuccess) {
       p = nullptr;
@@ -109,6 +125,7 @@ struct si_ctx {
   DevBuf gemm;                  // tcgen05 GEMM scratch (transposed activation scales)
   DevBuf hx, hy;                // device staging of the host-pointer step forms
   DevBuf attn;                  // tensor-core prefill attention: fp16 operand splits
+  DevBuf kv4;                   // 4-bit cache attention: split partials, a prompt's rows
   int exact_attention = 0;      // 1: prefill attention by the fp32 kernel (bit-identical
                                 // to decode steps) instead of the tensor cores
   int *pinned_idx = nullptr;    // host staging for idx: kIdxSlots slots of pinned_idx_n ints
@@ -207,6 +224,32 @@ struct si_kv {
   size_t seq_elems() const { return (size_t)max_ctx * row_elems(); }
 };
 
+// Paged KV cache in 4 bits: the pool, the device copies of the page tables and
+// reference counts, and the host's own.
+struct si_kv4 {
+  si_ctx *ctx = nullptr;
+  si_dims d{};
+  int max_ctx = 0, page_len = 0;
+  uint8_t *pool = nullptr;
+  bool own_pool = false;
+  size_t page_bytes = 0;
+  int *tables = nullptr, *refs = nullptr;
+  si::Kv4Pages *pages = nullptr;
+  si::Kv4View view() const {
+    si::Kv4View v;
+    v.pool = pool;
+    v.tables = tables;
+    v.refs = refs;
+    v.n_pages = pages->n_pages();
+    v.page_len = page_len;
+    v.n_kv_heads = d.n_kv_heads;
+    v.head_dim = d.head_dim;
+    v.n_seqs = pages->n_seqs();
+    v.max_pages = pages->max_pages();
+    return v;
+  }
+};
+
 static si_status set_device(si_ctx *ctx) {
   SI_CHECK(ctx, "null context");
   SI_CUDA(cudaSetDevice(ctx->device));
@@ -296,6 +339,7 @@ extern "C" SI_API void si_ctx_destroy(si_ctx *c) {
   c->hx.release();
   c->hy.release();
   c->attn.release();
+  c->kv4.release();
   if (c->pinned_idx) cudaFreeHost(c->pinned_idx);
   for (cudaEvent_t e : c->idx_ev)
     if (e) cudaEventDestroy(e);
@@ -335,9 +379,12 @@ extern "C" SI_API unsigned long long si_kernel_launches(void) {
 }
 
 extern "C" SI_API size_t si_ctx_scratch_bytes(const si_ctx *ctx) {
-  return ctx ? ctx->work.bytes + ctx->idx.bytes + ctx->gemm.bytes + ctx->hx.bytes +
-                   ctx->hy.bytes + ctx->attn.bytes
-             : 0;
+  if (!ctx) return 0;
+  size_t n = 0;
+  for (const DevBuf *b : {&ctx->work, &ctx->idx, &ctx->gemm, &ctx->hx, &ctx->hy, &ctx->attn,
+                          &ctx->kv4})
+    n += b->bytes + b->kept_bytes;
+  return n;
 }
 
 // ----------------------------------------------------------------------------
@@ -351,6 +398,8 @@ struct si_graph {
 extern "C" SI_API si_status si_graph_begin(si_ctx *ctx) {
   SI_TRY(set_device(ctx));
   SI_CUDA(cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal));
+  for (DevBuf *b : {&ctx->work, &ctx->idx, &ctx->gemm, &ctx->hx, &ctx->hy, &ctx->attn, &ctx->kv4})
+    b->keep = true;
   return SI_OK;
 }
 
@@ -1032,6 +1081,512 @@ extern "C" SI_API void *si_kv_device_ptr(si_kv *kv, int which) {
 }
 
 // ----------------------------------------------------------------------------
+// paged KV cache in 4 bits
+// ----------------------------------------------------------------------------
+static_assert(sizeof(si_kv4_run) == sizeof(si::Kv4Run), "one layout for runs");
+
+// No C++ exception leaves a C entry point: the bookkeeping's containers may
+// run out of host memory.
+template <class F>
+static si_status kv4_entry(F f) {
+  try {
+    return f();
+  } catch (...) {
+    return fail(SI_ERR_OOM, "out of host memory");
+  }
+}
+
+static const si::Kv4Run *as_runs(const si_kv4_run *r) {
+  return reinterpret_cast<const si::Kv4Run *>(r);
+}
+
+// Attention of a run of at least this many tokens goes through the prefill
+// kernels over the run's keys unpacked once.
+constexpr int kKv4PrefillMin = 16;
+
+extern "C" SI_API size_t si_kv4_page_bytes(const si_dims *d, int page_len) {
+  if (check_dims(d) != SI_OK || page_len <= 0 || page_len % si::kKv4Group) return 0;
+  return (size_t)(page_len / si::kKv4Group) * d->n_kv_heads * si::kv4_group_bytes(d->head_dim);
+}
+
+extern "C" SI_API si_status si_kv4_create(si_ctx *ctx, const si_dims *d, int n_seqs, int max_ctx,
+                                          int n_pages, int page_len, void *pool_dev,
+                                          si_kv4 **out) {
+  return kv4_entry([&]() -> si_status {
+    SI_TRY(set_device(ctx));
+    SI_TRY(check_dims(d));
+    SI_CHECK(out && n_seqs > 0 && max_ctx > 0 && n_pages > 0, "bad KV cache arguments");
+    *out = nullptr;
+    SI_CHECK(page_len >= si::kKv4Group && page_len <= 4096 && page_len % si::kKv4Group == 0,
+             "page_len must be a multiple of %d up to 4096", si::kKv4Group);
+    SI_CHECK(max_ctx <= (1 << 30), "max_ctx out of range");
+    const int64_t max_pages = ((int64_t)max_ctx + page_len - 1) / page_len;
+    SI_CHECK(max_pages * n_seqs < (1ll << 30), "too many table entries");
+    SI_CHECK((int64_t)n_pages * d->n_kv_heads * (page_len / si::kKv4Group) < (1ll << 31),
+             "too many pages");
+    SI_CHECK((reinterpret_cast<uintptr_t>(pool_dev) & 15) == 0, "pool must be 16-byte aligned");
+    si_kv4 *kv = new si_kv4();
+    kv->ctx = ctx;
+    kv->d = *d;
+    kv->max_ctx = max_ctx;
+    kv->page_len = page_len;
+    kv->page_bytes = si_kv4_page_bytes(d, page_len);
+    kv->pool = static_cast<uint8_t *>(pool_dev);
+    const size_t pool_bytes = kv->page_bytes * n_pages;
+    const size_t tb = (size_t)max_pages * n_seqs * sizeof(int), rb = (size_t)n_pages * sizeof(int);
+    cudaError_t e = cudaSuccess;
+    try {
+      kv->pages = new si::Kv4Pages(n_seqs, (int)max_pages, n_pages, page_len);
+    } catch (...) {
+      si_kv4_free(kv);
+      throw;
+    }
+    if (!kv->pool) {
+      e = cudaMalloc(&kv->pool, pool_bytes);
+      kv->own_pool = e == cudaSuccess;
+      if (e != cudaSuccess) kv->pool = nullptr;
+      if (e == cudaSuccess) e = cudaMemsetAsync(kv->pool, 0, pool_bytes, ctx->stream);
+    }
+    if (e == cudaSuccess) e = cudaMalloc(&kv->tables, tb);
+    if (e == cudaSuccess) e = cudaMalloc(&kv->refs, rb);
+    if (e == cudaSuccess) e = cudaMemsetAsync(kv->tables, 0xff, tb, ctx->stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(kv->refs, 0, rb, ctx->stream);
+    if (e != cudaSuccess) {
+      si_kv4_free(kv);
+      return fail(e == cudaErrorMemoryAllocation ? SI_ERR_OOM : SI_ERR_CUDA,
+                  "4-bit KV cache of %zu bytes: %s", pool_bytes, cudaGetErrorString(e));
+    }
+    *out = kv;
+    return SI_OK;
+  });
+}
+
+extern "C" SI_API void si_kv4_free(si_kv4 *kv) {
+  if (!kv) return;
+  // (cudaFree waits for work that is queued; the context may be gone already)
+  if (kv->own_pool) cudaFree(kv->pool);
+  cudaFree(kv->tables);
+  cudaFree(kv->refs);
+  delete kv->pages;
+  delete kv;
+}
+
+extern "C" SI_API void *si_kv4_device_ptr(si_kv4 *kv, int which) {
+  if (!kv) return nullptr;
+  return which == 0 ? static_cast<void *>(kv->pool) : kv->tables;
+}
+extern "C" SI_API int si_kv4_free_pages(const si_kv4 *kv) {
+  return kv ? kv->pages->free_pages() : 0;
+}
+extern "C" SI_API int si_kv4_pages(const si_kv4 *kv, int seq, int *pages, int cap) {
+  if (!kv || seq < 0 || seq >= kv->pages->n_seqs()) return -1;
+  const int n = kv->pages->count(seq);
+  for (int i = 0; pages && i < n && i < cap; ++i) pages[i] = kv->pages->page(seq, i);
+  return n;
+}
+
+// Page changes are not captured: a replay would put back the tables of the
+// time of capture.
+static si_status kv4_not_capturing(si_ctx *ctx) {
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  SI_CUDA(cudaStreamIsCapturing(ctx->stream, &cs));
+  SI_CHECK(cs == cudaStreamCaptureStatusNone,
+           "pages cannot change during a graph capture: reserve them before it");
+  return SI_OK;
+}
+
+template <int PAIRS>
+static si_status kv4_push(si_ctx *ctx, si_kv4 *kv, const std::vector<std::pair<int, int>> *part) {
+  si::Kv4Update<PAIRS> u;
+  u.tables = kv->tables;
+  u.refs = kv->refs;
+  u.pool = kv->pool;
+  u.page_bytes = kv->page_bytes;
+  size_t at[3] = {0, 0, 0};
+  do {
+    int n[3], used = 0;
+    for (int k = 0; k < 3; ++k) {
+      n[k] = (int)std::min<size_t>(part[k].size() - at[k], (size_t)(PAIRS - used));
+      for (int i = 0; i < n[k]; ++i) {
+        u.word[2 * (used + i)] = part[k][at[k] + i].first;
+        u.word[2 * (used + i) + 1] = part[k][at[k] + i].second;
+      }
+      at[k] += n[k];
+      used += n[k];
+    }
+    u.n_table = n[0];
+    u.n_refs = n[1];
+    u.n_copies = n[2];
+    SI_CUDA(si::launch_kv4_update(u, ctx->stream));
+  } while (at[0] < part[0].size() || at[1] < part[1].size() || at[2] < part[2].size());
+  return SI_OK;
+}
+
+// Queues a change of the pages on the context's stream.
+static si_status kv4_flush(si_ctx *ctx, si_kv4 *kv, si::Kv4Edits &e) {
+  std::sort(e.touched.begin(), e.touched.end());
+  e.touched.erase(std::unique(e.touched.begin(), e.touched.end()), e.touched.end());
+  std::vector<std::pair<int, int>> part[3];
+  part[0].swap(e.table);
+  for (int pg : e.touched) part[1].push_back({pg, kv->pages->refs(pg)});
+  part[2].swap(e.copies);
+  const size_t n = part[0].size() + part[1].size() + part[2].size();
+  if (n == 0) return SI_OK;
+  return n <= si::kKv4SmallPairs ? kv4_push<si::kKv4SmallPairs>(ctx, kv, part)
+                                 : kv4_push<si::kKv4LargePairs>(ctx, kv, part);
+}
+
+#define SI_PAGES(kv, call) \
+  SI_CHECK((kv)->pages->call, "%s", (kv)->pages->why().c_str())
+
+static si_status kv4_check(si_ctx *ctx, const si_kv4 *kv) {
+  SI_TRY(set_device(ctx));
+  SI_CHECK(kv && kv->ctx == ctx, "null KV cache, or one of another context");
+  return SI_OK;
+}
+
+// Pages to write the runs to, queued; no two tokens may go to one position.
+static si_status kv4_writable(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs, int n) {
+  SI_CHECK(kv->pages->runs_ok(as_runs(runs), n), "%s", kv->pages->why().c_str());
+  for (int i = 0; i < n; ++i)
+    SI_CHECK((int64_t)runs[i].pos + runs[i].count <= kv->max_ctx, "positions past max_ctx %d",
+             kv->max_ctx);
+  if (n > 1) {
+    std::vector<si::Kv4Run> r(as_runs(runs), as_runs(runs) + n);
+    std::sort(r.begin(), r.end(), [](const si::Kv4Run &a, const si::Kv4Run &b) {
+      return a.seq != b.seq ? a.seq < b.seq : a.pos < b.pos;
+    });
+    const si::Kv4Run *last = nullptr;
+    for (const si::Kv4Run &x : r) {
+      if (x.count == 0) continue;
+      SI_CHECK(!last || last->seq != x.seq || last->pos + last->count <= x.pos,
+               "two tokens for one position of sequence %d", x.seq);
+      last = &x;
+    }
+  }
+  if (kv->pages->writable(as_runs(runs), n)) return SI_OK;
+  SI_TRY(kv4_not_capturing(ctx));
+  si::Kv4Edits e;
+  SI_PAGES(kv, reserve(as_runs(runs), n, &e));
+  return kv4_flush(ctx, kv, e);
+}
+
+extern "C" SI_API si_status si_kv4_reserve(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs,
+                                           int n) {
+  return kv4_entry([&]() -> si_status {
+    SI_TRY(kv4_check(ctx, kv));
+    SI_CHECK(runs && n >= 0, "null runs");
+    SI_TRY(kv4_not_capturing(ctx));
+    for (int i = 0; i < n; ++i)
+      SI_CHECK((int64_t)runs[i].pos + runs[i].count <= kv->max_ctx, "positions past max_ctx %d",
+               kv->max_ctx);
+    si::Kv4Edits e;
+    SI_PAGES(kv, reserve(as_runs(runs), n, &e));
+    return kv4_flush(ctx, kv, e);
+  });
+}
+
+extern "C" SI_API si_status si_kv4_assign(si_ctx *ctx, si_kv4 *kv, const int *seqs,
+                                          const int *counts, int n, const int *pages) {
+  return kv4_entry([&]() -> si_status {
+    SI_TRY(kv4_check(ctx, kv));
+    SI_CHECK(n >= 0 && (n == 0 || (seqs && counts && pages)), "null argument");
+    SI_TRY(kv4_not_capturing(ctx));
+    si::Kv4Edits e;
+    SI_PAGES(kv, assign(seqs, counts, n, pages, &e));
+    return kv4_flush(ctx, kv, e);
+  });
+}
+
+extern "C" SI_API si_status si_kv4_fork(si_ctx *ctx, si_kv4 *kv, const int *src, const int *dst,
+                                        const int *lens, int n) {
+  return kv4_entry([&]() -> si_status {
+    SI_TRY(kv4_check(ctx, kv));
+    SI_CHECK(n >= 0 && (n == 0 || (src && dst && lens)), "null argument");
+    SI_TRY(kv4_not_capturing(ctx));
+    si::Kv4Edits e;
+    SI_PAGES(kv, fork(src, dst, lens, n, &e));
+    return kv4_flush(ctx, kv, e);
+  });
+}
+
+extern "C" SI_API si_status si_kv4_release(si_ctx *ctx, si_kv4 *kv, const int *seqs,
+                                           const int *keep, int n) {
+  return kv4_entry([&]() -> si_status {
+    SI_TRY(kv4_check(ctx, kv));
+    SI_CHECK(n >= 0 && (n == 0 || seqs), "null argument");
+    SI_TRY(kv4_not_capturing(ctx));
+    si::Kv4Edits e;
+    SI_PAGES(kv, release(seqs, keep, n, &e));
+    return kv4_flush(ctx, kv, e);
+  });
+}
+
+extern "C" SI_API si_status si_kv4_compact(si_ctx *ctx, si_kv4 *kv, int *used) {
+  return kv4_entry([&]() -> si_status {
+    SI_TRY(kv4_check(ctx, kv));
+    SI_TRY(kv4_not_capturing(ctx));
+    si::Kv4Edits e;
+    const int n = kv->pages->compact(&e);
+    SI_TRY(kv4_flush(ctx, kv, e));
+    if (used) *used = n;
+    return SI_OK;
+  });
+}
+
+// Calls f(runs by value, tokens) for consecutive pieces of the list: at most
+// kKv4MaxRuns runs and 32768 tokens each (a launch's grid holds 65535).
+template <class F>
+static si_status kv4_pieces(const si_kv4_run *runs, const int *rows, int n, F f) {
+  constexpr int kTokens = 32768;
+  si::Kv4Runs p;
+  p.n = 0;
+  int tokens = 0;
+  for (int i = 0; i < n; ++i) {
+    for (int done = 0; done < runs[i].count;) {
+      const int take = std::min(runs[i].count - done, kTokens - tokens);
+      p.seq[p.n] = runs[i].seq;
+      p.pos[p.n] = runs[i].pos + done;
+      p.row0[p.n++] = rows[i] + done;
+      p.row0[p.n] = rows[i] + done + take;
+      done += take;
+      tokens += take;
+      const bool next_apart = i + 1 < n && rows[i + 1] != rows[i] + done;
+      if (p.n == si::kKv4MaxRuns || tokens == kTokens || (done == runs[i].count && next_apart)) {
+        SI_TRY(f(p, tokens));
+        p.n = tokens = 0;
+      }
+    }
+  }
+  return tokens ? f(p, tokens) : SI_OK;
+}
+
+static std::vector<int> kv4_rows(const si_kv4_run *runs, int n) {
+  std::vector<int> rows(n);
+  int at = 0;
+  for (int i = 0; i < n; ++i) {
+    rows[i] = at;
+    at += runs[i].count;
+  }
+  return rows;
+}
+
+// Total rows of a list within the limits of one call.
+static si_status kv4_count(const si_kv4_run *runs, int n, int *T) {
+  SI_CHECK(n >= 0 && (n == 0 || runs), "null runs");
+  int64_t rows = 0;
+  for (int i = 0; i < n; ++i) {
+    SI_CHECK(runs[i].count >= 0, "negative token count");
+    rows += runs[i].count;
+  }
+  SI_CHECK(rows <= (1 << 22), "%lld tokens in one call", (long long)rows);
+  *T = (int)rows;
+  return SI_OK;
+}
+
+extern "C" SI_API si_status si_kv4_append_dev(si_ctx *ctx, si_kv4 *kv, const float *k,
+                                              const float *v, const si_kv4_run *runs, int n) {
+  return kv4_entry([&]() -> si_status {
+    SI_TRY(kv4_check(ctx, kv));
+    int T = 0;
+    SI_TRY(kv4_count(runs, n, &T));
+    if (T == 0) return SI_OK;
+    SI_CHECK(k && v, "null K or V rows");
+    SI_TRY(kv4_writable(ctx, kv, runs, n));
+    const std::vector<int> rows = kv4_rows(runs, n);
+    si::Kv4AppendArgs a{};
+    a.kv = kv->view();
+    a.k = k;
+    a.v = v;
+    a.ldkv = (size_t)kv->d.n_kv_heads * kv->d.head_dim;
+    a.err = ctx->err;
+    return kv4_pieces(runs, rows.data(), n, [&](const si::Kv4Runs &p, int tokens) -> si_status {
+      a.runs = p;
+      a.T = tokens;
+      SI_CUDA(si::launch_kv4_append(a, ctx->stream));
+      return SI_OK;
+    });
+  });
+}
+
+// Rows [pos, pos + count) of every run lie within its sequence's pages.
+static si_status kv4_covered(const si_kv4 *kv, const si_kv4_run *runs, int n, int lowest) {
+  for (int i = 0; i < n; ++i) {
+    SI_CHECK(kv->pages->seq_ok(runs[i].seq), "%s", kv->pages->why().c_str());
+    SI_CHECK(runs[i].pos >= lowest && runs[i].count >= 0 &&
+                 (int64_t)runs[i].pos + runs[i].count <= kv->pages->covered(runs[i].seq),
+             "positions [%d, %d + %d) outside the pages of sequence %d", runs[i].pos, runs[i].pos,
+             runs[i].count, runs[i].seq);
+  }
+  return SI_OK;
+}
+
+static si_status kv4_read(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs, int n, float *k,
+                          float *v) {
+  const std::vector<int> rows = kv4_rows(runs, n);
+  si::Kv4ReadArgs a{};
+  a.kv = kv->view();
+  a.k = k;
+  a.v = v;
+  a.err = ctx->err;
+  return kv4_pieces(runs, rows.data(), n, [&](const si::Kv4Runs &p, int tokens) -> si_status {
+    a.runs = p;
+    a.T = tokens;
+    SI_CUDA(si::launch_kv4_read(a, ctx->stream));
+    return SI_OK;
+  });
+}
+
+extern "C" SI_API si_status si_kv4_read_dev(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs, int n,
+                                            float *k, float *v) {
+  return kv4_entry([&]() -> si_status {
+    SI_TRY(kv4_check(ctx, kv));
+    int T = 0;
+    SI_TRY(kv4_count(runs, n, &T));
+    SI_TRY(kv4_covered(kv, runs, n, 0));
+    SI_CHECK(((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0,
+             "K and V rows must be 16-byte aligned");
+    return kv4_read(ctx, kv, runs, n, k, v);
+  });
+}
+
+// A step's queries rotated into q_out and its keys and values written to
+// their pages, from the fused projections [T][(Hq + 2 Hkv) * D].
+static si_status kv4_rope_append(si_ctx *ctx, si_kv4 *kv, const si_dims &d, const float *qkv, int T,
+                                 const si_kv4_run *runs, int n, const int *tok_ctx, float *q_out) {
+  const size_t QD = (size_t)d.n_q_heads * d.head_dim, KVD = (size_t)d.n_kv_heads * d.head_dim;
+  si::Kv4AppendArgs a{};
+  a.kv = kv->view();
+  a.q = qkv;
+  a.k = qkv + QD;
+  a.v = qkv + QD + KVD;
+  a.ldq = a.ldkv = QD + 2 * KVD;
+  a.q_out = q_out;
+  a.n_q_heads = d.n_q_heads;
+  a.cos_tab = ctx->cos_tab;
+  a.sin_tab = ctx->sin_tab;
+  a.max_positions = ctx->max_positions;
+  a.err = ctx->err;
+  if (tok_ctx) {
+    a.tok_ctx = tok_ctx;
+    a.T = T;
+    SI_CUDA(si::launch_kv4_append(a, ctx->stream));
+    return SI_OK;
+  }
+  const std::vector<int> rows = kv4_rows(runs, n);
+  return kv4_pieces(runs, rows.data(), n, [&](const si::Kv4Runs &p, int tokens) -> si_status {
+    a.runs = p;
+    a.T = tokens;
+    SI_CUDA(si::launch_kv4_append(a, ctx->stream));
+    return SI_OK;
+  });
+}
+
+// The attention of a list of runs (checked by the caller), or with tok_ctx of
+// token t at position tok_ctx[t] - 1 of sequence t.
+static si_status kv4_attend(si_ctx *ctx, si_kv4 *kv, int n_q_heads, const float *q,
+                            const si_kv4_run *runs, int n, int T, const int *tok_ctx, float *out) {
+  const int D = kv->d.head_dim;
+  const size_t row = (size_t)n_q_heads * D;
+  si::Kv4AttnArgs a{};
+  a.kv = kv->view();
+  a.n_q_heads = n_q_heads;
+  a.q = q;
+  a.out = out;
+  a.err = ctx->err;
+  if (tok_ctx) {
+    a.tok_ctx = tok_ctx;
+    a.T = T;
+    a.nsplit = si::kv4_pick_splits(T, kv->d.n_kv_heads, (long long)T * kv->max_ctx, kv->max_ctx);
+    SI_TRY(ctx->kv4.reserve(si::kv4_part_floats(T, n_q_heads, D, a.nsplit) * sizeof(float)));
+    a.part = static_cast<float *>(ctx->kv4.p);
+    SI_CUDA(si::launch_attention_kv4(a, ctx->stream));
+    return SI_OK;
+  }
+  const std::vector<int> rows = kv4_rows(runs, n);
+  // Few tokens a run: one token at a time over the packed cache.
+  std::vector<si_kv4_run> few;
+  std::vector<int> few_rows;
+  for (int i = 0; i < n; ++i)
+    if (runs[i].count > 0 && (runs[i].count < kKv4PrefillMin || runs[i].pos < 0)) {
+      few.push_back(runs[i]);
+      few_rows.push_back(rows[i]);
+    }
+  SI_TRY(kv4_pieces(
+      few.data(), few_rows.data(), (int)few.size(),
+      [&](const si::Kv4Runs &p, int tokens) -> si_status {
+        a.runs = p;
+        a.T = tokens;
+        long long keys = 0;
+        int longest = 0;
+        for (int i = 0; i < p.n; ++i) {
+          const int c = p.row0[i + 1] - p.row0[i];
+          keys += (long long)c * (p.pos[i] + 1) + (long long)c * (c - 1) / 2;
+          longest = std::max(longest, p.pos[i] + c);
+        }
+        a.nsplit = si::kv4_pick_splits(tokens, kv->d.n_kv_heads, keys, longest);
+        SI_TRY(ctx->kv4.reserve(si::kv4_part_floats(tokens, n_q_heads, D, a.nsplit) *
+                                sizeof(float)));
+        a.part = static_cast<float *>(ctx->kv4.p);
+        SI_CUDA(si::launch_attention_kv4(a, ctx->stream));
+        return SI_OK;
+      }));
+  for (int i = 0; i < n; ++i) {
+    if (runs[i].count < kKv4PrefillMin || runs[i].pos < 0) continue;
+    const int L = runs[i].pos + runs[i].count;
+    si::AttnArgs aa{};
+    aa.q = q + rows[i] * row;
+    aa.T = runs[i].count;
+    aa.n_q_heads = n_q_heads;
+    aa.n_kv_heads = kv->d.n_kv_heads;
+    aa.head_dim = D;
+    aa.max_ctx = L;
+    aa.ctx0 = runs[i].pos + 1;
+    aa.out = out + rows[i] * row;
+    aa.err = ctx->err;
+    aa.nsplit = 1;
+    if (!ctx->exact_attention && si::attn_tc_supported(aa)) {
+      // Tensor cores: the operand splits straight from the pages.
+      aa.kv4 = &a.kv;
+      aa.seq0 = runs[i].seq;
+      SI_TRY(ctx->attn.reserve(si::attn_tc_scratch_bytes(aa)));
+      SI_CUDA(si::launch_attention_tc(aa, ctx->attn.p, ctx->attn.bytes, ctx->stream));
+    } else {
+      // The fp32 kernel over the run's keys unpacked to an fp32 cache.
+      const size_t kvd = (size_t)kv->d.n_kv_heads * D;
+      SI_TRY(ctx->kv4.reserve(2 * L * kvd * sizeof(float)));
+      float *kf = static_cast<float *>(ctx->kv4.p), *vf = kf + L * kvd;
+      const si_kv4_run all{runs[i].seq, 0, L};
+      SI_TRY(kv4_read(ctx, kv, &all, 1, kf, vf));
+      aa.kc = kf;
+      aa.vc = vf;
+      aa.kv_f32 = 1;
+      SI_CUDA(si::launch_attention(aa, ctx->stream));
+    }
+  }
+  return SI_OK;
+}
+
+extern "C" SI_API si_status si_attention_kv4_dev(si_ctx *ctx, si_kv4 *kv, const si_dims *d,
+                                                 const float *q, const si_kv4_run *runs, int n,
+                                                 float *out) {
+  return kv4_entry([&]() -> si_status {
+    SI_TRY(kv4_check(ctx, kv));
+    SI_TRY(check_dims(d));
+    SI_CHECK(kv->d.n_kv_heads == d->n_kv_heads && kv->d.head_dim == d->head_dim,
+             "KV cache dims do not match");
+    int T = 0;
+    SI_TRY(kv4_count(runs, n, &T));
+    if (T == 0) return SI_OK;
+    SI_CHECK(q && out, "null q or out");
+    SI_CHECK(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
+             "q and out must be 16-byte aligned");
+    SI_TRY(kv4_covered(kv, runs, n, -1));
+    return kv4_attend(ctx, kv, d->n_q_heads, q, runs, n, T, nullptr, out);
+  });
+}
+
+// ----------------------------------------------------------------------------
 // layer schedules
 // ----------------------------------------------------------------------------
 namespace {
@@ -1238,19 +1793,31 @@ constexpr long kFuseRopeMaxCtas = 128;
 static si_status run_step(si_ctx *ctx, si_layer *l, si_kv *kv, const float *x, int T,
                           const int *seq_host, const int *ctx_host, int seq0, int prefix,
                           float *y, int mode, const si_captures *cap, bool timing,
-                          si_tp *tp = nullptr, const si_decode_state *st = nullptr) {
+                          si_tp *tp = nullptr, const si_decode_state *st = nullptr,
+                          si_kv4 *kv4 = nullptr, const si_kv4_run *runs = nullptr,
+                          int n_runs = 0) {
   const si_dims &d = l->d;
   const int H = d.hidden, QD = d.n_q_heads * d.head_dim, KVD = d.n_kv_heads * d.head_dim;
   SI_CHECK(mode == SI_LAYER_ATTN || mode == SI_LAYER_FULL, "bad layer mode");
   SI_CHECK(mode == SI_LAYER_ATTN || (d.intermediate > 0 && l->gate),
            "full-layer mode needs MLP weights");
-  SI_CHECK(kv->d.n_kv_heads == d.n_kv_heads && kv->d.head_dim == d.head_dim,
+  const si_dims &kd = kv4 ? kv4->d : kv->d;
+  SI_CHECK(kd.n_kv_heads == d.n_kv_heads && kd.head_dim == d.head_dim,
            "KV cache dims do not match the layer");
   SI_CHECK(ctx->head_dim == d.head_dim, "context RoPE table built for head_dim %d",
            ctx->head_dim);
   SI_CHECK(T > 0 && x && y, "bad step arguments");
   int max_len = 0;
-  if (st) {
+  if (kv4) {
+    SI_CHECK(!st || (st->ctx == ctx && T == st->batch && st->max_ctx == kv4->max_ctx &&
+                     kv4->max_ctx <= ctx->max_positions),
+             "decode state does not match this context, batch or cache");
+    for (int i = 0; i < n_runs; ++i)
+      SI_CHECK(runs[i].count <= 0 ||
+                   (int64_t)runs[i].pos + runs[i].count <= ctx->max_positions,
+               "positions past the context's %d", ctx->max_positions);
+    if (!st) SI_TRY(kv4_writable(ctx, kv4, runs, n_runs));
+  } else if (st) {
     // Lengths are on the device: the kernels bound every position by the
     // cache (rope_kv appends nothing past it, attention clamps), and the
     // split count covers the whole cache.
@@ -1272,7 +1839,7 @@ static si_status run_step(si_ctx *ctx, si_layer *l, si_kv *kv, const float *x, i
     max_len = prefix + T;
   }
   const bool decode_form = ctx_host != nullptr || st != nullptr;
-  const int nsplit = si::attn_pick_splits(T, decode_form, max_len);
+  const int nsplit = kv4 ? 1 : si::attn_pick_splits(T, decode_form, max_len);
   SI_TRY(ctx->work.reserve(step_bytes(d, T, nsplit, true)));
   StepBuffers b = carve(ctx->work.p, d, T, nsplit);
   cudaStream_t s = ctx->stream;
@@ -1335,52 +1902,62 @@ static si_status run_step(si_ctx *ctx, si_layer *l, si_kv *kv, const float *x, i
   if (cap && cap->qkv)
     SI_CUDA(cudaMemcpyAsync(cap->qkv, b.qkv, (size_t)T * (QD + 2 * KVD) * 4,
                             cudaMemcpyDeviceToDevice, s));
-  // 3. RoPE on q and k, KV append (qwen_one_layer.c:260-266).  A decode step
-  // (one token per sequence) with a small attention grid leaves both to the
-  // attention kernel, which then reads the raw projections: one kernel fewer
-  // (a 7B layer at batch 1, 68 CTAs: 63.1 -> 62.1 us per token).  Larger
-  // grids keep the separate kernel: every CTA's query fill then waits on the
-  // raw projections and the RoPE tables, which cost more than the launch it
-  // saves (a TP = 8 shard step at batch 8, 280 CTAs: +11 us per 8 layers; a
-  // 72B step at batch 8, 2112 CTAs: +12 us per layer).
-  const bool fuse_rope = (seq_host || st) && !cap && !timing &&
-                         kv->max_ctx <= ctx->max_positions &&
-                         (long)nsplit * d.n_kv_heads * T <= kFuseRopeMaxCtas;
-  si::RopeKvArgs ra{};
-  ra.qkv = b.qkv; ra.q_out = b.qrot; ra.kc = kv->k; ra.vc = kv->v; ra.kv_f32 = kv->kv_f32;
-  ra.T = T; ra.n_q_heads = d.n_q_heads; ra.n_kv_heads = d.n_kv_heads; ra.head_dim = d.head_dim;
-  ra.max_ctx = kv->max_ctx; ra.tok_pos = b.tok_pos; ra.tok_seq = b.tok_seq;
-  ra.seq0 = seq0; ra.pos0 = prefix; ra.cos_tab = ctx->cos_tab; ra.sin_tab = ctx->sin_tab;
-  ra.max_positions = ctx->max_positions;
-  if (!fuse_rope) SI_CUDA(si::launch_rope_kv(ra, s));
-  if (timing) SI_CUDA(cudaEventRecord(ctx->ev[EV_ROPE], s));
-  // 4. GQA attention (qwen_one_layer.c:269; causal for prefill).
-  si::AttnArgs aa{};
-  aa.q = b.qrot; aa.kc = kv->k; aa.vc = kv->v; aa.kv_f32 = kv->kv_f32; aa.T = T;
-  aa.n_q_heads = d.n_q_heads; aa.n_kv_heads = d.n_kv_heads; aa.head_dim = d.head_dim;
-  aa.max_ctx = kv->max_ctx; aa.tok_seq = b.tok_seq; aa.tok_ctx = b.tok_ctx; aa.seq0 = seq0;
-  aa.ctx0 = prefix + 1; aa.out = b.attn; aa.part = b.part; aa.nsplit = nsplit;
-  aa.err = ctx->err;
-  if (fuse_rope) {
-    aa.q = nullptr;
-    aa.qkv = b.qkv;
-    aa.cos_tab = ctx->cos_tab;
-    aa.sin_tab = ctx->sin_tab;
-  }
-  // 5. Q8 of the attention output (qwen_one_layer.c:272): in the decode form
-  // the attention kernel that writes each output row quantises it too.
   bool q8_done = false;
-  if (!ctx->exact_attention && si::attn_tc_supported(aa)) {
-    const size_t need = si::attn_tc_scratch_bytes(aa);
-    SI_TRY(ctx->attn.reserve(need));
-    SI_CUDA(si::launch_attention_tc(aa, ctx->attn.p, ctx->attn.bytes, s));
+  if (kv4) {
+    // 3, 4. The same two steps over the 4-bit cache: queries rotated, keys
+    // rotated and quantised into their pages, then the attention.
+    SI_TRY(kv4_rope_append(ctx, kv4, d, b.qkv, T, runs, n_runs, st ? st->idx + 2 * T : nullptr,
+                           b.qrot));
+    if (timing) SI_CUDA(cudaEventRecord(ctx->ev[EV_ROPE], s));
+    SI_TRY(kv4_attend(ctx, kv4, d.n_q_heads, b.qrot, runs, n_runs, T,
+                      st ? st->idx + 2 * T : nullptr, b.attn));
   } else {
-    if (si::attn_decode_form(aa)) {
-      aa.q8_qs = b.aq;
-      aa.q8_d = b.ad;
-      q8_done = true;
+    // 3. RoPE on q and k, KV append (qwen_one_layer.c:260-266).  A decode step
+    // (one token per sequence) with a small attention grid leaves both to the
+    // attention kernel, which then reads the raw projections: one kernel fewer
+    // (a 7B layer at batch 1, 68 CTAs: 63.1 -> 62.1 us per token).  Larger
+    // grids keep the separate kernel: every CTA's query fill then waits on the
+    // raw projections and the RoPE tables, which cost more than the launch it
+    // saves (a TP = 8 shard step at batch 8, 280 CTAs: +11 us per 8 layers; a
+    // 72B step at batch 8, 2112 CTAs: +12 us per layer).
+    const bool fuse_rope = (seq_host || st) && !cap && !timing &&
+                           kv->max_ctx <= ctx->max_positions &&
+                           (long)nsplit * d.n_kv_heads * T <= kFuseRopeMaxCtas;
+    si::RopeKvArgs ra{};
+    ra.qkv = b.qkv; ra.q_out = b.qrot; ra.kc = kv->k; ra.vc = kv->v; ra.kv_f32 = kv->kv_f32;
+    ra.T = T; ra.n_q_heads = d.n_q_heads; ra.n_kv_heads = d.n_kv_heads; ra.head_dim = d.head_dim;
+    ra.max_ctx = kv->max_ctx; ra.tok_pos = b.tok_pos; ra.tok_seq = b.tok_seq;
+    ra.seq0 = seq0; ra.pos0 = prefix; ra.cos_tab = ctx->cos_tab; ra.sin_tab = ctx->sin_tab;
+    ra.max_positions = ctx->max_positions;
+    if (!fuse_rope) SI_CUDA(si::launch_rope_kv(ra, s));
+    if (timing) SI_CUDA(cudaEventRecord(ctx->ev[EV_ROPE], s));
+    // 4. GQA attention (qwen_one_layer.c:269; causal for prefill).
+    si::AttnArgs aa{};
+    aa.q = b.qrot; aa.kc = kv->k; aa.vc = kv->v; aa.kv_f32 = kv->kv_f32; aa.T = T;
+    aa.n_q_heads = d.n_q_heads; aa.n_kv_heads = d.n_kv_heads; aa.head_dim = d.head_dim;
+    aa.max_ctx = kv->max_ctx; aa.tok_seq = b.tok_seq; aa.tok_ctx = b.tok_ctx; aa.seq0 = seq0;
+    aa.ctx0 = prefix + 1; aa.out = b.attn; aa.part = b.part; aa.nsplit = nsplit;
+    aa.err = ctx->err;
+    if (fuse_rope) {
+      aa.q = nullptr;
+      aa.qkv = b.qkv;
+      aa.cos_tab = ctx->cos_tab;
+      aa.sin_tab = ctx->sin_tab;
     }
-    SI_CUDA(si::launch_attention(aa, s));
+    // 5. Q8 of the attention output (qwen_one_layer.c:272): in the decode form
+    // the attention kernel that writes each output row quantises it too.
+    if (!ctx->exact_attention && si::attn_tc_supported(aa)) {
+      const size_t need = si::attn_tc_scratch_bytes(aa);
+      SI_TRY(ctx->attn.reserve(need));
+      SI_CUDA(si::launch_attention_tc(aa, ctx->attn.p, ctx->attn.bytes, s));
+    } else {
+      if (si::attn_decode_form(aa)) {
+        aa.q8_qs = b.aq;
+        aa.q8_d = b.ad;
+        q8_done = true;
+      }
+      SI_CUDA(si::launch_attention(aa, s));
+    }
   }
   if (timing) SI_CUDA(cudaEventRecord(ctx->ev[EV_ATTN], s));
   if (!q8_done) SI_CUDA(si::launch_q8_quantize(b.attn, T, QD, b.aq, b.ad, s));
@@ -1543,6 +2120,44 @@ extern "C" SI_API si_status si_prefill_dev(si_ctx *ctx, si_layer *l, si_kv *kv, 
   SI_TRY(set_device(ctx));
   SI_CHECK(l && kv, "null argument");
   return run_step(ctx, l, kv, x, ntok, nullptr, nullptr, seq, prefix, y, mode, nullptr, false);
+}
+
+// Rows of a list of runs (validated by the caller's checks later on).
+static si_status run_rows(const si_kv4_run *runs, int n, int *T) {
+  SI_CHECK(runs && n > 0, "no runs");
+  int64_t rows = 0;
+  for (int i = 0; i < n; ++i) {
+    SI_CHECK(runs[i].count >= 0, "negative token count");
+    rows += runs[i].count;
+  }
+  SI_CHECK(rows > 0 && rows <= (1 << 22), "step of %lld tokens", (long long)rows);
+  *T = (int)rows;
+  return SI_OK;
+}
+
+extern "C" SI_API si_status si_step_kv4_dev(si_ctx *ctx, si_layer *l, si_kv4 *kv, const float *x,
+                                            const si_kv4_run *runs, int n, float *y, int mode) {
+  return kv4_entry([&]() -> si_status {
+    SI_TRY(set_device(ctx));
+    SI_CHECK(l && kv && kv->ctx == ctx, "null argument, or a cache of another context");
+    int T = 0;
+    SI_TRY(run_rows(runs, n, &T));
+    return run_step(ctx, l, nullptr, x, T, nullptr, nullptr, 0, 0, y, mode, nullptr, false,
+                    nullptr, nullptr, kv, runs, n);
+  });
+}
+
+extern "C" SI_API si_status si_decode_step_state_kv4_dev(si_ctx *ctx, si_layer *l, si_kv4 *kv,
+                                                         const float *x, si_decode_state *st,
+                                                         float *y, int mode) {
+  return kv4_entry([&]() -> si_status {
+    SI_TRY(set_device(ctx));
+    SI_CHECK(l && kv && kv->ctx == ctx && st, "null argument, or a cache of another context");
+    SI_CHECK(st->batch <= kv->pages->n_seqs(), "batch %d exceeds the cache's %d sequences",
+             st->batch, kv->pages->n_seqs());
+    return run_step(ctx, l, nullptr, x, st->batch, nullptr, nullptr, 0, 0, y, mode, nullptr, false,
+                    nullptr, st, kv);
+  });
 }
 
 // Host-pointer forms: x and y are staged through two context-owned device

@@ -186,6 +186,9 @@ struct AttnArgs {
   // RoPE of rope_kv.cu, the same tables), so no separate RoPE kernel runs.
   const float *qkv;
   const float *cos_tab, *sin_tab;  // [positions][D/2]
+  // Tensor-core prefill form only: the 4-bit cache that holds sequence seq0,
+  // instead of kc and vc.
+  const struct Kv4View *kv4;
 };
 size_t attn_part_floats(int T, int n_q_heads, int head_dim, int nsplit);
 // Splits the launch needs: 1 when the prefill kernel runs (contiguous tokens
@@ -203,6 +206,79 @@ bool attn_tc_supported(const AttnArgs &a);
 size_t attn_tc_scratch_bytes(const AttnArgs &a);
 cudaError_t launch_attention_tc(const AttnArgs &a, void *scratch, size_t scratch_bytes,
                                 cudaStream_t s);
+
+// ---- kv4.cu, attention_kv4.cu (paged KV cache in 4 bits; layout in kv4.cu) -----
+constexpr int kKv4Group = 16;  // positions per contiguous group
+__host__ __device__ constexpr int kv4_group_bytes(int D) {
+  return kKv4Group * 2 * (D / 2 + D / 32 * 2);
+}
+struct Kv4View {
+  uint8_t *pool;
+  const int *tables;  // [n_seqs][max_pages] page of each stretch of page_len positions, or -1
+  const int *refs;    // [n_pages] table entries that hold the page
+  int n_pages, page_len, n_kv_heads, head_dim, n_seqs, max_pages;
+};
+// Ragged tokens by value: run i is rows [row0[i], row0[i + 1]) of the call's
+// row-wise tensors, at positions pos[i], pos[i] + 1, ... of sequence seq[i].
+constexpr int kKv4MaxRuns = 256;
+struct Kv4Runs {
+  int n;
+  int seq[kKv4MaxRuns], pos[kKv4MaxRuns], row0[kKv4MaxRuns + 1];
+};
+struct Kv4AppendArgs {
+  Kv4View kv;
+  Kv4Runs runs;          // used without tok_ctx
+  const int *tok_ctx;    // device context lengths: token t is position tok_ctx[t] - 1 of sequence t
+  int T;
+  const float *k, *v;    // rows [.][Hkv * D], ldkv floats apart
+  size_t ldkv;
+  const float *q;        // with q_out: query rows, ldq floats apart, rotated into q_out [.][Hq][D]
+  size_t ldq;
+  float *q_out;
+  int n_q_heads;
+  const float *cos_tab, *sin_tab;  // rotate K (and q) by position, or null
+  int max_positions;
+  int *err;
+};
+cudaError_t launch_kv4_append(const Kv4AppendArgs &a, cudaStream_t s);
+struct Kv4ReadArgs {
+  Kv4View kv;
+  Kv4Runs runs;
+  int T;
+  float *k, *v;  // [.][Hkv][D] fp32, either may be null
+  int *err;
+};
+cudaError_t launch_kv4_read(const Kv4ReadArgs &a, cudaStream_t s);
+// word: n_table pairs (entry, page), n_refs pairs (page, count), n_copies
+// pairs (from, to), taken when the launch is queued.  The small form keeps a
+// decode step's few entries from carrying 28 KB of kernel parameters.
+constexpr int kKv4SmallPairs = 240, kKv4LargePairs = 3584;
+template <int PAIRS>
+struct Kv4Update {
+  int *tables, *refs;
+  uint8_t *pool;
+  size_t page_bytes;
+  int n_table, n_refs, n_copies;
+  int word[2 * PAIRS];
+};
+cudaError_t launch_kv4_update(const Kv4Update<kKv4SmallPairs> &u, cudaStream_t s);
+cudaError_t launch_kv4_update(const Kv4Update<kKv4LargePairs> &u, cudaStream_t s);
+struct Kv4AttnArgs {
+  Kv4View kv;
+  Kv4Runs runs;        // used without tok_ctx; token j of run i attends positions [0, pos[i] + j]
+  const int *tok_ctx;  // device context lengths of sequences 0 .. T-1
+  int T, n_q_heads;
+  const float *q;      // rows [.][Hq][D]
+  float *out;          // rows [.][Hq][D]
+  int nsplit;          // kv4_pick_splits()
+  float *part;         // kv4_part_floats() of device memory when nsplit > 1
+  int *err;
+};
+// Splits of the key axis for T tokens that attend `keys` keys in all, `longest`
+// of them the most.
+int kv4_pick_splits(int T, int n_kv_heads, long long keys, int longest);
+size_t kv4_part_floats(int T, int n_q_heads, int head_dim, int nsplit);
+cudaError_t launch_attention_kv4(const Kv4AttnArgs &a, cudaStream_t s);
 
 // ---- tp_peer.cu --------------------------------------------------------------
 // y[i] = resid[i] + sum over ranks (in rank order) of the receive slots of

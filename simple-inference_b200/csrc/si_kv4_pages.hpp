@@ -1,0 +1,272 @@
+// si_kv4_pages.hpp -- host bookkeeping of the paged KV cache: which page holds
+// which positions of which sequence, how many sequences hold a page, and which
+// pages are free.  Plain C++ without CUDA; the C ABI (si_api.cu) queues what
+// each change asks of the device (table entries, reference counts, page
+// copies) on the context's stream.
+//
+// Every change is checked in full before anything is touched, so a refused
+// call leaves the tables as they were.  Free pages are handed out lowest first.
+#pragma once
+#include <stdint.h>
+
+#include <algorithm>
+#include <string>
+#include <utility>
+#include <vector>
+
+namespace si {
+
+struct Kv4Run {  // `count` consecutive tokens of sequence seq from position pos on
+  int seq, pos, count;
+};
+
+// What a change asks of the device.  Copies never chain: no destination of a
+// change is a source of the same change, and no destination occurs twice.
+struct Kv4Edits {
+  std::vector<std::pair<int, int>> table;  // (entry, page)
+  std::vector<int> touched;                // pages whose reference count changed
+  std::vector<std::pair<int, int>> copies; // (from page, to page)
+  void clear() {
+    table.clear();
+    touched.clear();
+    copies.clear();
+  }
+};
+
+class Kv4Pages {
+ public:
+  Kv4Pages(int n_seqs, int max_pages, int n_pages, int page_len)
+      : n_seqs_(n_seqs), max_pages_(max_pages), page_len_(page_len), n_free_(n_pages),
+        count_(n_seqs, 0), refs_(n_pages, 0),
+        table_((size_t)n_seqs * max_pages, -1) {}
+
+  int n_pages() const { return (int)refs_.size(); }
+  int n_seqs() const { return n_seqs_; }
+  int max_pages() const { return max_pages_; }
+  int page_len() const { return page_len_; }
+  int free_pages() const { return n_free_; }
+  int count(int seq) const { return count_[seq]; }
+  int refs(int page) const { return refs_[page]; }
+  int page(int seq, int i) const { return table_[at(seq, i)]; }
+  const std::string &why() const { return why_; }
+  // Positions of seq that its pages cover.
+  int64_t covered(int seq) const { return (int64_t)count_[seq] * page_len_; }
+
+  // Runs within the cache's sequences and positions.
+  bool runs_ok(const Kv4Run *runs, int n) {
+    for (int i = 0; i < n; ++i) {
+      if (!seq_ok(runs[i].seq)) return false;
+      if (runs[i].pos < 0 || runs[i].count < 0 ||
+          (int64_t)runs[i].pos + runs[i].count > (int64_t)max_pages_ * page_len_)
+        return no("positions outside the cache's max_ctx");
+    }
+    return true;
+  }
+
+  // Every page that the runs write to is there and held by their sequence alone.
+  bool writable(const Kv4Run *runs, int n) const {
+    for (int i = 0; i < n; ++i) {
+      const Kv4Run &x = runs[i];
+      if (x.count <= 0) continue;
+      const int p1 = last_page(x);
+      if (p1 >= count_[x.seq]) return false;
+      for (int p = x.pos / page_len_; p <= p1; ++p)
+        if (refs_[table_[at(x.seq, p)]] > 1) return false;
+    }
+    return true;
+  }
+
+  bool seq_ok(int seq) { return (seq >= 0 && seq < n_seqs_) || no("sequence out of range"); }
+
+  // Positions [pos, pos + count) of every run get pages that no other
+  // sequence holds: missing pages (from the sequence's first missing one) are
+  // taken, a shared page is replaced by a copy of it.
+  bool reserve(const Kv4Run *runs, int n, Kv4Edits *e) {
+    if (!runs_ok(runs, n)) return false;
+    if (writable(runs, n)) return true;  // the common decode step
+    std::vector<Kv4Run> r;
+    for (int i = 0; i < n; ++i)
+      if (runs[i].count > 0) r.push_back(runs[i]);
+    // A dry run that counts the pages taken.  Of a page's holders the ones that
+    // write get copies, except that the last holder left keeps the page.
+    std::vector<int> have(count_);
+    int64_t need = 0;
+    std::vector<std::pair<int, int>> shared;  // (page, table entry), each pair once
+    for (const Kv4Run &x : r) {
+      const int p0 = x.pos / page_len_, p1 = last_page(x);
+      for (int p = p0; p < std::min(p1 + 1, count_[x.seq]); ++p) {
+        const int pg = table_[at(x.seq, p)];
+        if (refs_[pg] > 1) shared.push_back({pg, (int)at(x.seq, p)});
+      }
+      if (p1 + 1 > have[x.seq]) {
+        need += p1 + 1 - have[x.seq];
+        have[x.seq] = p1 + 1;
+      }
+    }
+    std::sort(shared.begin(), shared.end());
+    shared.erase(std::unique(shared.begin(), shared.end()), shared.end());
+    for (size_t i = 0; i < shared.size();) {
+      size_t j = i;
+      while (j < shared.size() && shared[j].first == shared[i].first) ++j;
+      need += std::min((int64_t)(j - i), (int64_t)refs_[shared[i].first] - 1);
+      i = j;
+    }
+    if (need > n_free_) return no("not enough free pages");
+    for (const Kv4Run &x : r) {
+      const int p0 = x.pos / page_len_, p1 = last_page(x);
+      for (int p = p0; p < std::min(p1 + 1, count_[x.seq]); ++p) {
+        const int old = table_[at(x.seq, p)];
+        if (refs_[old] <= 1) continue;
+        const int pg = take(e);
+        e->copies.push_back({old, pg});
+        drop(old, e);
+        put(x.seq, p, pg, e);
+      }
+      for (int p = count_[x.seq]; p <= p1; ++p) put(x.seq, p, take(e), e);
+      count_[x.seq] = std::max(count_[x.seq], p1 + 1);
+    }
+    return true;
+  }
+
+  // Sequence seqs[i] (empty until now) holds the next counts[i] pages of the
+  // list, each of which may be held by others already.
+  bool assign(const int *seqs, const int *counts, int n, const int *pages, Kv4Edits *e) {
+    std::vector<char> seen(n_seqs_, 0);
+    int64_t total = 0;
+    for (int i = 0; i < n; ++i) {
+      if (!seq_ok(seqs[i])) return false;
+      if (count_[seqs[i]] || seen[seqs[i]]) return no("sequence already holds pages");
+      if (counts[i] < 0 || counts[i] > max_pages_) return no("page count out of range");
+      seen[seqs[i]] = 1;
+      total += counts[i];
+    }
+    for (int64_t i = 0; i < total; ++i)
+      if (pages[i] < 0 || pages[i] >= n_pages()) return no("page out of range");
+    for (int i = 0; i < n; ++i) {
+      for (int p = 0; p < counts[i]; ++p) {
+        const int pg = *pages++;
+        if (refs_[pg] == 0) --n_free_;
+        hold(pg, e);
+        put(seqs[i], p, pg, e);
+      }
+      count_[seqs[i]] = counts[i];
+    }
+    return true;
+  }
+
+  // dst[i] (empty until now) begins with the first lens[i] positions of
+  // src[i]: whole pages are shared, the page that lens[i] ends in is copied.
+  bool fork(const int *src, const int *dst, const int *lens, int n, Kv4Edits *e) {
+    std::vector<char> seen(n_seqs_, 0);
+    int64_t need = 0;
+    for (int i = 0; i < n; ++i) {
+      if (!seq_ok(src[i]) || !seq_ok(dst[i])) return false;
+      if (count_[dst[i]] || seen[dst[i]]) return no("destination sequence already holds pages");
+      if (src[i] == dst[i]) return no("a sequence cannot be forked into itself");
+      if (lens[i] < 0 || lens[i] > covered(src[i])) return no("length beyond the source's pages");
+      seen[dst[i]] = 1;
+      need += lens[i] % page_len_ != 0;
+    }
+    if (need > n_free_) return no("not enough free pages");
+    for (int i = 0; i < n; ++i) {
+      const int whole = lens[i] / page_len_;
+      for (int p = 0; p < whole; ++p) {
+        const int pg = table_[at(src[i], p)];
+        hold(pg, e);
+        put(dst[i], p, pg, e);
+      }
+      count_[dst[i]] = whole;
+      if (lens[i] % page_len_) {
+        const int pg = take(e);
+        e->copies.push_back({table_[at(src[i], whole)], pg});
+        put(dst[i], whole, pg, e);
+        count_[dst[i]] = whole + 1;
+      }
+    }
+    return true;
+  }
+
+  // seqs[i] keeps the pages of its first keep[i] positions (keep null: none).
+  bool release(const int *seqs, const int *keep, int n, Kv4Edits *e) {
+    for (int i = 0; i < n; ++i) {
+      if (!seq_ok(seqs[i])) return false;
+      if (keep && keep[i] < 0) return no("negative length");
+    }
+    for (int i = 0; i < n; ++i) {
+      const int64_t len = keep ? keep[i] : 0;
+      const int64_t stay = (len + page_len_ - 1) / page_len_;
+      for (int p = count_[seqs[i]] - 1; p >= stay; --p) {
+        drop(table_[at(seqs[i], p)], e);
+        put(seqs[i], p, -1, e);
+      }
+      count_[seqs[i]] = (int)std::min<int64_t>(count_[seqs[i]], stay);
+    }
+    return true;
+  }
+
+  // The used pages become pages [0, used): the used pages from `used` on move,
+  // in ascending order, to the free ones below.  Returns used.
+  int compact(Kv4Edits *e) {
+    const int used = n_pages() - n_free_;
+    std::vector<int> to(refs_.size(), -1);
+    int hole = 0;
+    for (int pg = used; pg < n_pages(); ++pg) {
+      if (!refs_[pg]) continue;
+      while (refs_[hole]) ++hole;
+      to[pg] = hole;
+      refs_[hole] = refs_[pg];
+      refs_[pg] = 0;
+      e->copies.push_back({pg, hole});
+      e->touched.push_back(pg);
+      e->touched.push_back(hole);
+      ++hole;
+    }
+    if (!e->copies.empty())
+      for (int s = 0; s < n_seqs_; ++s)
+        for (int p = 0; p < count_[s]; ++p) {
+          const int pg = table_[at(s, p)];
+          if (to[pg] >= 0) put(s, p, to[pg], e);
+        }
+    first_free_ = used;
+    return used;
+  }
+
+ private:
+  size_t at(int seq, int p) const { return (size_t)seq * max_pages_ + p; }
+  int last_page(const Kv4Run &x) const {
+    return (int)(((int64_t)x.pos + x.count - 1) / page_len_);
+  }
+  bool no(const char *why) {
+    why_ = why;
+    return false;
+  }
+  int take(Kv4Edits *e) {  // the lowest free page; the caller has checked that there is one
+    while (refs_[first_free_]) ++first_free_;
+    const int pg = first_free_++;
+    --n_free_;
+    hold(pg, e);
+    return pg;
+  }
+  void hold(int pg, Kv4Edits *e) {
+    ++refs_[pg];
+    e->touched.push_back(pg);
+  }
+  void drop(int pg, Kv4Edits *e) {
+    if (--refs_[pg] == 0) {
+      ++n_free_;
+      first_free_ = std::min(first_free_, pg);
+    }
+    e->touched.push_back(pg);
+  }
+  void put(int seq, int p, int pg, Kv4Edits *e) {
+    table_[at(seq, p)] = pg;
+    e->table.push_back({(int)at(seq, p), pg});
+  }
+
+  int n_seqs_, max_pages_, page_len_, n_free_;
+  int first_free_ = 0;  // no free page lies below
+  std::vector<int> count_, refs_, table_;
+  std::string why_;
+};
+
+}  // namespace si

@@ -143,6 +143,22 @@ def lib() -> C.CDLL:
         "si_decode_state_read": (i32, [vp, vp, vp]),
         "si_decode_step_state_dev": (i32, [vp, vp, vp, vp, vp, vp, i32]),
         "si_decode_step_state_tp_dev": (i32, [vp, vp, vp, vp, vp, vp, vp, i32]),
+        "si_kv4_page_bytes": (C.c_size_t, [C.POINTER(Dims), i32]),
+        "si_kv4_create": (i32, [vp, C.POINTER(Dims), i32, i32, i32, i32, vp, pp]),
+        "si_kv4_free": (None, [vp]),
+        "si_kv4_device_ptr": (vp, [vp, i32]),
+        "si_kv4_free_pages": (i32, [vp]),
+        "si_kv4_pages": (i32, [vp, i32, vp, i32]),
+        "si_kv4_reserve": (i32, [vp, vp, vp, i32]),
+        "si_kv4_assign": (i32, [vp, vp, vp, vp, i32, vp]),
+        "si_kv4_fork": (i32, [vp, vp, vp, vp, vp, i32]),
+        "si_kv4_release": (i32, [vp, vp, vp, vp, i32]),
+        "si_kv4_compact": (i32, [vp, vp, C.POINTER(C.c_int)]),
+        "si_kv4_append_dev": (i32, [vp, vp, vp, vp, vp, i32]),
+        "si_kv4_read_dev": (i32, [vp, vp, vp, i32, vp, vp]),
+        "si_attention_kv4_dev": (i32, [vp, vp, C.POINTER(Dims), vp, vp, i32, vp]),
+        "si_step_kv4_dev": (i32, [vp, vp, vp, vp, vp, i32, vp, i32]),
+        "si_decode_step_state_kv4_dev": (i32, [vp, vp, vp, vp, vp, vp, i32]),
         "si_graph_begin": (i32, [vp]),
         "si_graph_end": (i32, [vp, pp]),
         "si_graph_launch": (i32, [vp, vp]),
@@ -177,6 +193,27 @@ def _p(x):
     if hasattr(x, "data_ptr"):
         return x.data_ptr()
     return x.ctypes.data
+
+
+def _ints(x) -> np.ndarray:
+    """Whole numbers as a contiguous host int32 array (kept as it is when it is one)."""
+    a = np.asarray(x)
+    if a.dtype != np.int32:
+        if a.size == 0:
+            a = a.astype(np.int32)
+        elif a.dtype.kind not in "iu" or int(a.min()) < -2**31 or int(a.max()) >= 2**31:
+            raise ValueError("whole numbers of 32 bits are needed")
+    return np.ascontiguousarray(a, np.int32)
+
+
+def _runs(runs) -> np.ndarray:
+    """Runs (seq, pos, count) as a host int32 array [n, 3]."""
+    r = _ints(runs)
+    if r.size == 0:
+        return r.reshape(0, 3)
+    if r.ndim != 2 or r.shape[1] != 3:
+        raise ValueError("runs are rows of (seq, pos, count)")
+    return r
 
 
 class Context:
@@ -331,6 +368,27 @@ class Context:
         check(self.L.si_kv_create(self.h, C.byref(dm), batch, max_ctx, int(kv_f32), C.byref(h)),
               "si_kv_create")
         return KV(self, h, dims, batch, max_ctx, kv_f32)
+
+    def kv4(self, dims: dict, n_seqs: int, max_ctx: int, n_pages: int, page_len: int = 64,
+            pool=None) -> "KV4":
+        """Paged KV cache in 4 bits (see si_kv4_create); pool: device memory of
+        n_pages * kv4_page_bytes(dims, page_len) to use instead of its own."""
+        if pool is not None and hasattr(pool, "numel"):
+            have, need = pool.numel() * pool.element_size(), n_pages * kv4_page_bytes(dims, page_len)
+            if have < need or not pool.is_contiguous():
+                raise ValueError(f"pool: {have} bytes, {need} contiguous ones are needed")
+        dm = Dims.of(dims)
+        h = C.c_void_p()
+        check(self.L.si_kv4_create(self.h, C.byref(dm), n_seqs, max_ctx, n_pages, page_len,
+                                   _p(pool), C.byref(h)), "si_kv4_create")
+        return KV4(self, h, dims, n_seqs, max_ctx, n_pages, page_len, pool)
+
+    def attention_kv4(self, kv: "KV4", dims: dict, q, runs, out):
+        """Attention of the runs' query rows over a 4-bit cache (si_attention_kv4_dev)."""
+        dm = Dims.of(dims)
+        r = _runs(runs)
+        check(self.L.si_attention_kv4_dev(self.h, kv.h, C.byref(dm), _p(q), _p(r), len(r), _p(out)),
+              "si_attention_kv4_dev")
 
     def attention_prefill(self, kv: "KV", dims: dict, q, ntok, seq, prefix, out):
         dm = Dims.of(dims)
@@ -497,9 +555,21 @@ class Layer:
         check(self.ctx.L.si_decode_step_dev(self.ctx.h, self.h, kv.h, _p(x), len(ctx_lens),
                                             lens, _p(y), mode, None), "si_decode_step_dev")
 
-    def decode_state_dev(self, kv: "KV", x, state: "DecodeState", y, mode=SI_LAYER_ATTN):
+    def decode_state_dev(self, kv, x, state: "DecodeState", y, mode=SI_LAYER_ATTN):
+        if isinstance(kv, KV4):
+            check(self.ctx.L.si_decode_step_state_kv4_dev(self.ctx.h, self.h, kv.h, _p(x), state.h,
+                                                          _p(y), mode),
+                  "si_decode_step_state_kv4_dev")
+            return
         check(self.ctx.L.si_decode_step_state_dev(self.ctx.h, self.h, kv.h, _p(x), state.h,
                                                   _p(y), mode), "si_decode_step_state_dev")
+
+    def step_dev(self, kv: "KV4", x, runs, y, mode=SI_LAYER_ATTN):
+        """One step of the runs' tokens over a 4-bit cache: decode tokens, prompts
+        or both in one call (si_step_kv4_dev)."""
+        r = _runs(runs)
+        check(self.ctx.L.si_step_kv4_dev(self.ctx.h, self.h, kv.h, _p(x), _p(r), len(r), _p(y),
+                                         mode), "si_step_kv4_dev")
 
     def prefill(self, kv: "KV", seq, x_host, ntok, prefix, y_host, mode=SI_LAYER_ATTN):
         check(self.ctx.L.si_prefill(self.ctx.h, self.h, kv.h, seq, _p(x_host), ntok, prefix,
@@ -508,6 +578,12 @@ class Layer:
     def prefill_dev(self, kv: "KV", seq, x, ntok, prefix, y, mode=SI_LAYER_ATTN):
         check(self.ctx.L.si_prefill_dev(self.ctx.h, self.h, kv.h, seq, _p(x), ntok, prefix,
                                         _p(y), mode), "si_prefill_dev")
+
+
+def kv4_page_bytes(dims: dict, page_len: int) -> int:
+    """Bytes of one page of a 4-bit cache (host-only; no GPU needed)."""
+    dm = Dims.of(dims)
+    return int(lib().si_kv4_page_bytes(C.byref(dm), page_len))
 
 
 def tp_split(units: int, rank: int, world: int) -> tuple[int, int]:
@@ -582,6 +658,82 @@ class KV:
     def free(self):
         if self.h:
             self.ctx.L.si_kv_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class KV4:
+    """Paged KV cache in 4 bits (Context.kv4).  Runs are rows of (seq, pos, count)."""
+
+    def __init__(self, ctx: Context, h, dims, n_seqs, max_ctx, n_pages, page_len, pool):
+        self.ctx, self.h, self.dims = ctx, h, dims
+        self.n_seqs, self.max_ctx, self.n_pages, self.page_len = n_seqs, max_ctx, n_pages, page_len
+        self.pool = pool  # the caller's memory stays as long as the cache
+
+    def _call(self, name, *args):
+        check(getattr(self.ctx.L, name)(self.ctx.h, self.h, *args), name)
+
+    def device_ptr(self, which: int) -> int:
+        """0: the pool; 1: the device page tables (read only)."""
+        return self.ctx.L.si_kv4_device_ptr(self.h, which)
+
+    def free_pages(self) -> int:
+        return self.ctx.L.si_kv4_free_pages(self.h)
+
+    def pages(self, seq: int) -> list:
+        """The pages that a sequence holds, in order."""
+        n = self.ctx.L.si_kv4_pages(self.h, seq, None, 0)
+        if n < 0:
+            raise ValueError(f"sequence {seq} out of range")
+        out = np.zeros(n, np.int32)
+        self.ctx.L.si_kv4_pages(self.h, seq, _p(out), n)
+        return out.tolist()
+
+    def reserve(self, runs):
+        r = _runs(runs)
+        self._call("si_kv4_reserve", _p(r), len(r))
+
+    def assign(self, seqs, counts, pages):
+        s, c, p = _ints(seqs), _ints(counts), _ints(pages)
+        if s.size != c.size or int(c.sum(dtype=np.int64)) != p.size:
+            raise ValueError("one count per sequence, and as many pages as their sum")
+        self._call("si_kv4_assign", _p(s), _p(c), s.size, _p(p))
+
+    def fork(self, src, dst, lens):
+        s, d, n = _ints(src), _ints(dst), _ints(lens)
+        if not s.size == d.size == n.size:
+            raise ValueError("src, dst and lens differ in length")
+        self._call("si_kv4_fork", _p(s), _p(d), _p(n), s.size)
+
+    def release(self, seqs, keep=None):
+        s = _ints(seqs)
+        k = None if keep is None else _ints(keep)
+        if k is not None and k.size != s.size:
+            raise ValueError("seqs and keep differ in length")
+        self._call("si_kv4_release", _p(s), _p(k), s.size)
+
+    def compact(self) -> int:
+        """The used pages become the first ones of the pool; their number."""
+        used = C.c_int()
+        self._call("si_kv4_compact", C.byref(used))
+        return used.value
+
+    def append(self, k, v, runs):
+        r = _runs(runs)
+        self._call("si_kv4_append_dev", _p(k), _p(v), _p(r), len(r))
+
+    def read(self, runs, k_out, v_out):
+        r = _runs(runs)
+        self._call("si_kv4_read_dev", _p(r), len(r), _p(k_out), _p(v_out))
+
+    def free(self):
+        if self.h:
+            self.ctx.L.si_kv4_free(self.h)
             self.h = None
 
     def __del__(self):
