@@ -7,29 +7,42 @@
 //
 // Arithmetic.  Both contractions run on fp16 matrix instructions with fp32
 // accumulators, and no input is rounded to fewer than 22 bits:
-//   * a code n masked out of its word is the fp16 subnormal n 2^-24 (nibbles 0
-//     and 2) or n 2^-20 (nibbles 1 and 3) as it stands, so unpacking is one AND
-//     per two codes and a shift per eight; the powers of two go into the other
-//     operand or the result;
+//   * two codes n masked out of their word and ORed into the mantissa of 1024
+//     are the fp16 numbers 1024 + n (nibbles 0 and 2) or 1024 + 16 n (nibbles 1
+//     and 3); one packed subtraction leaves n - 8 or 16 (n - 8), exactly.  The 16
+//     goes into the other operand or the result.  (The masked word by itself,
+//     the subnormal n 2^-24, would save both steps, but the instruction aligns
+//     its products by the operands' nominal exponents and loses the low bits:
+//     2.5e-6 relative error against 2e-7.);
 //   * a query is scaled by a power of two so that its largest value is just
 //     below 2^15 and split into two halves, hi = fp16(q), lo = fp16(q - hi).
 //     The instruction has 16 rows and a KV group at most 8 heads: hi is rows
 //     0-7 and lo rows 8-15, whose results land in the same lane and are added,
 //     so the split costs no further instruction;
-//   * a block's sum of q (n - 8) is the instruction's sum of q n started at
-//     -8 sum q, then times d_k in fp32 and added to the score;
-//   * P.V: p d_v per block is the left operand, again as hi and lo rows, scaled
-//     by a power of two per warp that follows the largest |d_v| seen (so that a
-//     cache of small values keeps its bits); codes become n - 8 by one packed
-//     subtraction, exact in fp16;
+//   * a block's sum of q (n - 8) is multiplied by d_k in fp32 and added to the
+//     score;
+//   * P.V: p d_v per block is the left operand, again as hi and lo rows.  p is
+//     split once per key; the product's hi is the rounded fp16 product and its
+//     lo the exact remainder of that (a fused multiply-add) plus p_lo d_v.  Powers
+//     of two that follow the largest |d_v| seen keep both in range, so a cache of
+//     small values keeps its bits;
 //   * running maximum, sum and output are fp32 per warp, merged over the warps
-//     of the CTA and over splits at the end.
+//     of the CTA and over splits at the end.  The maximum is raised only by a
+//     score more than 2^4 above it, so probabilities stay below 16 and the
+//     output is rarely rescaled.
 //
 // Work split.  A CTA of four warps takes one (token, KV head, split of the
 // keys); a warp walks every fourth tile of 32 keys of its split on its own, its
 // tiles staged by cp.async into a private ring (a tile is two contiguous
 // groups of 16 positions with their scales), so there is no barrier between
-// the warps until the merge.
+// the warps until the merge.  The query operand is made once per CTA and read
+// from shared memory, which leaves registers for three CTAs per SM.
+//
+// Bound by instruction issue, not by the cache's bytes: a tile of 4608 bytes
+// takes about 800 instructions, of them 290 for unpacking the codes and 64
+// matrix instructions.
+#include <algorithm>
+
 #include "si_common.cuh"
 #include "si_kernels.cuh"
 #include "si_tma.cuh"
@@ -39,9 +52,11 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kTile = 2 * kKv4Group;       // keys per warp step
-constexpr int kSplitUnit = kWarps * kTile; // a split's keys are a multiple of this
-constexpr int kStages = 3;
+constexpr int kMinSplit = kWarps * kTile;  // a split has at least one tile per warp
+constexpr int kStages = 2;
 constexpr int kHeads = 8;                  // query heads of a KV group, at most
+constexpr int kCtasPerSm = 3;
+constexpr float kStaleMax = 4.0f;          // log2 units a score may lie above the maximum
 
 template <int D>
 struct Shape {
@@ -54,7 +69,9 @@ struct Shape {
   static constexpr int OROW = D + 4;                 // merge row, one 16-byte step of padding
   static constexpr int RING = kWarps * kStages * TILE;
   static constexpr int MERGE = kWarps * kHeads * (OROW + 2) * 4;
-  static constexpr int SMEM = RING > MERGE ? RING : MERGE;
+  static constexpr int Q = NB * 2 * 32 * 16;         // query operand
+  static constexpr int AMAX = NB * kHeads * 4;
+  static constexpr int SMEM = Q + AMAX + (RING > MERGE ? RING : MERGE);
 };
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x, relative error below 2^-22
@@ -71,6 +88,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]),
         "f"(c[3]));
 }
+__device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2 *>(&x); }
 __device__ __forceinline__ uint32_t h2bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 // (hi, lo) fp16 pairs of two floats: 22 significant bits together.
 __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
@@ -79,13 +97,24 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t 
   hi = h2bits(h);
   lo = h2bits(__floats2half2_rn(x - f.x, y - f.y));
 }
-__device__ __forceinline__ uint32_t sub_h2(uint32_t a, uint32_t b) {
-  const __half2 r = __hadd2(*reinterpret_cast<const __half2 *>(&a),
-                            *reinterpret_cast<const __half2 *>(&b));
-  return h2bits(r);
+// The codes of one nibble position of a word of four: n - 8 (low nibble of each
+// byte) or 16 (n - 8) (high nibble), two per register.  `one_k` is 1024 twice,
+// taken from the kernel's arguments: as a constant the compiler would mask and
+// OR in two steps, since an instruction holds one constant (72B, 131071 keys:
+// 66.2 -> 61.3 us).
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w, uint32_t one_k) {
+  uint32_t x;
+  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(x) : "r"(w), "r"(one_k));
+  return h2bits(__hsub2(as_h2(x), __half2half2(__ushort_as_half(0x6408))));
+}
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w, uint32_t one_k) {
+  uint32_t x;
+  asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xea;" : "=r"(x) : "r"(w), "r"(one_k));
+  return h2bits(__hsub2(as_h2(x), __half2half2(__ushort_as_half(0x6480))));
 }
 __device__ __forceinline__ float half_at(const uint32_t *w, int i) {
-  return f16_to_f32((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
+  const __half2 h = as_h2(w[i >> 1]);
+  return (i & 1) ? __high2float(h) : __low2float(h);
 }
 __device__ __forceinline__ float pow2(int e) {  // 2^e, 0 below the normal range
   return e < -126 ? 0.0f : __int_as_float((e + 127) << 23);
@@ -118,14 +147,35 @@ __device__ __forceinline__ Token token_of(const Kv4AttnArgs &a, int t) {
 // Keys per split of a token of `len` keys, and the splits it needs.
 __device__ __forceinline__ int split_keys(int len, int nsplit) {
   const int per = (len + nsplit - 1) / nsplit;
-  return (per + kSplitUnit - 1) / kSplitUnit * kSplitUnit;
+  return max(kMinSplit, (per + kTile - 1) / kTile * kTile);
+}
+// Two fp32 operations per instruction, each rounded on its own.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mov.b64 rc, {%6, %7};\n\tfma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
 }
 
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32, 3) k_attn_kv4(const __grid_constant__ Kv4AttnArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
+    k_attn_kv4(const __grid_constant__ Kv4AttnArgs a) {
   using S = Shape<D>;
   constexpr int NB = S::NB;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(16) uint8_t smem_all[];
+  uint4 *q_s = reinterpret_cast<uint4 *>(smem_all);                  // [NB][2][32 lanes]
+  float *amax_s = reinterpret_cast<float *>(smem_all + S::Q);        // [NB][8 heads]
+  uint8_t *smem = smem_all + S::Q + S::AMAX;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;  // operand row (head) and column group
   pdl_trigger();
@@ -184,58 +234,57 @@ __global__ void __launch_bounds__(kWarps * 32, 3) k_attn_kv4(const __grid_consta
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
 
-  // The query operand: head g's values of dims 32b + 8t + 0..7, scaled and split.
-  uint32_t aq[NB][2][4];
-  float cinit[NB];
+  // The query operand: head g's values of dims 32b + 8t + 0..7, scaled and
+  // split, block b by warp b.
   float sc;  // score in log2 units per unit of the accumulators
   {
-    float x[NB][8];
-    float amax = 0.0f;
-    const float *q = a.q + ((size_t)tk.row * a.n_q_heads + (size_t)kvh * G + g) * D + 8 * t;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
-      if (g < G) {
-        u = *reinterpret_cast<const float4 *>(q + 32 * b);
-        v = *reinterpret_cast<const float4 *>(q + 32 * b + 4);
-      }
-      x[b][0] = u.x; x[b][1] = u.y; x[b][2] = u.z; x[b][3] = u.w;
-      x[b][4] = v.x; x[b][5] = v.y; x[b][6] = v.z; x[b][7] = v.w;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[b][i]));
+    float x[8] = {};
+    if (warp < NB && g < G) {
+      const float *q = a.q + ((size_t)tk.row * a.n_q_heads + (size_t)kvh * G + g) * D + 32 * warp + 8 * t;
+      const float4 u = *reinterpret_cast<const float4 *>(q);
+      const float4 v = *reinterpret_cast<const float4 *>(q + 4);
+      x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+      x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
     }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const int e = min(127, 14 - ((int)(__float_as_uint(amax) >> 23) - 127));
+    if (warp < NB) {
+      float am = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) am = fmaxf(am, fabsf(x[i]));
+      am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
+      am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
+      if (t == 0) amax_s[warp * kHeads + g] = am;
+    }
+    __syncthreads();
+    float am = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) am = fmaxf(am, amax_s[b * kHeads + g]);
+    const int e = min(127, 14 - ((int)(__float_as_uint(am) >> 23) - 127));
     const float up = pow2(e);
-    sc = ldexpf(1.4426950408889634f / sqrtf((float)D), 24 - e);
+    sc = ldexpf(1.4426950408889634f / sqrtf((float)D), -e);
+    if (warp < NB) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        // k columns 2t, 2t+1: nibble 2s of the two half-words; 2t+8, 2t+9:
-        // nibble 2s + 1, whose codes carry 2^4 more.
-        const float x0 = x[b][2 * s] * up, x1 = x[b][2 * s + 4] * up;
-        const float y0 = x[b][2 * s + 1] * up, y1 = x[b][2 * s + 5] * up;
-        split2(x0, x1, aq[b][s][0], aq[b][s][1]);
-        split2(y0 * 0.0625f, y1 * 0.0625f, aq[b][s][2], aq[b][s][3]);
-        sum += (x0 + x1) + (y0 + y1);
+      for (int i = 0; i < 2; ++i) {
+        // k columns 2t, 2t+1: nibble 2i of the two half-words; 2t+8, 2t+9:
+        // nibble 2i + 1, whose codes come 16-fold.
+        uint4 f;
+        split2(x[2 * i] * up, x[2 * i + 4] * up, f.x, f.y);
+        split2(x[2 * i + 1] * up * 0.0625f, x[2 * i + 5] * up * 0.0625f, f.z, f.w);
+        q_s[(warp * 2 + i) * 32 + lane] = f;
       }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      cinit[b] = sum * (-8.0f / 16777216.0f);
     }
+    __syncthreads();
   }
 
+  const uint32_t one_k = a.one_k;
   float acc[NB * 4][4];
 #pragma unroll
   for (int i = 0; i < NB * 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
   float m = -INFINITY, l = 0.0f;
-  int eR = -1000;  // P.V operands are p d_v 2^(13 - eR)
-  float up_v = 0.0f;
+  // P.V operands are (p 2^sp) (d_v 2^dexp) for |d_v| < 2^(eR + 1); both factors
+  // and the product stay below 2^15.
+  int eR = -1000, sp = 0, dexp = 0;
 
   for (int n = 0; n < mine; ++n) {
     if (n + kStages - 1 < mine) issue(n + kStages - 1);
@@ -262,57 +311,56 @@ __global__ void __launch_bounds__(kWarps * 32, 3) k_attn_kv4(const __grid_consta
     }
     uint32_t vmax = 0;
 #pragma unroll
-    for (int i = 0; i < NB / 2; ++i) {
-      const uint32_t w = reinterpret_cast<const uint32_t *>(srow + S::V_OFF)[i] & 0x7fff7fffu;
-      vmax = max(vmax, max(w & 0xffffu, w >> 16));
-    }
-    vmax = __reduce_max_sync(0xffffffffu, vmax);
+    for (int i = 0; i < NB / 2; ++i)
+      vmax = __vmaxu2(vmax, reinterpret_cast<const uint32_t *>(srow + S::V_OFF)[i] & 0x7fff7fffu);
+    vmax = max(vmax & 0xffffu, vmax >> 16);
 
     // Scores: n-tile (grp, nt) column c is key 16 grp + 8 nt + c / 2 + 4 (c & 1).
     float s[8];
 #pragma unroll
     for (int grp = 0; grp < 2; ++grp) {
       const uint8_t *gp = st + grp * S::GB;
+      uint32_t w[2][NB], d0[2][NB / 2], d1[2][NB / 2];
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
         const uint8_t *kr = gp + (8 * nt + (g >> 1) + 4 * (g & 1)) * (D / 2) + t * (4 * NB);
-        uint32_t w[NB];
-        if constexpr (NB == 4) {
-          const uint4 r = *reinterpret_cast<const uint4 *>(kr);
-          w[0] = __byte_perm(r.x, r.z, 0x5410);
-          w[1] = __byte_perm(r.x, r.z, 0x7632);
-          w[2] = __byte_perm(r.y, r.w, 0x5410);
-          w[3] = __byte_perm(r.y, r.w, 0x7632);
-        } else {
-          const uint2 r = *reinterpret_cast<const uint2 *>(kr);
-          w[0] = __byte_perm(r.x, r.y, 0x5410);
-          w[1] = __byte_perm(r.x, r.y, 0x7632);
-        }
-        uint32_t d0[NB / 2], d1[NB / 2];
         const uint8_t *sp = gp + S::S_OFF + (8 * nt + t) * (2 * NB);
         if constexpr (NB == 4) {
+          const uint4 r = *reinterpret_cast<const uint4 *>(kr);
+          w[nt][0] = __byte_perm(r.x, r.z, 0x5410);
+          w[nt][1] = __byte_perm(r.x, r.z, 0x7632);
+          w[nt][2] = __byte_perm(r.y, r.w, 0x5410);
+          w[nt][3] = __byte_perm(r.y, r.w, 0x7632);
           const uint2 r0 = *reinterpret_cast<const uint2 *>(sp);
           const uint2 r1 = *reinterpret_cast<const uint2 *>(sp + 4 * (2 * NB));
-          d0[0] = r0.x; d0[1] = r0.y; d1[0] = r1.x; d1[1] = r1.y;
+          d0[nt][0] = r0.x; d0[nt][1] = r0.y; d1[nt][0] = r1.x; d1[nt][1] = r1.y;
         } else {
-          d0[0] = *reinterpret_cast<const uint32_t *>(sp);
-          d1[0] = *reinterpret_cast<const uint32_t *>(sp + 4 * (2 * NB));
+          const uint2 r = *reinterpret_cast<const uint2 *>(kr);
+          w[nt][0] = __byte_perm(r.x, r.y, 0x5410);
+          w[nt][1] = __byte_perm(r.x, r.y, 0x7632);
+          d0[nt][0] = *reinterpret_cast<const uint32_t *>(sp);
+          d1[nt][0] = *reinterpret_cast<const uint32_t *>(sp + 4 * (2 * NB));
         }
-        float s0 = 0.0f, s1 = 0.0f;
+      }
+      float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const float ci[4] = {cinit[b], cinit[b], 0.0f, 0.0f};
+      for (int b = 0; b < NB; ++b) {
+        const uint4 qa = q_s[(b * 2) * 32 + lane], qb = q_s[(b * 2 + 1) * 32 + lane];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
           float c[4];
-          mma16816(c, aq[b][0][0], aq[b][0][1], aq[b][0][2], aq[b][0][3], w[b] & 0x000f000fu,
-                   w[b] & 0x00f000f0u, ci);
-          const uint32_t h = w[b] >> 8;
-          mma16816(c, aq[b][1][0], aq[b][1][1], aq[b][1][2], aq[b][1][3], h & 0x000f000fu,
-                   h & 0x00f000f0u, c);
-          s0 = fmaf(half_at(d0, b), c[0] + c[2], s0);
-          s1 = fmaf(half_at(d1, b), c[1] + c[3], s1);
+          const uint32_t x = w[nt][b], h = x >> 8;
+          mma16816(c, qa.x, qa.y, qa.z, qa.w, codes_lo(x, one_k), codes_hi(x, one_k), zero);
+          mma16816(c, qb.x, qb.y, qb.z, qb.w, codes_lo(h, one_k), codes_hi(h, one_k), c);
+          s2[nt] = fma2(make_float2(half_at(d0[nt], b), half_at(d1[nt], b)),
+                        add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), s2[nt]);
         }
-        s[grp * 4 + nt * 2] = s0 * sc;
-        s[grp * 4 + nt * 2 + 1] = s1 * sc;
+      }
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        s[grp * 4 + nt * 2] = s2[nt].x * sc;
+        s[grp * 4 + nt * 2 + 1] = s2[nt].y * sc;
       }
     }
     if (!full) {
@@ -327,21 +375,25 @@ __global__ void __launch_bounds__(kWarps * 32, 3) k_attn_kv4(const __grid_consta
     for (int i = 1; i < 8; ++i) mt = fmaxf(mt, s[i]);
     mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
     mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-    // A raised maximum (or a larger V scale) rescales the sums; rare after the
-    // first tiles.
-    const int ev = (int)(vmax >> 10) - 15;
-    const bool grow = ev > eR + 1;  // the same in every lane
-    if (__any_sync(0xffffffffu, mt > m) || grow) {
-      const float mn = fmaxf(m, mt);
-      const float alpha = mn == -INFINITY ? 1.0f : ex2(m - mn);
-      float f = alpha;
-      if (grow) {
-        f *= pow2(eR - ev);
-        eR = ev;
-        up_v = pow2(13 - ev);
+    // A raised maximum or a larger V scale rescales the sums; rare after the
+    // first tile.
+    const bool raise = mt > m + kStaleMax;
+    const bool grow = (int)(vmax >> 10) - 15 > eR;
+    if (__any_sync(0xffffffffu, raise || grow)) {
+      float f = 1.0f;
+      if (raise) {
+        f = ex2(m - mt);  // 0 from no keys yet
+        m = mt;
+        l *= f;
       }
-      m = mn;
-      l *= alpha;
+      const uint32_t vm = __reduce_max_sync(0xffffffffu, vmax);
+      if ((int)(vm >> 10) - 15 > eR) {
+        const int old = sp + dexp;
+        eR = (int)(vm >> 10) - 15 + 1;  // one binade ahead
+        dexp = eR < -8 ? 10 : eR > 8 ? -8 : 0;
+        sp = min(11, 10 - (eR + dexp));
+        f *= pow2(sp + dexp - old);
+      }
 #pragma unroll
       for (int i = 0; i < NB * 4; ++i)
 #pragma unroll
@@ -357,7 +409,6 @@ __global__ void __launch_bounds__(kWarps * 32, 3) k_attn_kv4(const __grid_consta
     for (int grp = 0; grp < 2; ++grp) {
       const uint8_t *vp = st + grp * S::GB + S::V_OFF;
       uint32_t cw[4][NB / 2], dv[4][NB / 2];  // keys t, t + 4, t + 8, t + 12
-      float p[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint8_t *cp = vp + (t + 4 * e) * (D / 2) + g * (2 * NB);
@@ -370,14 +421,29 @@ __global__ void __launch_bounds__(kWarps * 32, 3) k_attn_kv4(const __grid_consta
           cw[e][0] = *reinterpret_cast<const uint32_t *>(cp);
           dv[e][0] = *reinterpret_cast<const uint32_t *>(dp);
         }
-        p[e] = s[grp * 4 + e] * up_v;
       }
+      if (dexp) {  // uncommon sizes of V: scales below 2^-8 or from 2^8 on
+        const __half2 c = __float2half2_rn(pow2(dexp));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int i = 0; i < NB / 2; ++i) dv[e][i] = h2bits(__hmul2(as_h2(dv[e][i]), c));
+      }
+      const float up = pow2(sp);
+      uint32_t ph01, pl01, ph23, pl23;
+      split2(s[grp * 4] * up, s[grp * 4 + 1] * up, ph01, pl01);
+      split2(s[grp * 4 + 2] * up, s[grp * 4 + 3] * up, ph23, pl23);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        uint32_t h01, l01, h23, l23;
-        split2(p[0] * half_at(dv[0], b), p[1] * half_at(dv[1], b), h01, l01);
-        split2(p[2] * half_at(dv[2], b), p[3] * half_at(dv[3], b), h23, l23);
         const uint32_t sel = (b & 1) ? 0x7632 : 0x5410;
+        const __half2 d01 = as_h2(__byte_perm(dv[0][b >> 1], dv[1][b >> 1], sel));
+        const __half2 d23 = as_h2(__byte_perm(dv[2][b >> 1], dv[3][b >> 1], sel));
+        const __half2 q01 = __hmul2_rn(as_h2(ph01), d01), q23 = __hmul2_rn(as_h2(ph23), d23);
+        const uint32_t h01 = h2bits(q01), h23 = h2bits(q23);
+        const uint32_t l01 =
+            h2bits(__hfma2(as_h2(pl01), d01, __hfma2(as_h2(ph01), d01, __hneg2(q01))));
+        const uint32_t l23 =
+            h2bits(__hfma2(as_h2(pl23), d23, __hfma2(as_h2(ph23), d23, __hneg2(q23))));
         uint32_t x = __byte_perm(cw[0][b >> 1], cw[1][b >> 1], sel);
         uint32_t y = __byte_perm(cw[2][b >> 1], cw[3][b >> 1], sel);
 #pragma unroll
@@ -386,11 +452,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) k_attn_kv4(const __grid_consta
             x >>= 8;
             y >>= 8;
           }
-          // -8 as 2^-24 and 2^-20 multiples: 0x8008 and 0x8080
-          mma16816(acc[b * 4 + j], h01, l01, h23, l23, sub_h2(x & 0x000f000fu, 0x80088008u),
-                   sub_h2(y & 0x000f000fu, 0x80088008u), acc[b * 4 + j]);
-          mma16816(acc[b * 4 + j + 1], h01, l01, h23, l23,
-                   sub_h2(x & 0x00f000f0u, 0x80808080u), sub_h2(y & 0x00f000f0u, 0x80808080u),
+          mma16816(acc[b * 4 + j], h01, l01, h23, l23, codes_lo(x, one_k), codes_lo(y, one_k), acc[b * 4 + j]);
+          mma16816(acc[b * 4 + j + 1], h01, l01, h23, l23, codes_hi(x, one_k), codes_hi(y, one_k),
                    acc[b * 4 + j + 1]);
         }
       }
@@ -406,7 +469,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) k_attn_kv4(const __grid_consta
   float *ow = reinterpret_cast<float *>(smem);
   float2 *ml = reinterpret_cast<float2 *>(smem + kWarps * kHeads * S::OROW * 4);
   {
-    const float f0 = mine ? ldexpf(1.0f, 24 - (13 - eR)) : 0.0f, f1 = f0 * 0.0625f;
+    const float f0 = mine ? ldexpf(1.0f, -(sp + dexp)) : 0.0f, f1 = f0 * 0.0625f;
     float *o = ow + (warp * kHeads + g) * S::OROW + 8 * t;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -479,7 +542,8 @@ __global__ void __launch_bounds__(D) k_kv4_combine(const __grid_constant__ Kv4At
 }
 
 template <int D>
-cudaError_t launch(const Kv4AttnArgs &a, cudaStream_t s) {
+cudaError_t launch(Kv4AttnArgs a, cudaStream_t s) {
+  a.one_k = 0x64006400u;
   cudaError_t e = cudaFuncSetAttribute(k_attn_kv4<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        Shape<D>::SMEM);
   if (e != cudaSuccess) return e;
@@ -492,14 +556,17 @@ cudaError_t launch(const Kv4AttnArgs &a, cudaStream_t s) {
 }  // namespace
 
 int kv4_pick_splits(int T, int n_kv_heads, long long keys, int longest) {
-  // About three CTAs per SM over the whole call, a split no shorter than one
-  // tile per warp.
-  const long long target = 148 * 3;
-  long long per = (keys * n_kv_heads + target - 1) / target;
-  per = (per + kSplitUnit - 1) / kSplitUnit * kSplitUnit;
-  if (per < kSplitUnit) per = kSplitUnit;
+  // One wave of CTAs over the whole call (a split of the longest token per
+  // slot that the others leave), a split no shorter than one tile per warp.
+  const long long slots = 148 * kCtasPerSm;
+  long long per = (keys * n_kv_heads + slots - 1) / slots;
+  per = std::max<long long>(kMinSplit, (per + kTile - 1) / kTile * kTile);
+  if (T * n_kv_heads < slots && longest > per) {
+    const long long fit = slots / ((long long)T * n_kv_heads);  // equal lengths: whole splits
+    const long long even = (longest + fit - 1) / fit;
+    if (keys >= (long long)T * longest - T) per = std::max(per, (even + kTile - 1) / kTile * kTile);
+  }
   const long long ns = (longest + per - 1) / per;
-  (void)T;
   return ns < 1 ? 1 : (int)ns;
 }
 

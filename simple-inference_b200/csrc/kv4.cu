@@ -187,20 +187,26 @@ __global__ void __launch_bounds__(256) k_kv4_read(const __grid_constant__ Kv4Rea
 constexpr int kCopyThreads = 256;
 constexpr int kCopyBytes = kCopyThreads * 16 * 4;
 
-template <int PAIRS>
+template <int WORDS>
 __global__ void __launch_bounds__(kCopyThreads)
-    k_kv4_update(const __grid_constant__ Kv4Update<PAIRS> u) {
+    k_kv4_update(const __grid_constant__ Kv4Update<WORDS> u) {
   pdl_trigger();
   pdl_wait();
   const int pieces = (int)((u.page_bytes + kCopyBytes - 1) / kCopyBytes);
   if (blockIdx.x == gridDim.x - 1) {
-    for (int i = threadIdx.x; i < u.n_table; i += kCopyThreads)
-      u.tables[u.word[2 * i]] = u.word[2 * i + 1];
-    const int *w = u.word + 2 * u.n_table;
+    for (int j = threadIdx.x >> 5; j < u.n_spans; j += kCopyThreads / 32) {
+      int *to = u.tables + u.word[3 * j];
+      const int n = u.word[3 * j + 1], from = u.word[3 * j + 2];
+      for (int i = threadIdx.x & 31; i < n; i += 32) to[i] = from < 0 ? -1 : u.tables[from + i];
+    }
+    const int *w = u.word + 3 * u.n_spans;
+    for (int i = threadIdx.x; i < u.n_table; i += kCopyThreads) u.tables[w[2 * i]] = w[2 * i + 1];
+    w += 2 * u.n_table;
     for (int i = threadIdx.x; i < u.n_refs; i += kCopyThreads) u.refs[w[2 * i]] = w[2 * i + 1];
     return;
   }
-  const int *w = u.word + 2 * (u.n_table + u.n_refs) + 2 * (blockIdx.x / pieces);
+  const int *w = u.word + 3 * u.n_spans + 2 * (u.n_table + u.n_refs) +
+                 2 * (blockIdx.x / pieces);
   const size_t off = (size_t)(blockIdx.x % pieces) * kCopyBytes;
   const uint8_t *src = u.pool + (size_t)w[0] * u.page_bytes + off;
   uint8_t *dst = u.pool + (size_t)w[1] * u.page_bytes + off;
@@ -235,16 +241,16 @@ cudaError_t launch_kv4_read(const Kv4ReadArgs &a, cudaStream_t s) {
                               : launch_pdl(k_kv4_read<64>, grid, dim3(256), 0, s, a);
 }
 
-template <int PAIRS>
-static cudaError_t update(const Kv4Update<PAIRS> &u, cudaStream_t s) {
+template <int WORDS>
+static cudaError_t update(const Kv4Update<WORDS> &u, cudaStream_t s) {
   const int pieces = (int)((u.page_bytes + kCopyBytes - 1) / kCopyBytes);
-  return launch_pdl(k_kv4_update<PAIRS>, dim3(u.n_copies * pieces + 1), dim3(kCopyThreads), 0, s,
+  return launch_pdl(k_kv4_update<WORDS>, dim3(u.n_copies * pieces + 1), dim3(kCopyThreads), 0, s,
                     u);
 }
-cudaError_t launch_kv4_update(const Kv4Update<kKv4SmallPairs> &u, cudaStream_t s) {
+cudaError_t launch_kv4_update(const Kv4Update<kKv4SmallWords> &u, cudaStream_t s) {
   return update(u, s);
 }
-cudaError_t launch_kv4_update(const Kv4Update<kKv4LargePairs> &u, cudaStream_t s) {
+cudaError_t launch_kv4_update(const Kv4Update<kKv4LargeWords> &u, cudaStream_t s) {
   return update(u, s);
 }
 

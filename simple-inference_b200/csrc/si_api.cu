@@ -235,6 +235,7 @@ struct si_kv4 {
   size_t page_bytes = 0;
   int *tables = nullptr, *refs = nullptr;
   si::Kv4Pages *pages = nullptr;
+  si::Kv4Edits edits;  // of the call in progress
   si::Kv4View view() const {
     si::Kv4View v;
     v.pool = pool;
@@ -1195,45 +1196,51 @@ static si_status kv4_not_capturing(si_ctx *ctx) {
   return SI_OK;
 }
 
-template <int PAIRS>
-static si_status kv4_push(si_ctx *ctx, si_kv4 *kv, const std::vector<std::pair<int, int>> *part) {
-  si::Kv4Update<PAIRS> u;
+template <int WORDS>
+static si_status kv4_push(si_ctx *ctx, si_kv4 *kv) {
+  const si::Kv4Edits &e = kv->edits;
+  si::Kv4Update<WORDS> u;
   u.tables = kv->tables;
   u.refs = kv->refs;
   u.pool = kv->pool;
   u.page_bytes = kv->page_bytes;
-  size_t at[3] = {0, 0, 0};
+  size_t s = 0, t = 0, r = 0, c = 0;
   do {
-    int n[3], used = 0;
-    for (int k = 0; k < 3; ++k) {
-      n[k] = (int)std::min<size_t>(part[k].size() - at[k], (size_t)(PAIRS - used));
-      for (int i = 0; i < n[k]; ++i) {
-        u.word[2 * (used + i)] = part[k][at[k] + i].first;
-        u.word[2 * (used + i) + 1] = part[k][at[k] + i].second;
-      }
-      at[k] += n[k];
-      used += n[k];
+    int *w = u.word, *const end = u.word + WORDS;
+    u.n_spans = u.n_table = u.n_refs = u.n_copies = 0;
+    for (; s < e.spans.size() && end - w >= 3; ++s, ++u.n_spans) {
+      *w++ = e.spans[s].to;
+      *w++ = e.spans[s].n;
+      *w++ = e.spans[s].from;
     }
-    u.n_table = n[0];
-    u.n_refs = n[1];
-    u.n_copies = n[2];
+    for (; t < e.table.size() && end - w >= 2; ++t, ++u.n_table) {
+      *w++ = e.table[t].first;
+      *w++ = e.table[t].second;
+    }
+    for (; r < e.touched.size() && end - w >= 2; ++r, ++u.n_refs) {
+      *w++ = e.touched[r];
+      *w++ = kv->pages->refs(e.touched[r]);
+    }
+    for (; c < e.copies.size() && end - w >= 2; ++c, ++u.n_copies) {
+      *w++ = e.copies[c].first;
+      *w++ = e.copies[c].second;
+    }
     SI_CUDA(si::launch_kv4_update(u, ctx->stream));
-  } while (at[0] < part[0].size() || at[1] < part[1].size() || at[2] < part[2].size());
+  } while (s < e.spans.size() || t < e.table.size() || r < e.touched.size() ||
+           c < e.copies.size());
   return SI_OK;
 }
 
 // Queues a change of the pages on the context's stream.
-static si_status kv4_flush(si_ctx *ctx, si_kv4 *kv, si::Kv4Edits &e) {
-  std::sort(e.touched.begin(), e.touched.end());
-  e.touched.erase(std::unique(e.touched.begin(), e.touched.end()), e.touched.end());
-  std::vector<std::pair<int, int>> part[3];
-  part[0].swap(e.table);
-  for (int pg : e.touched) part[1].push_back({pg, kv->pages->refs(pg)});
-  part[2].swap(e.copies);
-  const size_t n = part[0].size() + part[1].size() + part[2].size();
-  if (n == 0) return SI_OK;
-  return n <= si::kKv4SmallPairs ? kv4_push<si::kKv4SmallPairs>(ctx, kv, part)
-                                 : kv4_push<si::kKv4LargePairs>(ctx, kv, part);
+static si_status kv4_flush(si_ctx *ctx, si_kv4 *kv) {
+  si::Kv4Edits &e = kv->edits;
+  const size_t n = 3 * e.spans.size() + 2 * (e.table.size() + e.touched.size() + e.copies.size());
+  si_status st = SI_OK;
+  if (n)
+    st = n <= si::kKv4SmallWords ? kv4_push<si::kKv4SmallWords>(ctx, kv)
+                                 : kv4_push<si::kKv4LargeWords>(ctx, kv);
+  kv->pages->done(&e);
+  return st;
 }
 
 #define SI_PAGES(kv, call) \
@@ -1266,9 +1273,8 @@ static si_status kv4_writable(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs, i
   }
   if (kv->pages->writable(as_runs(runs), n)) return SI_OK;
   SI_TRY(kv4_not_capturing(ctx));
-  si::Kv4Edits e;
-  SI_PAGES(kv, reserve(as_runs(runs), n, &e));
-  return kv4_flush(ctx, kv, e);
+  SI_PAGES(kv, reserve(as_runs(runs), n, &kv->edits));
+  return kv4_flush(ctx, kv);
 }
 
 extern "C" SI_API si_status si_kv4_reserve(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs,
@@ -1280,9 +1286,8 @@ extern "C" SI_API si_status si_kv4_reserve(si_ctx *ctx, si_kv4 *kv, const si_kv4
     for (int i = 0; i < n; ++i)
       SI_CHECK((int64_t)runs[i].pos + runs[i].count <= kv->max_ctx, "positions past max_ctx %d",
                kv->max_ctx);
-    si::Kv4Edits e;
-    SI_PAGES(kv, reserve(as_runs(runs), n, &e));
-    return kv4_flush(ctx, kv, e);
+    SI_PAGES(kv, reserve(as_runs(runs), n, &kv->edits));
+    return kv4_flush(ctx, kv);
   });
 }
 
@@ -1292,9 +1297,8 @@ extern "C" SI_API si_status si_kv4_assign(si_ctx *ctx, si_kv4 *kv, const int *se
     SI_TRY(kv4_check(ctx, kv));
     SI_CHECK(n >= 0 && (n == 0 || (seqs && counts && pages)), "null argument");
     SI_TRY(kv4_not_capturing(ctx));
-    si::Kv4Edits e;
-    SI_PAGES(kv, assign(seqs, counts, n, pages, &e));
-    return kv4_flush(ctx, kv, e);
+    SI_PAGES(kv, assign(seqs, counts, n, pages, &kv->edits));
+    return kv4_flush(ctx, kv);
   });
 }
 
@@ -1304,9 +1308,8 @@ extern "C" SI_API si_status si_kv4_fork(si_ctx *ctx, si_kv4 *kv, const int *src,
     SI_TRY(kv4_check(ctx, kv));
     SI_CHECK(n >= 0 && (n == 0 || (src && dst && lens)), "null argument");
     SI_TRY(kv4_not_capturing(ctx));
-    si::Kv4Edits e;
-    SI_PAGES(kv, fork(src, dst, lens, n, &e));
-    return kv4_flush(ctx, kv, e);
+    SI_PAGES(kv, fork(src, dst, lens, n, &kv->edits));
+    return kv4_flush(ctx, kv);
   });
 }
 
@@ -1316,9 +1319,8 @@ extern "C" SI_API si_status si_kv4_release(si_ctx *ctx, si_kv4 *kv, const int *s
     SI_TRY(kv4_check(ctx, kv));
     SI_CHECK(n >= 0 && (n == 0 || seqs), "null argument");
     SI_TRY(kv4_not_capturing(ctx));
-    si::Kv4Edits e;
-    SI_PAGES(kv, release(seqs, keep, n, &e));
-    return kv4_flush(ctx, kv, e);
+    SI_PAGES(kv, release(seqs, keep, n, &kv->edits));
+    return kv4_flush(ctx, kv);
   });
 }
 
@@ -1326,9 +1328,8 @@ extern "C" SI_API si_status si_kv4_compact(si_ctx *ctx, si_kv4 *kv, int *used) {
   return kv4_entry([&]() -> si_status {
     SI_TRY(kv4_check(ctx, kv));
     SI_TRY(kv4_not_capturing(ctx));
-    si::Kv4Edits e;
-    const int n = kv->pages->compact(&e);
-    SI_TRY(kv4_flush(ctx, kv, e));
+    const int n = kv->pages->compact(&kv->edits);
+    SI_TRY(kv4_flush(ctx, kv));
     if (used) *used = n;
     return SI_OK;
   });

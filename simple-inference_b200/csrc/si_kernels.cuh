@@ -249,20 +249,21 @@ struct Kv4ReadArgs {
   int *err;
 };
 cudaError_t launch_kv4_read(const Kv4ReadArgs &a, cudaStream_t s);
-// word: n_table pairs (entry, page), n_refs pairs (page, count), n_copies
-// pairs (from, to), taken when the launch is queued.  The small form keeps a
-// decode step's few entries from carrying 28 KB of kernel parameters.
-constexpr int kKv4SmallPairs = 240, kKv4LargePairs = 3584;
-template <int PAIRS>
+// word: n_spans triples (to, n, from) of table entries that become the entries
+// from `from` on, or -1; n_table pairs (entry, page), n_refs pairs (page, count),
+// n_copies pairs (from, to), taken when the launch is queued.  The small form
+// keeps a decode step's few words from carrying 28 KB of kernel parameters.
+constexpr int kKv4SmallWords = 960, kKv4LargeWords = 7168;
+template <int WORDS>
 struct Kv4Update {
   int *tables, *refs;
   uint8_t *pool;
   size_t page_bytes;
-  int n_table, n_refs, n_copies;
-  int word[2 * PAIRS];
+  int n_spans, n_table, n_refs, n_copies;
+  int word[WORDS];
 };
-cudaError_t launch_kv4_update(const Kv4Update<kKv4SmallPairs> &u, cudaStream_t s);
-cudaError_t launch_kv4_update(const Kv4Update<kKv4LargePairs> &u, cudaStream_t s);
+cudaError_t launch_kv4_update(const Kv4Update<kKv4SmallWords> &u, cudaStream_t s);
+cudaError_t launch_kv4_update(const Kv4Update<kKv4LargeWords> &u, cudaStream_t s);
 struct Kv4AttnArgs {
   Kv4View kv;
   Kv4Runs runs;        // used without tok_ctx; token j of run i attends positions [0, pos[i] + j]
@@ -271,6 +272,7 @@ struct Kv4AttnArgs {
   const float *q;      // rows [.][Hq][D]
   float *out;          // rows [.][Hq][D]
   int nsplit;          // kv4_pick_splits()
+  uint32_t one_k;      // set by the launch
   float *part;         // kv4_part_floats() of device memory when nsplit > 1
   int *err;
 };

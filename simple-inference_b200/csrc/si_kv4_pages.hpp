@@ -20,13 +20,22 @@ struct Kv4Run {  // `count` consecutive tokens of sequence seq from position pos
   int seq, pos, count;
 };
 
+// Table entries [to, to + n) become entries [from, from + n), or -1 where from
+// is -1.
+struct Kv4Span {
+  int to, n, from;
+};
+
 // What a change asks of the device.  Copies never chain: no destination of a
-// change is a source of the same change, and no destination occurs twice.
+// change is a source of the same change, and no destination occurs twice; the
+// same holds of the table's entries and spans.
 struct Kv4Edits {
+  std::vector<Kv4Span> spans;
   std::vector<std::pair<int, int>> table;  // (entry, page)
-  std::vector<int> touched;                // pages whose reference count changed
+  std::vector<int> touched;                // pages whose reference count changed, each once
   std::vector<std::pair<int, int>> copies; // (from page, to page)
   void clear() {
+    spans.clear();
     table.clear();
     touched.clear();
     copies.clear();
@@ -37,7 +46,7 @@ class Kv4Pages {
  public:
   Kv4Pages(int n_seqs, int max_pages, int n_pages, int page_len)
       : n_seqs_(n_seqs), max_pages_(max_pages), page_len_(page_len), n_free_(n_pages),
-        count_(n_seqs, 0), refs_(n_pages, 0),
+        count_(n_seqs, 0), refs_(n_pages, 0), mark_(n_pages, 0),
         table_((size_t)n_seqs * max_pages, -1) {}
 
   int n_pages() const { return (int)refs_.size(); }
@@ -77,6 +86,12 @@ class Kv4Pages {
   }
 
   bool seq_ok(int seq) { return (seq >= 0 && seq < n_seqs_) || no("sequence out of range"); }
+
+  // Called with a change's edits once they are done with.
+  void done(Kv4Edits *e) {
+    for (int pg : e->touched) mark_[pg] = 0;
+    e->clear();
+  }
 
   // Positions [pos, pos + count) of every run get pages that no other
   // sequence holds: missing pages (from the sequence's first missing one) are
@@ -173,8 +188,9 @@ class Kv4Pages {
       for (int p = 0; p < whole; ++p) {
         const int pg = table_[at(src[i], p)];
         hold(pg, e);
-        put(dst[i], p, pg, e);
+        table_[at(dst[i], p)] = pg;
       }
+      if (whole) e->spans.push_back({(int)at(dst[i], 0), whole, (int)at(src[i], 0)});
       count_[dst[i]] = whole;
       if (lens[i] % page_len_) {
         const int pg = take(e);
@@ -195,11 +211,15 @@ class Kv4Pages {
     for (int i = 0; i < n; ++i) {
       const int64_t len = keep ? keep[i] : 0;
       const int64_t stay = (len + page_len_ - 1) / page_len_;
-      for (int p = count_[seqs[i]] - 1; p >= stay; --p) {
-        drop(table_[at(seqs[i], p)], e);
-        put(seqs[i], p, -1, e);
+      const int n = count_[seqs[i]] - (int)std::min<int64_t>(count_[seqs[i]], stay);
+      if (n == 0) continue;
+      int *row = table_.data() + at(seqs[i], count_[seqs[i]] - n);
+      for (int p = 0; p < n; ++p) {
+        drop(row[p], e);
+        row[p] = -1;
       }
-      count_[seqs[i]] = (int)std::min<int64_t>(count_[seqs[i]], stay);
+      e->spans.push_back({(int)(row - table_.data()), n, -1});
+      count_[seqs[i]] -= n;
     }
     return true;
   }
@@ -217,8 +237,8 @@ class Kv4Pages {
       refs_[hole] = refs_[pg];
       refs_[pg] = 0;
       e->copies.push_back({pg, hole});
-      e->touched.push_back(pg);
-      e->touched.push_back(hole);
+      touch(pg, e);
+      touch(hole, e);
       ++hole;
     }
     if (!e->copies.empty())
@@ -247,16 +267,21 @@ class Kv4Pages {
     hold(pg, e);
     return pg;
   }
+  void touch(int pg, Kv4Edits *e) {
+    if (mark_[pg]) return;
+    mark_[pg] = 1;
+    e->touched.push_back(pg);
+  }
   void hold(int pg, Kv4Edits *e) {
     ++refs_[pg];
-    e->touched.push_back(pg);
+    touch(pg, e);
   }
   void drop(int pg, Kv4Edits *e) {
     if (--refs_[pg] == 0) {
       ++n_free_;
       first_free_ = std::min(first_free_, pg);
     }
-    e->touched.push_back(pg);
+    touch(pg, e);
   }
   void put(int seq, int p, int pg, Kv4Edits *e) {
     table_[at(seq, p)] = pg;
@@ -265,7 +290,9 @@ class Kv4Pages {
 
   int n_seqs_, max_pages_, page_len_, n_free_;
   int first_free_ = 0;  // no free page lies below
-  std::vector<int> count_, refs_, table_;
+  std::vector<int> count_, refs_;
+  std::vector<char> mark_;  // pages in the present change's `touched`
+  std::vector<int> table_;
   std::string why_;
 };
 

@@ -54,11 +54,14 @@ int main() {
     printf("%d %d %d", ok, used, k.free_pages());
     printf(" C %zu", e.copies.size());
     for (auto &c : e.copies) printf(" %d %d", c.first, c.second);
+    printf(" S %zu", e.spans.size());
+    for (auto &c : e.spans) printf(" %d %d %d", c.to, c.n, c.from);
     printf(" T %zu", e.table.size());
     for (auto &c : e.table) printf(" %d %d", c.first, c.second);
     printf(" R %zu", e.touched.size());
     for (int p : e.touched) printf(" %d %d", p, k.refs(p));
     printf("\n");
+    k.done(&e);
     fflush(stdout);
   }
 }
@@ -100,16 +103,22 @@ class Model:
         at, parts = 3, {}
         while at < len(out):
             key, n = out[at], int(out[at + 1])
-            v = list(map(int, out[at + 2:at + 2 + 2 * n]))
-            parts[key] = list(zip(v[0::2], v[1::2]))
-            at += 2 + 2 * n
+            k = 3 if key == "S" else 2
+            v = list(map(int, out[at + 2:at + 2 + k * n]))
+            parts[key] = [tuple(v[i:i + k]) for i in range(0, k * n, k)]
+            at += 2 + k * n
         if not ok:
             assert not any(parts.values()), "a refused call asked for changes"
             assert free == sum(r == 0 for r in self.refs)
             return ok, used, free
         froms, tos = {a for a, _ in parts["C"]}, [b for _, b in parts["C"]]
         assert not froms & set(tos) and len(tos) == len(set(tos)), "copies chain or collide"
-        assert len({t for t, _ in parts["T"]}) == len(parts["T"]), "an entry is written twice"
+        assert len({t for t, _ in parts["R"]}) == len(parts["R"]), "a count is written twice"
+        written = [t + i for t, n, _ in parts["S"] for i in range(n)] + [t for t, _ in parts["T"]]
+        sources = {f + i for _, n, f in parts["S"] if f >= 0 for i in range(n)}
+        assert len(written) == len(set(written)) and not sources & set(written), "entries collide"
+        for t, n, f in parts["S"]:
+            self.table[t:t + n] = [-1] * n if f < 0 else self.table[f:f + n]
         for a, b in parts["C"]:
             assert self.refs[b] == 0, "copied over a page that was in use"
             self.pool[b] = list(self.pool[a])
