@@ -80,17 +80,7 @@ struct Params {
   int T, Hq, Hkv, G, TQ, prefix, Lp, ntiles_rows, kv_split;
   float *out;  // [T][Hq][D]
   int *err;
-  // 4-bit cache: its operands are scaled by powers of two (k_split_q4,
-  // k_split_kv4); rowf [T][Hq] takes the scores back, vbits the output.
-  const float *rowf;
-  const int *vbits;
 };
-
-// The power of two by which a KV head's K or V operands are scaled, from its
-// largest |scale| as fp16 bits: |scale| < 2^(e + 1), values < 2^(e + 4), operands
-// just below 2^14, so that fp16's smallest step is 2^-38 of the largest value and
-// the lo halves keep their bits at any size of the cache's values.
-__device__ __forceinline__ int kv4_shift(int bits) { return 10 - ((bits >> 10) - 15); }
 
 // kind::f16 instruction descriptor: fp32 accumulate, fp16 A and B, both K-major.
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n) {
@@ -287,7 +277,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int tok = t0 + tl;
     const bool valid = r < rows && tok < p.T;
     const int pos = p.prefix + tok;
-    const float rf = p.rowf && valid ? p.rowf[(size_t)tok * p.Hq + (size_t)g * p.G + hh] : 1.0f;
     const uint32_t lane_off = (uint32_t)(q * 32) << 16;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
@@ -321,7 +310,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!valid || key0 + j > pos) sv[j] = -INFINITY;
         mt = fmaxf(mt, sv[j]);
       }
-      mt *= rf;
       float alpha = 1.0f;
       const bool resc = valid && mt > m + kRescaleLog2;
       if (resc) {
@@ -332,8 +320,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t hw[32], lw[32];
 #pragma unroll
       for (int j = 0; j < BK; j += 2) {
-        const float p0 = valid ? ex2_approx(fmaf(sv[j], rf, -m)) : 0.0f;
-        const float p1 = valid ? ex2_approx(fmaf(sv[j + 1], rf, -m)) : 0.0f;
+        const float p0 = valid ? ex2_approx(sv[j] - m) : 0.0f;
+        const float p1 = valid ? ex2_approx(sv[j + 1] - m) : 0.0f;
         sum += p0 + p1;
         // hi = fp16(p), lo = fp16(p - hi), two values per packed conversion.
         const __half2 h = __floats2half2_rn(p0, p1);
@@ -400,8 +388,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (lane == 0) fail();
     } else {
       tc_fence_after();
-      float inv = valid ? 1.0f / l : 0.0f;
-      if (p.vbits) inv = ldexpf(inv, -kv4_shift(p.vbits[2 * g + 1]));
+      const float inv = valid ? 1.0f / l : 0.0f;
       float *orow = p.out + ((size_t)tok * p.Hq + (size_t)g * p.G + hh) * D;
       // The open window (tiles since the last flush) plus O total, if any.
       const bool have_total = nkt > kWindow;
@@ -500,129 +487,6 @@ __global__ void __launch_bounds__(256) k_split_kv(const void *__restrict__ kc,
   }
 }
 
-// ---- operands from the 4-bit cache (layout in kv4.cu) ----------------------
-// Largest |scale| of K and of V over positions [0, L) of one KV head, as fp16
-// bits: grid (pieces of 1024 positions, Hkv); bits [Hkv][2] start at 0.
-__global__ void __launch_bounds__(256) k_kv4_absmax(const __grid_constant__ Kv4View kv, int seq,
-                                                    int L, int *__restrict__ bits) {
-  pdl_trigger();
-  pdl_wait();
-  constexpr int NB = D / 32, GB = kv4_group_bytes(D);
-  const int head = blockIdx.y, gpp = kv.page_len / kKv4Group;
-  const int *table = kv.tables + (size_t)seq * kv.max_pages;
-  uint32_t mk = 0, mv = 0;
-  for (int i = threadIdx.x; i < 1024; i += blockDim.x) {
-    const int pos = blockIdx.x * 1024 + i;
-    if (pos >= L) break;
-    const int gi = pos / kKv4Group, page = table[gi / gpp];
-    if (page < 0 || page >= kv.n_pages) continue;
-    const uint8_t *g = kv.pool + (((size_t)page * kv.n_kv_heads + head) * gpp + gi % gpp) * GB +
-                       kKv4Group * (D / 2) + (pos % kKv4Group) * (2 * NB);
-    const uint2 k = *reinterpret_cast<const uint2 *>(g), v = *reinterpret_cast<const uint2 *>(g + GB / 2);
-    const uint32_t a = k.x & 0x7fff7fffu, b = k.y & 0x7fff7fffu;
-    const uint32_t c = v.x & 0x7fff7fffu, d = v.y & 0x7fff7fffu;
-    mk = max(mk, max(max(a & 0xffffu, a >> 16), max(b & 0xffffu, b >> 16)));
-    mv = max(mv, max(max(c & 0xffffu, c >> 16), max(d & 0xffffu, d >> 16)));
-  }
-  mk = __reduce_max_sync(0xffffffffu, mk);
-  mv = __reduce_max_sync(0xffffffffu, mv);
-  if ((threadIdx.x & 31) == 0) {
-    atomicMax(bits + 2 * head, (int)mk);
-    atomicMax(bits + 2 * head + 1, (int)mv);
-  }
-}
-
-// q * scale, times the power of two that puts the row's largest value just
-// below 2^14, as hi / lo halves; rowf undoes it and the K operand's.  One warp
-// per (token, head) row.
-__global__ void __launch_bounds__(256) k_split_q4(const float *__restrict__ q, int rows, int Hq,
-                                                  int G, float scale, const int *__restrict__ bits,
-                                                  __half *__restrict__ qh, __half *__restrict__ ql,
-                                                  float *__restrict__ rowf) {
-  pdl_trigger();
-  pdl_wait();
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= rows) return;
-  const float4 v = reinterpret_cast<const float4 *>(q + (size_t)row * D)[lane];
-  float x[4] = {__fmul_rn(v.x, scale), __fmul_rn(v.y, scale), __fmul_rn(v.z, scale),
-                __fmul_rn(v.w, scale)};
-  const float am = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-  const int ex = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(am)) >> 23);
-  const int e = min(127, 13 - (ex - 127));
-  const float up = __int_as_float((max(e, -126) + 127) << 23);
-  uint32_t h[2], l[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float a = x[2 * i] * up, b = x[2 * i + 1] * up;
-    const __half2 hh = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(hh);
-    const __half2 ll = __floats2half2_rn(a - f.x, b - f.y);
-    h[i] = *reinterpret_cast<const uint32_t *>(&hh);
-    l[i] = *reinterpret_cast<const uint32_t *>(&ll);
-  }
-  reinterpret_cast<uint2 *>(qh + (size_t)row * D)[lane] = make_uint2(h[0], h[1]);
-  reinterpret_cast<uint2 *>(ql + (size_t)row * D)[lane] = make_uint2(l[0], l[1]);
-  if (lane == 0) rowf[row] = ldexpf(1.0f, -e - kv4_shift(bits[2 * (row % Hq / G)]));
-}
-
-// k_split_kv's output from the 4-bit cache, scaled by kv4_shift: one CTA per
-// (64 positions, KV head), a thread per half-word of four codes.  scale *
-// (code - 8) has 15 bits, so hi and lo together are exact.
-__global__ void __launch_bounds__(256) k_split_kv4(const __grid_constant__ Kv4View kv, int seq,
-                                                   int L, int Lp, const int *__restrict__ bits,
-                                                   __half *__restrict__ kh, __half *__restrict__ kl,
-                                                   __half *__restrict__ vh, __half *__restrict__ vl,
-                                                   int *err) {
-  pdl_trigger();
-  pdl_wait();
-  constexpr int NB = D / 32, GB = kv4_group_bytes(D);
-  __shared__ __half sh[BK][D + 8], sl[BK][D + 8];
-  const int p0 = blockIdx.x * BK, head = blockIdx.y, gpp = kv.page_len / kKv4Group;
-  const int *table = kv.tables + (size_t)seq * kv.max_pages;
-  const float ck = ldexpf(1.0f, kv4_shift(bits[2 * head]));
-  const float cv = ldexpf(1.0f, kv4_shift(bits[2 * head + 1]));
-  for (int e = threadIdx.x; e < BK * (D / 4); e += blockDim.x) {
-    const int pp = e / (D / 4), hw = e % (D / 4), pos = p0 + pp;
-    const int b = hw % NB, d = 32 * b + 4 * (hw / NB);
-    uint32_t wk = 0x8888u, wv = 0x8888u;
-    float sk = 0.0f, sv = 0.0f;
-    if (pos < L) {
-      const int gi = pos / kKv4Group, page = table[gi / gpp], r = pos % kKv4Group;
-      if (page >= 0 && page < kv.n_pages) {
-        const uint8_t *g = kv.pool + (((size_t)page * kv.n_kv_heads + head) * gpp + gi % gpp) * GB;
-        const uint16_t *c = reinterpret_cast<const uint16_t *>(g + r * (D / 2)) + hw;
-        const uint16_t *s = reinterpret_cast<const uint16_t *>(g + kKv4Group * (D / 2)) + r * NB + b;
-        wk = c[0];
-        wv = c[GB / 4];
-        sk = f16_to_f32(s[0]) * ck;
-        sv = f16_to_f32(s[GB / 4]) * cv;
-      } else {
-        raise_error(err, 1);
-      }
-    }
-    __half khi[4], klo[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float k = sk * (float)((int)((wk >> (4 * i)) & 15u) - 8);
-      const float v = sv * (float)((int)((wv >> (4 * i)) & 15u) - 8);
-      khi[i] = __float2half_rn(k);
-      klo[i] = __float2half_rn(k - __half2float(khi[i]));
-      sh[pp][d + i] = __float2half_rn(v);
-      sl[pp][d + i] = __float2half_rn(v - __half2float(sh[pp][d + i]));
-    }
-    const size_t kd = ((size_t)head * Lp + pos) * D + d;
-    *reinterpret_cast<uint2 *>(kh + kd) = *reinterpret_cast<const uint2 *>(khi);
-    *reinterpret_cast<uint2 *>(kl + kd) = *reinterpret_cast<const uint2 *>(klo);
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < BK * D; e += blockDim.x) {
-    const int d = e / BK, pp = e % BK;
-    const size_t vd = ((size_t)head * D + d) * Lp + p0 + pp;
-    vh[vd] = sh[pp][d];
-    vl[vd] = sl[pp][d];
-  }
-}
-
 }  // namespace atc
 
 bool attn_tc_supported(const AttnArgs &a) {
@@ -636,8 +500,7 @@ size_t attn_tc_scratch_bytes(const AttnArgs &a) {
   const size_t Lp = (L + atc::BK - 1) / atc::BK * atc::BK;
   const size_t q = (size_t)a.T * a.n_q_heads * atc::D;
   const size_t kv = (size_t)a.n_kv_heads * Lp * atc::D;
-  const size_t q4 = a.kv4 ? ((size_t)a.T * a.n_q_heads + 2 * a.n_kv_heads) * 4 + 2 * 256 : 0;
-  return (2 * q + 4 * kv) * sizeof(__half) + q4 + 4 * 256;
+  return (2 * q + 4 * kv) * sizeof(__half) + 4 * 256;
 }
 
 cudaError_t launch_attention_tc(const AttnArgs &a, void *scratch, size_t scratch_bytes,
@@ -661,36 +524,14 @@ cudaError_t launch_attention_tc(const AttnArgs &a, void *scratch, size_t scratch
 
   const float scale = 1.4426950408889634f / sqrtf((float)D);
   if (reinterpret_cast<uintptr_t>(a.q) & 15) return cudaErrorMisalignedAddress;  // float4 reads
-  float *rowf = nullptr;
-  int *bits = nullptr;
-  cudaError_t e = cudaSuccess;
-  if (a.kv4) {
-    cur = align(cur + kv * 2);
-    bits = reinterpret_cast<int *>(cur);
-    cur = align(cur + 2 * a.n_kv_heads * sizeof(int));
-    rowf = reinterpret_cast<float *>(cur);
-    const int rows = a.T * a.n_q_heads;
-    e = cudaMemsetAsync(bits, 0, 2 * a.n_kv_heads * sizeof(int), s);
-    if (e != cudaSuccess) return e;
-    e = launch_pdl(k_kv4_absmax, dim3((L + 1023) / 1024, a.n_kv_heads), dim3(256), 0, s, *a.kv4,
-                   a.seq0, L, bits);
-    if (e != cudaSuccess) return e;
-    e = launch_pdl(k_split_q4, dim3((rows + 7) / 8), dim3(256), 0, s, a.q, rows, a.n_q_heads, G,
-                   scale, bits, qh, ql, rowf);
-    if (e != cudaSuccess) return e;
-    e = launch_pdl(k_split_kv4, dim3(Lp / BK, a.n_kv_heads), dim3(256), 0, s, *a.kv4, a.seq0, L,
-                   Lp, bits, kh, kl, vh, vl, a.err);
-    if (e != cudaSuccess) return e;
-  } else {
-    e = launch_pdl(k_split_q, dim3((unsigned)((q + 255) / 256 < 4096 ? (q + 255) / 256 : 4096)),
-                               dim3(256), 0, s, a.q, q, scale, qh, ql);
-    if (e != cudaSuccess) return e;
-    e = a.kv_f32 ? launch_pdl(k_split_kv<true>, dim3(Lp / BK, a.n_kv_heads), dim3(256), 0, s,
-                              a.kc, a.vc, a.seq0, a.max_ctx, a.n_kv_heads, L, Lp, kh, kl, vh, vl)
-                 : launch_pdl(k_split_kv<false>, dim3(Lp / BK, a.n_kv_heads), dim3(256), 0, s,
-                              a.kc, a.vc, a.seq0, a.max_ctx, a.n_kv_heads, L, Lp, kh, kl, vh, vl);
-    if (e != cudaSuccess) return e;
-  }
+  cudaError_t e = launch_pdl(k_split_q, dim3((unsigned)((q + 255) / 256 < 4096 ? (q + 255) / 256 : 4096)),
+                             dim3(256), 0, s, a.q, q, scale, qh, ql);
+  if (e != cudaSuccess) return e;
+  e = a.kv_f32 ? launch_pdl(k_split_kv<true>, dim3(Lp / BK, a.n_kv_heads), dim3(256), 0, s,
+                            a.kc, a.vc, a.seq0, a.max_ctx, a.n_kv_heads, L, Lp, kh, kl, vh, vl)
+               : launch_pdl(k_split_kv<false>, dim3(Lp / BK, a.n_kv_heads), dim3(256), 0, s,
+                            a.kc, a.vc, a.seq0, a.max_ctx, a.n_kv_heads, L, Lp, kh, kl, vh, vl);
+  if (e != cudaSuccess) return e;
 
   CUtensorMap mQh, mQl, mKh, mKl, mVh, mVl;
   cuuint64_t dQ[3] = {(cuuint64_t)D, (cuuint64_t)a.n_q_heads, (cuuint64_t)a.T};
@@ -710,9 +551,7 @@ cudaError_t launch_attention_tc(const AttnArgs &a, void *scratch, size_t scratch
     return cudaErrorInvalidValue;
   Params p{};
   p.T = a.T; p.Hq = a.n_q_heads; p.Hkv = a.n_kv_heads; p.G = G; p.TQ = TQ;
-  p.prefix = prefix; p.Lp = Lp; p.ntiles_rows = (a.T + TQ - 1) / TQ; p.kv_split = a.kv_f32 || a.kv4 ? 1 : 0;
-  p.rowf = rowf;
-  p.vbits = bits;
+  p.prefix = prefix; p.Lp = Lp; p.ntiles_rows = (a.T + TQ - 1) / TQ; p.kv_split = a.kv_f32 ? 1 : 0;
   p.out = a.out; p.err = a.err;
   e = cudaFuncSetAttribute(k_attn_prefill_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
   if (e != cudaSuccess) return e;

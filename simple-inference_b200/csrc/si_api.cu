@@ -1534,9 +1534,32 @@ static si_status kv4_attend(si_ctx *ctx, si_kv4 *kv, int n_q_heads, const float 
       }));
   for (int i = 0; i < n; ++i) {
     if (runs[i].count < kKv4PrefillMin || runs[i].pos < 0) continue;
+    if (!ctx->exact_attention) {
+      si::Kv4PromptArgs pa{};
+      pa.kv = a.kv;
+      pa.seq = runs[i].seq;
+      pa.prefix = runs[i].pos;
+      pa.T = runs[i].count;
+      pa.n_q_heads = n_q_heads;
+      pa.q = q + rows[i] * row;
+      pa.out = out + rows[i] * row;
+      pa.err = ctx->err;
+      SI_TRY(ctx->attn.reserve(si::kv4_prompt_scratch_bytes(pa)));
+      SI_CUDA(si::launch_attention_kv4_prompt(pa, ctx->attn.p, ctx->attn.bytes, ctx->stream));
+      continue;
+    }
+    // The fp32 kernel over the run's keys unpacked to an fp32 cache.
     const int L = runs[i].pos + runs[i].count;
+    const size_t kvd = (size_t)kv->d.n_kv_heads * D;
+    SI_TRY(ctx->kv4.reserve(2 * L * kvd * sizeof(float)));
+    float *kf = static_cast<float *>(ctx->kv4.p), *vf = kf + L * kvd;
+    const si_kv4_run all{runs[i].seq, 0, L};
+    SI_TRY(kv4_read(ctx, kv, &all, 1, kf, vf));
     si::AttnArgs aa{};
     aa.q = q + rows[i] * row;
+    aa.kc = kf;
+    aa.vc = vf;
+    aa.kv_f32 = 1;
     aa.T = runs[i].count;
     aa.n_q_heads = n_q_heads;
     aa.n_kv_heads = kv->d.n_kv_heads;
@@ -1546,24 +1569,7 @@ static si_status kv4_attend(si_ctx *ctx, si_kv4 *kv, int n_q_heads, const float 
     aa.out = out + rows[i] * row;
     aa.err = ctx->err;
     aa.nsplit = 1;
-    if (!ctx->exact_attention && si::attn_tc_supported(aa)) {
-      // Tensor cores: the operand splits straight from the pages.
-      aa.kv4 = &a.kv;
-      aa.seq0 = runs[i].seq;
-      SI_TRY(ctx->attn.reserve(si::attn_tc_scratch_bytes(aa)));
-      SI_CUDA(si::launch_attention_tc(aa, ctx->attn.p, ctx->attn.bytes, ctx->stream));
-    } else {
-      // The fp32 kernel over the run's keys unpacked to an fp32 cache.
-      const size_t kvd = (size_t)kv->d.n_kv_heads * D;
-      SI_TRY(ctx->kv4.reserve(2 * L * kvd * sizeof(float)));
-      float *kf = static_cast<float *>(ctx->kv4.p), *vf = kf + L * kvd;
-      const si_kv4_run all{runs[i].seq, 0, L};
-      SI_TRY(kv4_read(ctx, kv, &all, 1, kf, vf));
-      aa.kc = kf;
-      aa.vc = vf;
-      aa.kv_f32 = 1;
-      SI_CUDA(si::launch_attention(aa, ctx->stream));
-    }
+    SI_CUDA(si::launch_attention(aa, ctx->stream));
   }
   return SI_OK;
 }

@@ -186,9 +186,6 @@ struct AttnArgs {
   // RoPE of rope_kv.cu, the same tables), so no separate RoPE kernel runs.
   const float *qkv;
   const float *cos_tab, *sin_tab;  // [positions][D/2]
-  // Tensor-core prefill form only: the 4-bit cache that holds sequence seq0,
-  // instead of kc and vc.
-  const struct Kv4View *kv4;
 };
 size_t attn_part_floats(int T, int n_q_heads, int head_dim, int nsplit);
 // Splits the launch needs: 1 when the prefill kernel runs (contiguous tokens
@@ -207,7 +204,7 @@ size_t attn_tc_scratch_bytes(const AttnArgs &a);
 cudaError_t launch_attention_tc(const AttnArgs &a, void *scratch, size_t scratch_bytes,
                                 cudaStream_t s);
 
-// ---- kv4.cu, attention_kv4.cu (paged KV cache in 4 bits; layout in kv4.cu) -----
+// ---- kv4.cu, attention_kv4.cu, attention_kv4_tc.cu (paged KV cache in 4 bits) ---
 constexpr int kKv4Group = 16;  // positions per contiguous group
 __host__ __device__ constexpr int kv4_group_bytes(int D) {
   return kKv4Group * 2 * (D / 2 + D / 32 * 2);
@@ -281,6 +278,18 @@ struct Kv4AttnArgs {
 int kv4_pick_splits(int T, int n_kv_heads, long long keys, int longest);
 size_t kv4_part_floats(int T, int n_q_heads, int head_dim, int nsplit);
 cudaError_t launch_attention_kv4(const Kv4AttnArgs &a, cudaStream_t s);
+// A run of T consecutive tokens of sequence seq from position prefix on, on the
+// tensor cores (attention_kv4_tc.cu).
+struct Kv4PromptArgs {
+  Kv4View kv;
+  int seq, prefix, T, n_q_heads;
+  const float *q;  // [T][Hq][D], 16-byte aligned
+  float *out;      // [T][Hq][D], 16-byte aligned
+  int *err;
+};
+size_t kv4_prompt_scratch_bytes(const Kv4PromptArgs &a);
+cudaError_t launch_attention_kv4_prompt(const Kv4PromptArgs &a, void *scratch, size_t scratch_bytes,
+                                        cudaStream_t s);
 
 // ---- tp_peer.cu --------------------------------------------------------------
 // y[i] = resid[i] + sum over ranks (in rank order) of the receive slots of

@@ -244,6 +244,38 @@ def test_what_lies_behind_a_sequence_is_not_seen(si_ctx, heads, count):
     c.kv.free()
 
 
+@pytest.mark.parametrize("heads", [(12, 2, 128), (14, 2, 64)])
+@pytest.mark.parametrize("where", [0, 40, 99])
+def test_a_nan_inside_a_prompt_reaches_only_later_rows(si_ctx, heads, where):
+    """Position 20 + where of a prompt holds a NaN value: the queries before it do not see it."""
+    c = Cache(si_ctx, heads, 1, 120, 32, seed=13)
+    hq, hkv, D = heads
+    c.random([(0, 0, 120)])
+    bad = np.full((1, hkv, D), np.nan, np.float32)
+    one = np.ones((1, hkv, D), np.float32)
+    kd, vd = up(one), up(bad)
+    torch.cuda.synchronize()
+    c.kv.append(kd, vd, [(0, 20 + where, 1)])
+    q = c.rng.standard_normal((100, hq, D))
+    got = c.attend(q, [(0, 20, 100)])
+    if where:
+        c.check(got[:where], q[:where], [(0, 20, where)])
+    assert np.isnan(got[where:]).all()
+    c.kv.free()
+
+
+@pytest.mark.parametrize("heads", [(64, 8, 128), (14, 2, 64), (4, 4, 128)])
+@pytest.mark.parametrize("prefix,count", [(3000, 17), (2047, 40), (511, 16)])
+def test_short_prompt_on_a_long_prefix(si_ctx, heads, prefix, count):
+    """The key axis is split over CTAs and joined."""
+    c = Cache(si_ctx, heads, 1, prefix + count, 64, seed=14)
+    c.random([(0, 0, prefix + count)])
+    runs = [(0, prefix, count)]
+    q = c.rng.standard_normal((count, heads[0], heads[2]))
+    c.check(c.attend(q, runs), q, runs)
+    c.kv.free()
+
+
 def test_sharp_and_flat_softmax(si_ctx):
     c = Cache(si_ctx, (28, 4, 128), 1, 700, 64, seed=8)
     c.random([(0, 0, 700)])
