@@ -24,12 +24,14 @@
 // transposed [Hkv][D][Lp] (Lp = the context rounded up to 64 keys).  A CTA takes
 // 128 query rows -- TQ tokens x the G heads of a KV group -- and a split of
 // their keys, in tiles of 64:
-//   S = Q.K^T   TMEM, 128 x 64 fp32, two buffers
-//   P           TMEM, over its own scores: 32 columns of hi pairs, 32 of lo pairs
-//   O += P.V    TMEM, P as the MMA's TMEM operand; O, O_lo and the windows' sum
-// Warp roles (320 threads): warp 0 TMA producer, warp 1 MMA issue, warps 2-5 and
-// 6-9 softmax, the two groups taking turns at the tiles, so that one tile's
-// softmax runs beside the next tile's scores and the previous tile's P.V.  The
+//   S = Q.K^T   TMEM, two tiles by one MMA of 128 columns (one of 64 columns takes
+//               the tensor pipe as long)
+//   P           shared memory, hi and lo in the swizzled K-major layout
+//   O += P.V    TMEM: O, O_lo and the windows' sum
+// Warp roles (352 threads): warp 0 loads Q and K, warp 2 V (TMA), warp 1 issues
+// the MMAs, warps 3-6 and 7-10 are two softmax groups, one for each tile of a
+// pair.  The scores of pair n + 1 are queued ahead of P.V of pair n, so the
+// tensor pipe has work while the softmax of pair n runs.  The
 // running maximum is handed from tile to tile through shared memory; it is only
 // raised by a score more than 2^8 above it.  Every wait is bounded (about 2 s;
 // SI_ERR_TIMEOUT in the context's error word); on expiry every role stops, the
@@ -47,7 +49,8 @@ using namespace si::tc;
 
 constexpr int BK = 64;     // keys per tile
 constexpr int ROWS = 128;  // query rows per CTA
-constexpr int THREADS = 320;
+constexpr int PK = 2 * BK;   // keys per score MMA
+constexpr int THREADS = 352;
 constexpr float kRescaleLog2 = 8.0f;
 constexpr int kWindow = 4;  // tiles per window
 constexpr int kMaxSplits = 32;
@@ -57,13 +60,15 @@ struct Shape {
   static constexpr int NC = D / 64;               // 128-byte swizzle columns of a Q or K row
   static constexpr int Q_CHUNK = ROWS * 128;
   static constexpr int Q_BYTES = NC * Q_CHUNK;    // one split of Q
-  static constexpr int K_CHUNK = BK * 128;
-  static constexpr int K_BYTES = NC * K_CHUNK;    // one split of a K tile
+  static constexpr int K_CHUNK = PK * 128;
+  static constexpr int K_BYTES = NC * K_CHUNK;    // one split of a pair of K tiles
   static constexpr int V_BYTES = D * 128;         // one split of a V^T tile
+  static constexpr int P_BYTES = ROWS * 128;      // one split of P (128 rows x 64 keys)
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_K = OFF_Q + 2 * Q_BYTES;        // [stage][hi, lo]
-  static constexpr int OFF_V = OFF_K + 4 * K_BYTES;        // [stage][hi, lo]
-  static constexpr int OFF_BAR = OFF_V + 4 * V_BYTES;
+  static constexpr int OFF_K = OFF_Q + 2 * Q_BYTES;        // [hi, lo]
+  static constexpr int OFF_V = OFF_K + 2 * K_BYTES;        // [stage][hi, lo]
+  static constexpr int OFF_P = OFF_V + 4 * V_BYTES;        // [hi, lo]
+  static constexpr int OFF_BAR = OFF_P + 2 * P_BYTES;
   static constexpr int OFF_M = OFF_BAR + 256;              // running maximum per row
   static constexpr int OFF_L = OFF_M + ROWS * 4;           // row sums of the two groups
   static constexpr int SMEM = OFF_L + 2 * ROWS * 4 + 1024;
@@ -87,20 +92,12 @@ __device__ __forceinline__ int operand_shift(int bits) { return 10 - ((bits >> 1
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                        uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
-}
-// The left operand from TMEM: lane = row, a column holds two fp16 of the row.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int c0, int c1,
                                             int c2, uint32_t bar) {
@@ -129,6 +126,14 @@ __device__ __forceinline__ uint32_t pack_h2(float x, float y) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// x in two fp16 halves, two values per register.
+__device__ __forceinline__ void split_h2(float x, float y, uint32_t &hi, uint32_t &lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = *reinterpret_cast<const uint32_t *>(&h);
+  lo = pack_h2(x - f.x, y - f.y);
+}
+
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1)
     k_attn_kv4_tc(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__ CUtensorMap tmQl,
@@ -150,12 +155,13 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int kt0 = (int)blockIdx.z * per;
   const int nkt = min(all_kt - kt0, per);
   const int nsplits = (all_kt + per - 1) / per;
+  const int npair = (nkt + 1) / 2;
   if (nkt <= 0) return;
 
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::OFF_BAR);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  constexpr int B_Q = 0, B_KF = 1, B_KE = 3, B_VF = 5, B_VE = 7, B_SF = 9, B_PF = 11, B_MX = 13,
-                B_OD = 15, B_FIN = 17, NBAR = 18;
+  constexpr int B_Q = 0, B_KF = 1, B_KE = 2, B_SF = 3, B_SE = 4, B_VF = 5, B_VE = 7, B_PF = 9,
+                B_MX = 11, B_OD = 13, B_FIN = 15, NBAR = 16;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + S::OFF_BAR + NBAR * 8);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + S::OFF_BAR + NBAR * 8 + 16);
   float *m_s = reinterpret_cast<float *>(smem + S::OFF_M);
@@ -163,7 +169,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NBAR; ++i)
-      mbar_init(bar(i), (i >= B_PF && i < B_OD) ? 4 : 1);
+      mbar_init(bar(i), i == B_SE ? 8 : i >= B_PF && i < B_OD ? 4 : 1);  // per softmax warp
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -183,45 +189,47 @@ __global__ void __launch_bounds__(THREADS, 1)
   };
 
   if (warp == 0) {
-    // ---------------- producer ----------------
+    // ---------------- Q and K producer ----------------
     if (lane == 0) {
-      const uint32_t qb = smem_u32(smem + S::OFF_Q);
+      const uint32_t qb = smem_u32(smem + S::OFF_Q), kb = smem_u32(smem + S::OFF_K);
       mbar_expect_tx(bar(B_Q), 2 * S::NC * 128 * rows);
       for (int c = 0; c < S::NC; ++c) {
         tma_load_3d(qb + c * S::Q_CHUNK, &tmQh, c * 64, g * p.G, t0, bar(B_Q));
         tma_load_3d(qb + S::Q_BYTES + c * S::Q_CHUNK, &tmQl, c * 64, g * p.G, t0, bar(B_Q));
       }
-      int nk = 0, nv = 0;
-      bool ok = true;
-      for (int i = 0; i < nkt; ++i) {
-        const int s = i & 1, par = ((i >> 1) & 1) ^ 1;
-        if (!mbar_wait(bar(B_KE + s), par, abort_flag)) {
-          ok = false;
-          break;
-        }
-        const uint32_t kb = smem_u32(smem + S::OFF_K + s * 2 * S::K_BYTES);
-        mbar_expect_tx(bar(B_KF + s), 2 * S::K_BYTES);
-        const int krow = g * p.Lp + (kt0 + i) * BK;
+      int n = 0;
+      for (; n < npair; ++n) {
+        if (!mbar_wait(bar(B_KE), (n & 1) ^ 1, abort_flag)) break;
+        mbar_expect_tx(bar(B_KF), 2 * S::K_BYTES);
+        // (rows past this head's are read with an odd last tile, and not used)
+        const int krow = g * p.Lp + (kt0 + 2 * n) * BK;
         for (int c = 0; c < S::NC; ++c) {
-          tma_load_2d(kb + c * S::K_CHUNK, &tmKh, c * 64, krow, bar(B_KF + s));
-          tma_load_2d(kb + S::K_BYTES + c * S::K_CHUNK, &tmKl, c * 64, krow, bar(B_KF + s));
+          tma_load_2d(kb + c * S::K_CHUNK, &tmKh, c * 64, krow, bar(B_KF));
+          tma_load_2d(kb + S::K_BYTES + c * S::K_CHUNK, &tmKl, c * 64, krow, bar(B_KF));
         }
-        ++nk;
-        if (!mbar_wait(bar(B_VE + s), par, abort_flag)) {
-          ok = false;
-          break;
-        }
+      }
+      if (n < npair) {
+        fail();
+        mbar_drain(bar(B_Q), 0);
+        if (n > 0) mbar_drain(bar(B_KF), (n - 1) & 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // ---------------- V producer ----------------
+    if (lane == 0) {
+      int i = 0;
+      for (; i < nkt; ++i) {
+        const int s = i & 1;
+        if (!mbar_wait(bar(B_VE + s), ((i >> 1) & 1) ^ 1, abort_flag)) break;
         const uint32_t vb = smem_u32(smem + S::OFF_V + s * 2 * S::V_BYTES);
         mbar_expect_tx(bar(B_VF + s), 2 * S::V_BYTES);
         tma_load_2d(vb, &tmVh, (kt0 + i) * BK, g * D, bar(B_VF + s));
         tma_load_2d(vb + S::V_BYTES, &tmVl, (kt0 + i) * BK, g * D, bar(B_VF + s));
-        ++nv;
       }
-      if (!ok) {
+      if (i < nkt) {
         fail();
-        mbar_drain(bar(B_Q), 0);
-        for (int k = nk > 2 ? nk - 2 : 0; k < nk; ++k) mbar_drain(bar(B_KF + (k & 1)), (k >> 1) & 1);
-        for (int k = nv > 2 ? nv - 2 : 0; k < nv; ++k) mbar_drain(bar(B_VF + (k & 1)), (k >> 1) & 1);
+        for (int k = i > 2 ? i - 2 : 0; k < i; ++k) mbar_drain(bar(B_VF + (k & 1)), (k >> 1) & 1);
       }
     }
     __syncwarp();
@@ -229,20 +237,19 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ---------------- MMA issuer ----------------
     if (lane == 0) {
       const uint32_t qh = smem_u32(smem + S::OFF_Q), ql = qh + S::Q_BYTES;
-      constexpr uint32_t id_s = idesc_f16(ROWS, BK), id_o = idesc_f16(ROWS, D);
+      const uint32_t kh = smem_u32(smem + S::OFF_K), kl = kh + S::K_BYTES;
+      const uint32_t ph = smem_u32(smem + S::OFF_P), pl = ph + S::P_BYTES;
+      constexpr uint32_t id_s = idesc_f16(ROWS, PK), id_o = idesc_f16(ROWS, D);
       bool ok = mbar_wait(bar(B_Q), 0, abort_flag);
-      for (int i = 0; ok && i <= nkt; ++i) {
-        if (i < nkt) {
-          // S_i goes over P_(i-2), which P.V_(i-2) must have read.
-          const int s = i & 1;
-          if (!mbar_wait(bar(B_KF + s), (i >> 1) & 1, abort_flag) ||
-              (i >= 2 && !mbar_wait(bar(B_OD + s), ((i >> 1) - 1) & 1, abort_flag))) {
+      for (int n = 0; ok && n <= npair; ++n) {
+        if (n < npair) {
+          // The scores of two tiles, over those that the softmax warps have read.
+          if (!mbar_wait(bar(B_KF), n & 1, abort_flag) ||
+              (n >= 1 && !mbar_wait(bar(B_SE), (n - 1) & 1, abort_flag))) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t kh = smem_u32(smem + S::OFF_K + s * 2 * S::K_BYTES), kl = kh + S::K_BYTES;
-          const uint32_t d = tmem + S::COL_S + s * BK;
           uint32_t acc = 0;
 #pragma unroll
           for (int pass = 0; pass < 3; ++pass) {  // small products first
@@ -250,16 +257,16 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               const uint32_t off = (k & 3) * 32;
-              mma_ss(d, smem_desc(a + (k >> 2) * S::Q_CHUNK + off),
-                     smem_desc(b + (k >> 2) * S::K_CHUNK + off), id_s, acc);
+              mma_f16(tmem + S::COL_S, smem_desc(a + (k >> 2) * S::Q_CHUNK + off),
+                      smem_desc(b + (k >> 2) * S::K_CHUNK + off), id_s, acc);
               acc = 1;
             }
           }
-          mma_commit(bar(B_SF + s));
-          mma_commit(bar(B_KE + s));
+          mma_commit(bar(B_SF));
+          mma_commit(bar(B_KE));
         }
-        if (i >= 1) {
-          const int j = i - 1, s = j & 1;
+        for (int j = 2 * n - 2; n >= 1 && j < min(2 * n, nkt); ++j) {
+          const int s = j & 1;
           if (!mbar_wait(bar(B_VF + s), (j >> 1) & 1, abort_flag) ||
               !mbar_wait(bar(B_PF + s), (j >> 1) & 1, abort_flag)) {
             ok = false;
@@ -267,18 +274,19 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           tc_fence_after();
           const uint32_t vh = smem_u32(smem + S::OFF_V + s * 2 * S::V_BYTES), vl = vh + S::V_BYTES;
-          const uint32_t ph = tmem + S::COL_S + s * BK, pl = ph + BK / 2;
           // A window's first tile overwrites (the softmax warps have moved it on).
           const uint32_t first = j % kWindow != 0;
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            mma_ts(tmem + S::COL_OL, ph + 8 * k, smem_desc(vl + k * 32), id_o, k ? 1u : first);
+            mma_f16(tmem + S::COL_OL, smem_desc(ph + k * 32), smem_desc(vl + k * 32), id_o,
+                    k ? 1u : first);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            mma_ts(tmem + S::COL_OL, pl + 8 * k, smem_desc(vh + k * 32), id_o, 1u);
+            mma_f16(tmem + S::COL_OL, smem_desc(pl + k * 32), smem_desc(vh + k * 32), id_o, 1u);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            mma_ts(tmem + S::COL_O, ph + 8 * k, smem_desc(vh + k * 32), id_o, k ? 1u : first);
+            mma_f16(tmem + S::COL_O, smem_desc(ph + k * 32), smem_desc(vh + k * 32), id_o,
+                    k ? 1u : first);
           mma_commit(bar(B_OD + s));
           mma_commit(bar(B_VE + s));
         }
@@ -290,7 +298,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncwarp();
   } else {
     // ---------------- softmax (two groups of four warps) and epilogue ----------------
-    const int grp = (warp - 2) >> 2;
+    const int grp = (warp - 3) >> 2;
     const int q = warp & 3;  // TMEM lane quarter
     const int r = q * 32 + lane;
     const int tl = r / p.G, hh = r - tl * p.G;
@@ -299,11 +307,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int pos = valid ? p.prefix + tok : -1;  // a padding row attends nothing
     const float rf = valid ? p.rowf[(size_t)tok * p.Hq + (size_t)g * p.G + hh] : 0.0f;
     const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16);
+    uint8_t *prow = smem + S::OFF_P + (r >> 3) * 1024 + (r & 7) * 128;
     float mine = -INFINITY, l = 0.0f;  // this group's sum, relative to the maximum `mine`
     bool ok = true;
     for (int i = grp; i < nkt; i += 2) {
       const uint32_t t_s = t_row + S::COL_S + grp * BK;
-      if (!mbar_wait_warp(bar(B_SF + grp), (i >> 1) & 1, abort_flag)) {
+      if (!mbar_wait_warp(bar(B_SF), (i >> 1) & 1, abort_flag)) {
         ok = false;
         break;
       }
@@ -320,6 +329,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           sv[32 + j] = __uint_as_float(b[j]);
         }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_SE));
       const int key0 = (kt0 + i) * BK;
       if (__any_sync(0xffffffffu, key0 + BK - 1 > pos)) {
 #pragma unroll
@@ -354,11 +366,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       // rescales what there is.  Both once P.V_(i-1) is done.
       const bool flush = i > 0 && i % kWindow == 0;
       const bool have_total = i > kWindow;  // before this tile's flush
+      bool pv_done = i == 0;
       if (flush || (i > 0 && __any_sync(0xffffffffu, resc))) {
         if (!mbar_wait_warp(bar(B_OD + ((i - 1) & 1)), ((i - 1) >> 1) & 1, abort_flag)) {
           ok = false;
           break;
         }
+        pv_done = true;
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < D; c += 16) {
@@ -405,9 +419,21 @@ __global__ void __launch_bounds__(THREADS, 1)
         lw[j / 2] = pack_h2(p0 - h0, p1 - h1);
       }
       l += sum0 + sum1;
-      tmem_st32(t_s, hw);
-      tmem_st32(t_s + 32, lw);
-      tmem_wait_st();
+      // P belongs to the previous tile until its P.V is done.
+      if (!pv_done &&
+          !mbar_wait_warp(bar(B_OD + ((i - 1) & 1)), ((i - 1) >> 1) & 1, abort_flag)) {
+        ok = false;
+        break;
+      }
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const int sw = (c ^ (r & 7)) << 4;
+        *reinterpret_cast<uint4 *>(prow + sw) =
+            make_uint4(hw[4 * c], hw[4 * c + 1], hw[4 * c + 2], hw[4 * c + 3]);
+        *reinterpret_cast<uint4 *>(prow + S::P_BYTES + sw) =
+            make_uint4(lw[4 * c], lw[4 * c + 1], lw[4 * c + 2], lw[4 * c + 3]);
+      }
+      fence_proxy_async();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(B_PF + grp));
@@ -500,7 +526,7 @@ __global__ void __launch_bounds__(D) k_kv4_tc_combine(const Params p) {
 
 // ---- operands from the cache (layout in kv4.cu) ----------------------------
 // Largest |scale| of K and of V over positions [0, L) of one KV head, as fp16
-// bits: grid (pieces of 1024 positions, Hkv); bits [Hkv][2] start at 0.
+// bits: grid (pieces of 256 positions, Hkv); bits [Hkv][2] start at 0.
 template <int D>
 __global__ void __launch_bounds__(256) k_kv4_absmax(const __grid_constant__ Kv4View kv, int seq,
                                                     int L, int *__restrict__ bits) {
@@ -510,12 +536,9 @@ __global__ void __launch_bounds__(256) k_kv4_absmax(const __grid_constant__ Kv4V
   const int head = blockIdx.y, gpp = kv.page_len / kKv4Group;
   const int *table = kv.tables + (size_t)seq * kv.max_pages;
   uint32_t mk = 0, mv = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int pos = blockIdx.x * 1024 + i * 256 + threadIdx.x;
-    if (pos >= L) break;
-    const int gi = pos / kKv4Group, page = table[gi / gpp];
-    if (page < 0 || page >= kv.n_pages) continue;
+  const int pos = blockIdx.x * 256 + threadIdx.x;
+  const int gi = pos / kKv4Group, page = pos < L ? table[gi / gpp] : -1;
+  if (page >= 0 && page < kv.n_pages) {
     const uint8_t *g = kv.pool + (((size_t)page * kv.n_kv_heads + head) * gpp + gi % gpp) * GB +
                        kKv4Group * (D / 2) + (pos % kKv4Group) * (2 * NB);
     // (infinite and NaN scales, 0x7c00 and above, do not count)
@@ -535,68 +558,77 @@ __global__ void __launch_bounds__(256) k_kv4_absmax(const __grid_constant__ Kv4V
   }
 }
 
-// q * scale, times the power of two that puts the row's largest value just
+// The split operands of Q, K and V, in one launch: the first Hkv * Lp / 64 CTAs
+// take (64 positions, KV head) of the cache, the others eight query rows each.
+//
+// Q: q * scale, times the power of two that puts the row's largest value just
 // below 2^14, split; rowf undoes it and the K operand's.  One warp per (token,
 // head) row.
-template <int D>
-__global__ void __launch_bounds__(256) k_split_q4(const float *__restrict__ q, int rows, int Hq,
-                                                  int G, float scale, const int *__restrict__ bits,
-                                                  __half *__restrict__ qh, __half *__restrict__ ql,
-                                                  float *__restrict__ rowf) {
-  pdl_trigger();
-  pdl_wait();
-  constexpr int N = D / 32;  // values per lane
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= rows) return;
-  float x[N], am = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const float2 v = *reinterpret_cast<const float2 *>(q + (size_t)row * D + lane * N + i);
-    x[i] = __fmul_rn(v.x, scale);
-    x[i + 1] = __fmul_rn(v.y, scale);
-    am = fmaxf(am, fmaxf(fabsf(x[i]), fabsf(x[i + 1])));
-  }
-  const int ex = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(am)) >> 23);
-  const int e = max(-126, min(127, 13 - (ex - 127)));
-  const float up = __int_as_float((e + 127) << 23);
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const float a = x[i] * up, b = x[i + 1] * up;
-    const float ha = bf16_part(a), hb = bf16_part(b);
-    reinterpret_cast<uint32_t *>(qh)[((size_t)row * D + lane * N + i) / 2] = pack_h2(ha, hb);
-    reinterpret_cast<uint32_t *>(ql)[((size_t)row * D + lane * N + i) / 2] = pack_h2(a - ha, b - hb);
-  }
-  // (kept above zero: a masked score times it stays -inf)
-  if (lane == 0)
-    rowf[row] = fmaxf(ldexpf(1.0f, -e - operand_shift(bits[2 * (row % Hq / G)])), 1.2e-38f);
-}
-
 // K as [Hkv][Lp][D] and V transposed as [Hkv][D][Lp], hi and lo halves, zero
-// past L: one CTA per (64 positions, KV head), a thread per half-word of four
-// codes; V goes through shared memory for the transpose.
+// past L: a thread per half-word of four codes; V goes through shared memory for
+// the transpose, its 16-byte pieces XORed by the position's octet so that the
+// reads along positions meet different banks.
+struct SplitArgs {
+  Kv4View kv;
+  int seq, L, Lp, q_rows, Hq, G;
+  float scale;
+  const float *q;
+  const int *bits;
+  __half *qh, *ql, *kh, *kl, *vh, *vl;
+  float *rowf;
+  int *err;
+};
 template <int D>
-__global__ void __launch_bounds__(256) k_split_kv4(const __grid_constant__ Kv4View kv, int seq,
-                                                   int L, int Lp, const int *__restrict__ bits,
-                                                   __half *__restrict__ kh, __half *__restrict__ kl,
-                                                   __half *__restrict__ vh, __half *__restrict__ vl,
-                                                   int *err) {
+__global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs a) {
   pdl_trigger();
   pdl_wait();
   constexpr int NB = D / 32, GB = kv4_group_bytes(D);
-  __shared__ __half sh[BK][D + 8], sl[BK][D + 8];
-  const int p0 = blockIdx.x * BK, head = blockIdx.y, gpp = kv.page_len / kKv4Group;
-  const int *table = kv.tables + (size_t)seq * kv.max_pages;
-  const float ck = ldexpf(1.0f, operand_shift(bits[2 * head]));
-  const float cv = ldexpf(1.0f, operand_shift(bits[2 * head + 1]));
+  __shared__ __align__(16) __half sh[BK * D], sl[BK * D];
+  const int kv_ctas = a.Lp / BK * a.kv.n_kv_heads;
+  if ((int)blockIdx.x >= kv_ctas) {
+    constexpr int N = D / 32;  // values per lane
+    const int row = (blockIdx.x - kv_ctas) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row >= a.q_rows) return;
+    float x[N], am = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 v = *reinterpret_cast<const float2 *>(a.q + (size_t)row * D + lane * N + i);
+      x[i] = __fmul_rn(v.x, a.scale);
+      x[i + 1] = __fmul_rn(v.y, a.scale);
+      am = fmaxf(am, fmaxf(fabsf(x[i]), fabsf(x[i + 1])));
+    }
+    const int ex = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(am)) >> 23);
+    const int e = max(-126, min(127, 13 - (ex - 127)));
+    const float up = __int_as_float((e + 127) << 23);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float u = x[i] * up, v = x[i + 1] * up;
+      const float hu = bf16_part(u), hv = bf16_part(v);
+      const size_t at = ((size_t)row * D + lane * N + i) / 2;
+      reinterpret_cast<uint32_t *>(a.qh)[at] = pack_h2(hu, hv);
+      reinterpret_cast<uint32_t *>(a.ql)[at] = pack_h2(u - hu, v - hv);
+    }
+    // (kept above zero: a masked score times it stays -inf)
+    if (lane == 0)
+      a.rowf[row] =
+          fmaxf(ldexpf(1.0f, -e - operand_shift(a.bits[2 * (row % a.Hq / a.G)])), 1.2e-38f);
+    return;
+  }
+  const int head = blockIdx.x / (a.Lp / BK), p0 = blockIdx.x % (a.Lp / BK) * BK;
+  const int gpp = a.kv.page_len / kKv4Group;
+  const int *table = a.kv.tables + (size_t)a.seq * a.kv.max_pages;
+  const float ck = ldexpf(1.0f, operand_shift(a.bits[2 * head]));
+  const float cv = ldexpf(1.0f, operand_shift(a.bits[2 * head + 1]));
   for (int e = threadIdx.x; e < BK * (D / 4); e += blockDim.x) {
     const int pp = e / (D / 4), hw = e % (D / 4), pos = p0 + pp;
     const int b = hw % NB, d = 32 * b + 4 * (hw / NB);
     uint32_t wk = 0x8888u, wv = 0x8888u;
     float sk = 0.0f, sv = 0.0f;
-    if (pos < L) {
+    if (pos < a.L) {
       const int gi = pos / kKv4Group, page = table[gi / gpp], r = pos % kKv4Group;
-      if (page >= 0 && page < kv.n_pages) {
-        const uint8_t *g = kv.pool + (((size_t)page * kv.n_kv_heads + head) * gpp + gi % gpp) * GB;
+      if (page >= 0 && page < a.kv.n_pages) {
+        const uint8_t *g =
+            a.kv.pool + (((size_t)page * a.kv.n_kv_heads + head) * gpp + gi % gpp) * GB;
         const uint16_t *c = reinterpret_cast<const uint16_t *>(g + r * (D / 2)) + hw;
         const uint16_t *s = reinterpret_cast<const uint16_t *>(g + kKv4Group * (D / 2)) + r * NB + b;
         wk = c[0];
@@ -611,30 +643,38 @@ __global__ void __launch_bounds__(256) k_split_kv4(const __grid_constant__ Kv4Vi
           sk = __int_as_float(0x7fffffff);
         }
       } else {
-        raise_error(err, 1);
+        raise_error(a.err, 1);
       }
     }
-    __half khi[4], klo[4];
+    uint32_t kh2[2], kl2[2], vh2[2], vl2[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float k = sk * (float)((int)((wk >> (4 * i)) & 15u) - 8);
-      const float v = sv * (float)((int)((wv >> (4 * i)) & 15u) - 8);
-      khi[i] = __float2half_rn(k);
-      klo[i] = __float2half_rn(k - __half2float(khi[i]));
-      const __half vhi = __float2half_rn(v);
-      sh[pp][d + i] = vhi;
-      sl[pp][d + i] = __float2half_rn(v - __half2float(vhi));
+    for (int i = 0; i < 2; ++i) {
+      const int c0 = (int)((wk >> (8 * i)) & 15u) - 8, c1 = (int)((wk >> (8 * i + 4)) & 15u) - 8;
+      const int e0 = (int)((wv >> (8 * i)) & 15u) - 8, e1 = (int)((wv >> (8 * i + 4)) & 15u) - 8;
+      split_h2(sk * (float)c0, sk * (float)c1, kh2[i], kl2[i]);
+      split_h2(sv * (float)e0, sv * (float)e1, vh2[i], vl2[i]);
     }
-    const size_t kd = ((size_t)head * Lp + pos) * D + d;
-    *reinterpret_cast<uint2 *>(kh + kd) = *reinterpret_cast<const uint2 *>(khi);
-    *reinterpret_cast<uint2 *>(kl + kd) = *reinterpret_cast<const uint2 *>(klo);
+    const size_t kd = ((size_t)head * a.Lp + pos) * D + d;
+    *reinterpret_cast<uint2 *>(a.kh + kd) = make_uint2(kh2[0], kh2[1]);
+    *reinterpret_cast<uint2 *>(a.kl + kd) = make_uint2(kl2[0], kl2[1]);
+    const int at = pp * D + (d ^ ((pp >> 3) * 8));
+    *reinterpret_cast<uint2 *>(sh + at) = make_uint2(vh2[0], vh2[1]);
+    *reinterpret_cast<uint2 *>(sl + at) = make_uint2(vl2[0], vl2[1]);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < BK * D / 2; e += blockDim.x) {
-    const int d = e / (BK / 2), pp = e % (BK / 2) * 2;
-    const size_t vd = ((size_t)head * D + d) * Lp + p0 + pp;
-    *reinterpret_cast<__half2 *>(vh + vd) = __halves2half2(sh[pp][d], sh[pp + 1][d]);
-    *reinterpret_cast<__half2 *>(vl + vd) = __halves2half2(sl[pp][d], sl[pp + 1][d]);
+  for (int e = threadIdx.x; e < D * (BK / 8); e += blockDim.x) {  // a dim's eight positions
+    const int d = e / (BK / 8), o = e % (BK / 8);
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r0 = (8 * o + 2 * j) * D + (d ^ (o * 8)), r1 = r0 + D;
+      const __half2 x = __halves2half2(sh[r0], sh[r1]), y = __halves2half2(sl[r0], sl[r1]);
+      h[j] = *reinterpret_cast<const uint32_t *>(&x);
+      l[j] = *reinterpret_cast<const uint32_t *>(&y);
+    }
+    const size_t vd = ((size_t)head * D + d) * a.Lp + p0 + 8 * o;
+    *reinterpret_cast<uint4 *>(a.vh + vd) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4 *>(a.vl + vd) = make_uint4(l[0], l[1], l[2], l[3]);
   }
 }
 
@@ -683,14 +723,12 @@ cudaError_t launch(const Kv4PromptArgs &a, char *base, const Scratch &sc, cudaSt
   const int rows = a.T * Hq;
   cudaError_t e = cudaMemsetAsync(bits, 0, 2 * Hkv * sizeof(int), s);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(k_kv4_absmax<D>, dim3((L + 1023) / 1024, Hkv), dim3(256), 0, s, a.kv, a.seq, L,
+  e = launch_pdl(k_kv4_absmax<D>, dim3((L + 255) / 256, Hkv), dim3(256), 0, s, a.kv, a.seq, L,
                  bits);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(k_split_q4<D>, dim3((rows + 7) / 8), dim3(256), 0, s, a.q, rows, Hq, G, scale,
-                 bits, qh, ql, rowf);
-  if (e != cudaSuccess) return e;
-  e = launch_pdl(k_split_kv4<D>, dim3(Lp / BK, Hkv), dim3(256), 0, s, a.kv, a.seq, L, Lp, bits, kh,
-                 kl, vh, vl, a.err);
+  SplitArgs sa{a.kv, a.seq, L, Lp, rows, Hq, G, scale, a.q, bits, qh, ql, kh, kl, vh, vl, rowf,
+               a.err};
+  e = launch_pdl(k_split<D>, dim3(Lp / BK * Hkv + (rows + 7) / 8), dim3(256), 0, s, sa);
   if (e != cudaSuccess) return e;
 
   CUtensorMap mQh, mQl, mKh, mKl, mVh, mVl;
@@ -699,7 +737,7 @@ cudaError_t launch(const Kv4PromptArgs &a, char *base, const Scratch &sc, cudaSt
   cuuint32_t bQ[3] = {64, (cuuint32_t)G, (cuuint32_t)TQ};
   cuuint64_t dK[2] = {(cuuint64_t)D, (cuuint64_t)Hkv * Lp};
   cuuint64_t sK[1] = {(cuuint64_t)D * 2};
-  cuuint32_t bK[2] = {64, (cuuint32_t)BK};
+  cuuint32_t bK[2] = {64, (cuuint32_t)PK};
   cuuint64_t dV[2] = {(cuuint64_t)Lp, (cuuint64_t)Hkv * D};
   cuuint64_t sV[1] = {(cuuint64_t)Lp * 2};
   cuuint32_t bV[2] = {(cuuint32_t)BK, (cuuint32_t)D};
