@@ -107,6 +107,12 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
       : "memory");
 }
+// Two waits, asked for at once.
+__device__ __forceinline__ bool mbar_wait2(uint32_t b1, uint32_t p1, uint32_t b2, uint32_t p2,
+                                           volatile int *abort) {
+  const bool t1 = mbar_try(b1, p1), t2 = mbar_try(b2, p2);
+  return (t1 || mbar_wait(b1, p1, abort)) && (t2 || mbar_wait(b2, p2, abort));
+}
 __device__ __forceinline__ bool mbar_drain(uint32_t bar, uint32_t parity) {
   const uint64_t t0 = globaltimer();
   while (!mbar_try_sleep(bar, parity))
@@ -244,8 +250,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int n = 0; ok && n <= npair; ++n) {
         if (n < npair) {
           // The scores of two tiles, over those that the softmax warps have read.
-          if (!mbar_wait(bar(B_KF), n & 1, abort_flag) ||
-              (n >= 1 && !mbar_wait(bar(B_SE), (n - 1) & 1, abort_flag))) {
+          if (n >= 1 ? !mbar_wait2(bar(B_KF), n & 1, bar(B_SE), (n - 1) & 1, abort_flag)
+                     : !mbar_wait(bar(B_KF), 0, abort_flag)) {
             ok = false;
             break;
           }
@@ -267,8 +273,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         for (int j = 2 * n - 2; n >= 1 && j < min(2 * n, nkt); ++j) {
           const int s = j & 1;
-          if (!mbar_wait(bar(B_VF + s), (j >> 1) & 1, abort_flag) ||
-              !mbar_wait(bar(B_PF + s), (j >> 1) & 1, abort_flag)) {
+          if (!mbar_wait2(bar(B_VF + s), (j >> 1) & 1, bar(B_PF + s), (j >> 1) & 1, abort_flag)) {
             ok = false;
             break;
           }
@@ -362,17 +367,30 @@ __global__ void __launch_bounds__(THREADS, 1)
         l *= ex2(mine - m);
         mine = m;
       }
-      // A window that tile i - 1 closed goes into the sum; a raised maximum
-      // rescales what there is.  Both once P.V_(i-1) is done.
+      const float mu = m == -INFINITY ? 0.0f : m;
+      float sum0 = 0.0f, sum1 = 0.0f;
+      uint32_t hw[32], lw[32];
+#pragma unroll
+      for (int j = 0; j < BK; j += 2) {
+        // (-inf * 0 of a padding row would be NaN; its results are not used)
+        const float p0 = ex2(fmaf(sv[j], rf, -mu)), p1 = ex2(fmaf(sv[j + 1], rf, -mu));
+        sum0 += p0;
+        sum1 += p1;
+        const float h0 = bf16_part(p0), h1 = bf16_part(p1);
+        hw[j / 2] = pack_h2(h0, h1);
+        lw[j / 2] = pack_h2(p0 - h0, p1 - h1);
+      }
+      l += sum0 + sum1;
+      // P and the output belong to the previous tile until its P.V is done.  A
+      // window that it closed goes into the sum; a raised maximum rescales what
+      // there is.
+      if (i > 0 && !mbar_wait_warp(bar(B_OD + ((i - 1) & 1)), ((i - 1) >> 1) & 1, abort_flag)) {
+        ok = false;
+        break;
+      }
       const bool flush = i > 0 && i % kWindow == 0;
       const bool have_total = i > kWindow;  // before this tile's flush
-      bool pv_done = i == 0;
       if (flush || (i > 0 && __any_sync(0xffffffffu, resc))) {
-        if (!mbar_wait_warp(bar(B_OD + ((i - 1) & 1)), ((i - 1) >> 1) & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
-        pv_done = true;
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < D; c += 16) {
@@ -404,26 +422,6 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
         tmem_wait_st();
-      }
-      const float mu = m == -INFINITY ? 0.0f : m;
-      float sum0 = 0.0f, sum1 = 0.0f;
-      uint32_t hw[32], lw[32];
-#pragma unroll
-      for (int j = 0; j < BK; j += 2) {
-        // (-inf * 0 of a padding row would be NaN; its results are not used)
-        const float p0 = ex2(fmaf(sv[j], rf, -mu)), p1 = ex2(fmaf(sv[j + 1], rf, -mu));
-        sum0 += p0;
-        sum1 += p1;
-        const float h0 = bf16_part(p0), h1 = bf16_part(p1);
-        hw[j / 2] = pack_h2(h0, h1);
-        lw[j / 2] = pack_h2(p0 - h0, p1 - h1);
-      }
-      l += sum0 + sum1;
-      // P belongs to the previous tile until its P.V is done.
-      if (!pv_done &&
-          !mbar_wait_warp(bar(B_OD + ((i - 1) & 1)), ((i - 1) >> 1) & 1, abort_flag)) {
-        ok = false;
-        break;
       }
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
