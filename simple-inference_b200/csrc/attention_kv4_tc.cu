@@ -26,12 +26,19 @@
 // their keys, in tiles of 64:
 //   S = Q.K^T   TMEM, two tiles by one MMA of 128 columns (one of 64 columns takes
 //               the tensor pipe as long)
-//   P           shared memory, hi and lo in the swizzled K-major layout
-//   O += P.V    TMEM: O, O_lo and the windows' sum
-// Warp roles (352 threads): warp 0 loads Q and K, warp 2 V (TMA), warp 1 issues
-// the MMAs, warps 3-6 and 7-10 are two softmax groups, one for each tile of a
-// pair.  The scores of pair n + 1 are queued ahead of P.V of pair n, so the
-// tensor pipe has work while the softmax of pair n runs.  The
+//   P           TMEM, hi and lo, a buffer for each tile of a pair: the MMA takes its
+//               left operand from there, which halves its shared-memory reads
+//   O += P.V    TMEM: O and O_lo; finished windows in the softmax warps' registers,
+//               half of the dims in each group
+// Warp roles (384 threads): warp 0 loads Q and K, warp 2 V (TMA), warp 1 issues
+// the MMAs of the scores, warp 3 those of P.V (a thread's wait on a barrier takes
+// some 300 cycles even when it is open, during which the other one's MMAs run),
+// warps 4-7 and 8-11 are two softmax groups, one for each tile of a
+// pair.  The scores of pair n + 1 follow as soon as both groups have read those of
+// pair n, so the tensor pipe has work while the softmax of pair n runs.  Shared memory is what
+// bounds this: an MMA of 128 x 128 x 16 reads 8 KB of it in 64 cycles, all that
+// there is, beside the copies that bring K and V.  (P through shared memory, in one
+// buffer: 417 us for 509 tokens of 72B on 7680.)  The
 // running maximum is handed from tile to tile through shared memory; it is only
 // raised by a score more than 2^8 above it.  Every wait is bounded (about 2 s;
 // SI_ERR_TIMEOUT in the context's error word); on expiry every role stops, the
@@ -50,7 +57,11 @@ using namespace si::tc;
 constexpr int BK = 64;     // keys per tile
 constexpr int ROWS = 128;  // query rows per CTA
 constexpr int PK = 2 * BK;   // keys per score MMA
-constexpr int THREADS = 352;
+constexpr int THREADS = 384;
+// Registers: launched with kRegs a thread; the control warps give up what the
+// softmax warps take (the sums match, else the kernel would wait for good).
+constexpr int kRegs = 168, kRegsControl = 56, kRegsSoftmax = 224;
+static_assert(THREADS * kRegs >= 128 * kRegsControl + 256 * kRegsSoftmax, "register split");
 constexpr float kRescaleLog2 = 8.0f;
 constexpr int kWindow = 4;  // tiles per window
 constexpr int kMaxSplits = 32;
@@ -63,16 +74,14 @@ struct Shape {
   static constexpr int K_CHUNK = PK * 128;
   static constexpr int K_BYTES = NC * K_CHUNK;    // one split of a pair of K tiles
   static constexpr int V_BYTES = D * 128;         // one split of a V^T tile
-  static constexpr int P_BYTES = ROWS * 128;      // one split of P (128 rows x 64 keys)
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = OFF_Q + 2 * Q_BYTES;        // [hi, lo]
   static constexpr int OFF_V = OFF_K + 2 * K_BYTES;        // [stage][hi, lo]
-  static constexpr int OFF_P = OFF_V + 4 * V_BYTES;        // [hi, lo]
-  static constexpr int OFF_BAR = OFF_P + 2 * P_BYTES;
+  static constexpr int OFF_BAR = OFF_V + 4 * V_BYTES;
   static constexpr int OFF_M = OFF_BAR + 256;              // running maximum per row
   static constexpr int OFF_L = OFF_M + ROWS * 4;           // row sums of the two groups
   static constexpr int SMEM = OFF_L + 2 * ROWS * 4 + 1024;
-  static constexpr uint32_t COL_S = 0, COL_O = 128, COL_OL = 128 + D, COL_OT = 128 + 2 * D;
+  static constexpr uint32_t COL_S = 0, COL_P = 128, COL_O = 256, COL_OL = 256 + D;
 };
 static_assert(Shape<128>::SMEM <= 232448, "shared memory budget");
 
@@ -98,6 +107,14 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+// The left operand from TMEM: lane = row, a column holds two fp16 of the row.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int c0, int c1,
                                             int c2, uint32_t bar) {
@@ -167,7 +184,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::OFF_BAR);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   constexpr int B_Q = 0, B_KF = 1, B_KE = 2, B_SF = 3, B_SE = 4, B_VF = 5, B_VE = 7, B_PF = 9,
-                B_MX = 11, B_OD = 13, B_FIN = 15, NBAR = 16;
+                B_MX = 11, B_OD = 13, B_FL = 17, B_FIN = 18, NBAR = 20;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + S::OFF_BAR + NBAR * 8);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + S::OFF_BAR + NBAR * 8 + 16);
   float *m_s = reinterpret_cast<float *>(smem + S::OFF_M);
@@ -175,7 +192,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NBAR; ++i)
-      mbar_init(bar(i), i == B_SE ? 8 : i >= B_PF && i < B_OD ? 4 : 1);  // per softmax warp
+      mbar_init(bar(i), i == B_SE || i == B_FL ? 8 : i >= B_PF && i < B_OD ? 4 : 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -194,61 +211,61 @@ __global__ void __launch_bounds__(THREADS, 1)
     *abort_flag = 1;
   };
 
-  if (warp == 0) {
-    // ---------------- Q and K producer ----------------
-    if (lane == 0) {
-      const uint32_t qb = smem_u32(smem + S::OFF_Q), kb = smem_u32(smem + S::OFF_K);
-      mbar_expect_tx(bar(B_Q), 2 * S::NC * 128 * rows);
-      for (int c = 0; c < S::NC; ++c) {
-        tma_load_3d(qb + c * S::Q_CHUNK, &tmQh, c * 64, g * p.G, t0, bar(B_Q));
-        tma_load_3d(qb + S::Q_BYTES + c * S::Q_CHUNK, &tmQl, c * 64, g * p.G, t0, bar(B_Q));
-      }
-      int n = 0;
-      for (; n < npair; ++n) {
-        if (!mbar_wait(bar(B_KE), (n & 1) ^ 1, abort_flag)) break;
-        mbar_expect_tx(bar(B_KF), 2 * S::K_BYTES);
-        // (rows past this head's are read with an odd last tile, and not used)
-        const int krow = g * p.Lp + (kt0 + 2 * n) * BK;
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+    if (warp == 0) {
+      // ---------------- Q and K producer ----------------
+      if (lane == 0) {
+        const uint32_t qb = smem_u32(smem + S::OFF_Q), kb = smem_u32(smem + S::OFF_K);
+        mbar_expect_tx(bar(B_Q), 2 * S::NC * 128 * rows);
         for (int c = 0; c < S::NC; ++c) {
-          tma_load_2d(kb + c * S::K_CHUNK, &tmKh, c * 64, krow, bar(B_KF));
-          tma_load_2d(kb + S::K_BYTES + c * S::K_CHUNK, &tmKl, c * 64, krow, bar(B_KF));
+          tma_load_3d(qb + c * S::Q_CHUNK, &tmQh, c * 64, g * p.G, t0, bar(B_Q));
+          tma_load_3d(qb + S::Q_BYTES + c * S::Q_CHUNK, &tmQl, c * 64, g * p.G, t0, bar(B_Q));
+        }
+        int n = 0;
+        for (; n < npair; ++n) {
+          if (!mbar_wait(bar(B_KE), (n & 1) ^ 1, abort_flag)) break;
+          mbar_expect_tx(bar(B_KF), 2 * S::K_BYTES);
+          // (rows past this head's are read with an odd last tile, and not used)
+          const int krow = g * p.Lp + (kt0 + 2 * n) * BK;
+          for (int c = 0; c < S::NC; ++c) {
+            tma_load_2d(kb + c * S::K_CHUNK, &tmKh, c * 64, krow, bar(B_KF));
+            tma_load_2d(kb + S::K_BYTES + c * S::K_CHUNK, &tmKl, c * 64, krow, bar(B_KF));
+          }
+        }
+        if (n < npair) {
+          fail();
+          mbar_drain(bar(B_Q), 0);
+          if (n > 0) mbar_drain(bar(B_KF), (n - 1) & 1);
         }
       }
-      if (n < npair) {
-        fail();
-        mbar_drain(bar(B_Q), 0);
-        if (n > 0) mbar_drain(bar(B_KF), (n - 1) & 1);
+      __syncwarp();
+    } else if (warp == 2) {
+      // ---------------- V producer ----------------
+      if (lane == 0) {
+        int i = 0;
+        for (; i < nkt; ++i) {
+          const int s = i & 1;
+          if (!mbar_wait(bar(B_VE + s), ((i >> 1) & 1) ^ 1, abort_flag)) break;
+          const uint32_t vb = smem_u32(smem + S::OFF_V + s * 2 * S::V_BYTES);
+          mbar_expect_tx(bar(B_VF + s), 2 * S::V_BYTES);
+          tma_load_2d(vb, &tmVh, (kt0 + i) * BK, g * D, bar(B_VF + s));
+          tma_load_2d(vb + S::V_BYTES, &tmVl, (kt0 + i) * BK, g * D, bar(B_VF + s));
+        }
+        if (i < nkt) {
+          fail();
+          for (int k = i > 2 ? i - 2 : 0; k < i; ++k) mbar_drain(bar(B_VF + (k & 1)), (k >> 1) & 1);
+        }
       }
-    }
-    __syncwarp();
-  } else if (warp == 2) {
-    // ---------------- V producer ----------------
-    if (lane == 0) {
-      int i = 0;
-      for (; i < nkt; ++i) {
-        const int s = i & 1;
-        if (!mbar_wait(bar(B_VE + s), ((i >> 1) & 1) ^ 1, abort_flag)) break;
-        const uint32_t vb = smem_u32(smem + S::OFF_V + s * 2 * S::V_BYTES);
-        mbar_expect_tx(bar(B_VF + s), 2 * S::V_BYTES);
-        tma_load_2d(vb, &tmVh, (kt0 + i) * BK, g * D, bar(B_VF + s));
-        tma_load_2d(vb + S::V_BYTES, &tmVl, (kt0 + i) * BK, g * D, bar(B_VF + s));
-      }
-      if (i < nkt) {
-        fail();
-        for (int k = i > 2 ? i - 2 : 0; k < i; ++k) mbar_drain(bar(B_VF + (k & 1)), (k >> 1) & 1);
-      }
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      const uint32_t qh = smem_u32(smem + S::OFF_Q), ql = qh + S::Q_BYTES;
-      const uint32_t kh = smem_u32(smem + S::OFF_K), kl = kh + S::K_BYTES;
-      const uint32_t ph = smem_u32(smem + S::OFF_P), pl = ph + S::P_BYTES;
-      constexpr uint32_t id_s = idesc_f16(ROWS, PK), id_o = idesc_f16(ROWS, D);
-      bool ok = mbar_wait(bar(B_Q), 0, abort_flag);
-      for (int n = 0; ok && n <= npair; ++n) {
-        if (n < npair) {
+      __syncwarp();
+    } else if (warp == 1) {
+      // ---------------- S issuer ----------------
+      if (lane == 0) {
+        const uint32_t qh = smem_u32(smem + S::OFF_Q), ql = qh + S::Q_BYTES;
+        const uint32_t kh = smem_u32(smem + S::OFF_K), kl = kh + S::K_BYTES;
+        constexpr uint32_t id_s = idesc_f16(ROWS, PK);
+        bool ok = mbar_wait(bar(B_Q), 0, abort_flag);
+        for (int n = 0; ok && n < npair; ++n) {
           // The scores of two tiles, over those that the softmax warps have read.
           if (n >= 1 ? !mbar_wait2(bar(B_KF), n & 1, bar(B_SE), (n - 1) & 1, abort_flag)
                      : !mbar_wait(bar(B_KF), 0, abort_flag)) {
@@ -271,39 +288,51 @@ __global__ void __launch_bounds__(THREADS, 1)
           mma_commit(bar(B_SF));
           mma_commit(bar(B_KE));
         }
-        for (int j = 2 * n - 2; n >= 1 && j < min(2 * n, nkt); ++j) {
+        if (!ok) fail();
+        mma_commit(bar(B_FIN));
+        mbar_drain(bar(B_FIN), 0);
+      }
+      __syncwarp();
+    } else if (warp == 3) {
+      // ---------------- P.V issuer ----------------
+      if (lane == 0) {
+        constexpr uint32_t id_o = idesc_f16(ROWS, D);
+        bool ok = true;
+        for (int j = 0; j < nkt; ++j) {
           const int s = j & 1;
-          if (!mbar_wait2(bar(B_VF + s), (j >> 1) & 1, bar(B_PF + s), (j >> 1) & 1, abort_flag)) {
+          // (a window's first tile also: both groups have taken the last window's sums)
+          if (!mbar_wait2(bar(B_VF + s), (j >> 1) & 1, bar(B_PF + s), (j >> 1) & 1, abort_flag) ||
+              (j > 0 && j % kWindow == 0 &&
+               !mbar_wait(bar(B_FL), (j / kWindow - 1) & 1, abort_flag))) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t vh = smem_u32(smem + S::OFF_V + s * 2 * S::V_BYTES), vl = vh + S::V_BYTES;
-          // A window's first tile overwrites (the softmax warps have moved it on).
-          const uint32_t first = j % kWindow != 0;
+          const uint32_t ph = tmem + S::COL_P + s * BK, pl = ph + BK / 2;
+          const uint32_t first = j % kWindow != 0;  // a window's first tile overwrites
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            mma_f16(tmem + S::COL_OL, smem_desc(ph + k * 32), smem_desc(vl + k * 32), id_o,
-                    k ? 1u : first);
+            mma_ts(tmem + S::COL_OL, ph + 8 * k, smem_desc(vl + k * 32), id_o, k ? 1u : first);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            mma_f16(tmem + S::COL_OL, smem_desc(pl + k * 32), smem_desc(vh + k * 32), id_o, 1u);
+            mma_ts(tmem + S::COL_OL, pl + 8 * k, smem_desc(vh + k * 32), id_o, 1u);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            mma_f16(tmem + S::COL_O, smem_desc(ph + k * 32), smem_desc(vh + k * 32), id_o,
-                    k ? 1u : first);
-          mma_commit(bar(B_OD + s));
+            mma_ts(tmem + S::COL_O, ph + 8 * k, smem_desc(vh + k * 32), id_o, k ? 1u : first);
+          mma_commit(bar(B_OD + (j & 3)));
           mma_commit(bar(B_VE + s));
         }
+        if (!ok) fail();
+        mma_commit(bar(B_FIN + 1));
+        mbar_drain(bar(B_FIN + 1), 0);
       }
-      if (!ok) fail();
-      mma_commit(bar(B_FIN));
-      mbar_drain(bar(B_FIN), 0);
+      __syncwarp();
     }
-    __syncwarp();
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     // ---------------- softmax (two groups of four warps) and epilogue ----------------
-    const int grp = (warp - 3) >> 2;
+    const int grp = (warp - 4) >> 2;
     const int q = warp & 3;  // TMEM lane quarter
     const int r = q * 32 + lane;
     const int tl = r / p.G, hh = r - tl * p.G;
@@ -312,9 +341,30 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int pos = valid ? p.prefix + tok : -1;  // a padding row attends nothing
     const float rf = valid ? p.rowf[(size_t)tok * p.Hq + (size_t)g * p.G + hh] : 0.0f;
     const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16);
-    uint8_t *prow = smem + S::OFF_P + (r >> 3) * 1024 + (r & 7) * 128;
-    float mine = -INFINITY, l = 0.0f;  // this group's sum, relative to the maximum `mine`
+    constexpr int H = D / 2;   // this group keeps dims [grp * H, grp * H + H) of the sums
+    const uint32_t t_o = t_row + S::COL_O + grp * H, t_ol = t_row + S::COL_OL + grp * H;
+    const uint32_t t_p = t_row + S::COL_P + grp * BK;
+    float tot[H];              // finished windows, relative to the maximum `mine`
+#pragma unroll
+    for (int k = 0; k < H; ++k) tot[k] = 0.0f;
+    float mine = -INFINITY, l = 0.0f;  // l: this group's tiles, relative to `mine`
     bool ok = true;
+    // (tot + the open window's sums) * f
+    auto take_window = [&](float f) {
+#pragma unroll
+      for (int c = 0; c < H; c += 16) {
+        uint32_t o[16], ol[16];
+        tmem_ld16(t_o + c, o);
+        tmem_ld16(t_ol + c, ol);
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          tot[c + k] = (tot[c + k] + (__uint_as_float(o[k]) + __uint_as_float(ol[k]))) * f;
+      }
+    };
+    auto wait_od = [&](int j) {  // P.V of tile j is done
+      return mbar_wait_warp(bar(B_OD + (j & 3)), (j >> 2) & 1, abort_flag);
+    };
     for (int i = grp; i < nkt; i += 2) {
       const uint32_t t_s = t_row + S::COL_S + grp * BK;
       if (!mbar_wait_warp(bar(B_SF), (i >> 1) & 1, abort_flag)) {
@@ -359,14 +409,18 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       const bool resc = mt > m + kRescaleLog2;
       const float alpha = resc ? ex2(m - mt) : 1.0f;  // 0 from no keys yet
+      if (m != mine) {
+        const float f = ex2(mine - m);
+        l *= f;
+#pragma unroll
+        for (int k = 0; k < H; ++k) tot[k] *= f;
+      }
       if (resc) m = mt;
       m_s[r] = m;
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(B_MX + grp));
-      if (m != mine) {
-        l *= ex2(mine - m);
-        mine = m;
-      }
+      l *= alpha;
+      mine = m;  // (tot follows below)
       const float mu = m == -INFINITY ? 0.0f : m;
       float sum0 = 0.0f, sum1 = 0.0f;
       uint32_t hw[32], lw[32];
@@ -381,60 +435,59 @@ __global__ void __launch_bounds__(THREADS, 1)
         lw[j / 2] = pack_h2(p0 - h0, p1 - h1);
       }
       l += sum0 + sum1;
-      // P and the output belong to the previous tile until its P.V is done.  A
-      // window that it closed goes into the sum; a raised maximum rescales what
-      // there is.
-      if (i > 0 && !mbar_wait_warp(bar(B_OD + ((i - 1) & 1)), ((i - 1) >> 1) & 1, abort_flag)) {
+      // The P buffer is free once P.V two tiles ago is done.
+      if (i >= 2 && !wait_od(i - 2)) {
         ok = false;
         break;
       }
+      tc_fence_after();
+      tmem_st32(t_p, hw);
+      tmem_st32(t_p + 32, lw);
+      // A window that tile i - 1 closed goes into the sums, half of the dims by
+      // each group; a raised maximum rescales what there is.  Both once P.V of
+      // that tile is done.
       const bool flush = i > 0 && i % kWindow == 0;
-      const bool have_total = i > kWindow;  // before this tile's flush
       if (flush || (i > 0 && __any_sync(0xffffffffu, resc))) {
+        if (!wait_od(i - 1)) {
+          ok = false;
+          break;
+        }
         tc_fence_after();
+        if (flush) {
+          take_window(alpha);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(B_FL));
+        } else {
+#pragma unroll
+          for (int k = 0; k < H; ++k) tot[k] *= alpha;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          uint32_t o[16], ol[16], ot[16];
-          tmem_ld16(t_row + S::COL_O + c, o);
-          tmem_ld16(t_row + S::COL_OL + c, ol);
-          if (have_total) tmem_ld16(t_row + S::COL_OT + c, ot);
-          tmem_wait_ld();
-          if (flush) {
+          for (int c = 0; c < 2 * D; c += 16) {  // O and O_lo are neighbours
+            uint32_t o[16];
+            tmem_ld16(t_row + S::COL_O + c, o);
+            tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const float w = __uint_as_float(o[k]) + __uint_as_float(ol[k]);
-              ot[k] = __float_as_uint((have_total ? __uint_as_float(ot[k]) + w : w) * alpha);
-            }
-            tmem_st16(t_row + S::COL_OT + c, ot);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-              ol[k] = __float_as_uint(__uint_as_float(ol[k]) * alpha);
-            }
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
             tmem_st16(t_row + S::COL_O + c, o);
-            tmem_st16(t_row + S::COL_OL + c, ol);
-            if (have_total) {
-#pragma unroll
-              for (int k = 0; k < 16; ++k) ot[k] = __float_as_uint(__uint_as_float(ot[k]) * alpha);
-              tmem_st16(t_row + S::COL_OT + c, ot);
-            }
           }
         }
-        tmem_wait_st();
       }
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const int sw = (c ^ (r & 7)) << 4;
-        *reinterpret_cast<uint4 *>(prow + sw) =
-            make_uint4(hw[4 * c], hw[4 * c + 1], hw[4 * c + 2], hw[4 * c + 3]);
-        *reinterpret_cast<uint4 *>(prow + S::P_BYTES + sw) =
-            make_uint4(lw[4 * c], lw[4 * c + 1], lw[4 * c + 2], lw[4 * c + 3]);
-      }
-      fence_proxy_async();
+      tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(B_PF + grp));
+      // The other group's half of a window that tile i closes.
+      if ((i + 1) % kWindow == 0 && i + 1 < nkt) {
+        if (!wait_od(i)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        take_window(1.0f);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_FL));
+      }
     }
     // The last maximum, both groups' sums relative to it, and the last P.V.
     float m = -INFINITY;
@@ -442,11 +495,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       ok = false;
     if (ok) {
       m = m_s[r];
-      if (m != mine) l *= ex2(mine - m);
+      if (m != mine) {
+        const float f = ex2(mine - m);
+        l *= f;
+#pragma unroll
+        for (int k = 0; k < H; ++k) tot[k] *= f;
+      }
       l_s[grp * ROWS + r] = l;
     }
-    if (ok && !mbar_wait_warp(bar(B_OD + ((nkt - 1) & 1)), ((nkt - 1) >> 1) & 1, abort_flag))
-      ok = false;
+    if (ok && !wait_od(nkt - 1)) ok = false;
     if (!ok && lane == 0) fail();
     asm volatile("bar.sync 1, 256;" ::: "memory");
     if (ok) {
@@ -463,27 +520,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         orow = p.part + (size_t)p.T * p.Hq * p.nsplit * 2 + slot * D;
         if (grp == 0) reinterpret_cast<float2 *>(p.part)[slot] = make_float2(m, l);
       }
-      const bool have_total = nkt > kWindow;
-#pragma unroll 1
-      for (int c = grp * (D / 2); c < (grp + 1) * (D / 2); c += 16) {
-        uint32_t o[16], ol[16], ot[16];
-        tmem_ld16(t_row + S::COL_O + c, o);
-        tmem_ld16(t_row + S::COL_OL + c, ol);
-        if (have_total) tmem_ld16(t_row + S::COL_OT + c, ot);
-        tmem_wait_ld();
-        if (valid) {
-          float w[16];
+      take_window(f);
+      if (valid) {
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            w[k] = __uint_as_float(o[k]) + __uint_as_float(ol[k]);
-            if (have_total) w[k] += __uint_as_float(ot[k]);
-            w[k] *= f;
-          }
-#pragma unroll
-          for (int k = 0; k < 16; k += 4)
-            *reinterpret_cast<float4 *>(orow + c + k) =
-                make_float4(w[k], w[k + 1], w[k + 2], w[k + 3]);
-        }
+        for (int k = 0; k < H; k += 4)
+          *reinterpret_cast<float4 *>(orow + grp * H + k) =
+              make_float4(tot[k], tot[k + 1], tot[k + 2], tot[k + 3]);
       }
     }
   }
@@ -752,6 +794,12 @@ cudaError_t launch(const Kv4PromptArgs &a, char *base, const Scratch &sc, cudaSt
   p.err = a.err; p.rowf = rowf; p.bits = bits;
   e = cudaFuncSetAttribute(k_attn_kv4_tc<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
   if (e != cudaSuccess) return e;
+  // The register split needs the count that the kernel was to be compiled to.
+  static const int regs = [] {
+    cudaFuncAttributes fa;
+    return cudaFuncGetAttributes(&fa, k_attn_kv4_tc<D>) == cudaSuccess ? fa.numRegs : 0;
+  }();
+  if (regs < kRegs) return cudaErrorInvalidConfiguration;
   count_launch();
   k_attn_kv4_tc<D><<<dim3(p.ntiles_rows, Hkv, p.nsplit), THREADS, S::SMEM, s>>>(mQh, mQl, mKh, mKl,
                                                                                mVh, mVl, p);
