@@ -349,8 +349,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int k = 0; k < H; ++k) tot[k] = 0.0f;
     float mine = -INFINITY, l = 0.0f;  // l: this group's tiles, relative to `mine`
     bool ok = true;
-    // (tot + the open window's sums) * f
-    auto take_window = [&](float f) {
+    // tot * f1 and the window's sums, times f2
+    auto take_window = [&](float f1, float f2) {
 #pragma unroll
       for (int c = 0; c < H; c += 16) {
         uint32_t o[16], ol[16];
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_wait_ld();
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-          tot[c + k] = (tot[c + k] + (__uint_as_float(o[k]) + __uint_as_float(ol[k]))) * f;
+          tot[c + k] = fmaf(tot[c + k], f1, __uint_as_float(o[k]) + __uint_as_float(ol[k])) * f2;
       }
     };
     auto wait_od = [&](int j) {  // P.V of tile j is done
@@ -409,18 +409,21 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       const bool resc = mt > m + kRescaleLog2;
       const float alpha = resc ? ex2(m - mt) : 1.0f;  // 0 from no keys yet
-      if (m != mine) {
-        const float f = ex2(mine - m);
-        l *= f;
-#pragma unroll
-        for (int k = 0; k < H; ++k) tot[k] *= f;
-      }
+      const float sync = m != mine ? ex2(mine - m) : 1.0f;  // 0 from no keys yet
       if (resc) m = mt;
       m_s[r] = m;
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(B_MX + grp));
-      l *= alpha;
-      mine = m;  // (tot follows below)
+      mine = m;
+      l *= sync * alpha;
+      // A pair whose first tile begins a window: the last one's sums are taken
+      // below, before P.V of that tile overwrites them.
+      const int i0 = i & ~1;
+      const bool take = i0 > 0 && i0 % kWindow == 0;
+      if (!take && __any_sync(0xffffffffu, sync * alpha != 1.0f)) {
+#pragma unroll
+        for (int k = 0; k < H; ++k) tot[k] *= sync * alpha;
+      }
       const float mu = m == -INFINITY ? 0.0f : m;
       float sum0 = 0.0f, sum1 = 0.0f;
       uint32_t hw[32], lw[32];
@@ -443,50 +446,53 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_after();
       tmem_st32(t_p, hw);
       tmem_st32(t_p + 32, lw);
-      // A window that tile i - 1 closed goes into the sums, half of the dims by
-      // each group; a raised maximum rescales what there is.  Both once P.V of
-      // that tile is done.
-      const bool flush = i > 0 && i % kWindow == 0;
-      if (flush || (i > 0 && __any_sync(0xffffffffu, resc))) {
+      if (take) {
+        if (!wait_od(i0 - 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        // The window is relative to the maximum as tile i0 - 1 left it: what group
+        // 0 has read, and group 1's own last one.
+        take_window(grp == 0 ? sync : 1.0f, grp == 0 ? alpha : sync * alpha);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_FL));
+      }
+      // A raised maximum rescales the open window, once the previous tile's P.V is
+      // done.
+      if (i > 0 && !(take && grp == 0) && __any_sync(0xffffffffu, resc)) {
         if (!wait_od(i - 1)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        if (flush) {
-          take_window(alpha);
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(B_FL));
-        } else {
-#pragma unroll
-          for (int k = 0; k < H; ++k) tot[k] *= alpha;
 #pragma unroll 1
-          for (int c = 0; c < 2 * D; c += 16) {  // O and O_lo are neighbours
-            uint32_t o[16];
-            tmem_ld16(t_row + S::COL_O + c, o);
-            tmem_wait_ld();
+        for (int c = 0; c < 2 * D; c += 16) {  // O and O_lo are neighbours
+          uint32_t o[16];
+          tmem_ld16(t_row + S::COL_O + c, o);
+          tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            tmem_st16(t_row + S::COL_O + c, o);
-          }
+          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+          tmem_st16(t_row + S::COL_O + c, o);
         }
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(B_PF + grp));
-      // The other group's half of a window that tile i closes.
-      if ((i + 1) % kWindow == 0 && i + 1 < nkt) {
-        if (!wait_od(i)) {
-          ok = false;
-          break;
-        }
+    }
+    // A window that begins with an odd last tile: group 1 has no tile to take the
+    // last one's sums at.
+    if (ok && grp == 1 && (nkt & 1) && nkt > 1 && (nkt - 1) % kWindow == 0) {
+      if (wait_od(nkt - 2)) {
         tc_fence_after();
-        take_window(1.0f);
+        take_window(1.0f, 1.0f);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_FL));
+      } else {
+        ok = false;
       }
     }
     // The last maximum, both groups' sums relative to it, and the last P.V.
@@ -520,7 +526,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         orow = p.part + (size_t)p.T * p.Hq * p.nsplit * 2 + slot * D;
         if (grp == 0) reinterpret_cast<float2 *>(p.part)[slot] = make_float2(m, l);
       }
-      take_window(f);
+      take_window(1.0f, f);
       if (valid) {
 #pragma unroll
         for (int k = 0; k < H; k += 4)
