@@ -38,8 +38,9 @@
 // pair n, so the tensor pipe has work while the softmax of pair n runs.  Shared memory is what
 // bounds this: an MMA of 128 x 128 x 16 reads 8 KB of it in 64 cycles, all that
 // there is, beside the copies that bring K and V.  (P through shared memory, in one
-// buffer: 417 us for 509 tokens of 72B on 7680.)  The
-// running maximum is handed from tile to tile through shared memory; it is only
+// buffer, and one issuing warp: 417 us for 509 tokens of 72B on 7680, against 322.)  The
+// running maximum is handed from tile to tile through shared memory, by a tagged
+// word per row (a barrier's wait took 300 to 800 cycles there); it is only
 // raised by a score more than 2^8 above it.  Every wait is bounded (about 2 s;
 // SI_ERR_TIMEOUT in the context's error word); on expiry every role stops, the
 // CTA's own copies and MMAs in flight are waited for (bounded) and TMEM is freed.
@@ -63,7 +64,7 @@ constexpr int THREADS = 384;
 constexpr int kRegs = 168, kRegsControl = 56, kRegsSoftmax = 224;
 static_assert(THREADS * kRegs >= 128 * kRegsControl + 256 * kRegsSoftmax, "register split");
 constexpr float kRescaleLog2 = 8.0f;
-constexpr int kWindow = 4;  // tiles per window
+constexpr int kWindow = 6;  // tiles per window
 constexpr int kMaxSplits = 32;
 
 template <int D>
@@ -75,12 +76,12 @@ struct Shape {
   static constexpr int K_BYTES = NC * K_CHUNK;    // one split of a pair of K tiles
   static constexpr int V_BYTES = D * 128;         // one split of a V^T tile
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_K = OFF_Q + 2 * Q_BYTES;        // [hi, lo]
-  static constexpr int OFF_V = OFF_K + 2 * K_BYTES;        // [stage][hi, lo]
+  static constexpr int OFF_K = OFF_Q + 2 * Q_BYTES;        // ring of three: lo, hi, lo, ...
+  static constexpr int OFF_V = OFF_K + 3 * K_BYTES;        // [stage][hi, lo]
   static constexpr int OFF_BAR = OFF_V + 4 * V_BYTES;
-  static constexpr int OFF_M = OFF_BAR + 256;              // running maximum per row
-  static constexpr int OFF_L = OFF_M + ROWS * 4;           // row sums of the two groups
-  static constexpr int SMEM = OFF_L + 2 * ROWS * 4 + 1024;
+  static constexpr int OFF_M = OFF_BAR + 256;              // (running maximum, tile) per row
+  static constexpr int OFF_L = OFF_M;                      // later: row sums of the two groups
+  static constexpr int SMEM = OFF_M + ROWS * 8 + 1024;
   static constexpr uint32_t COL_S = 0, COL_P = 128, COL_O = 256, COL_OL = 256 + D;
 };
 static_assert(Shape<128>::SMEM <= 232448, "shared memory budget");
@@ -183,16 +184,20 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::OFF_BAR);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  constexpr int B_Q = 0, B_KF = 1, B_KE = 2, B_SF = 3, B_SE = 4, B_VF = 5, B_VE = 7, B_PF = 9,
-                B_MX = 11, B_OD = 13, B_FL = 17, B_FIN = 18, NBAR = 20;
+  constexpr int B_Q = 0, B_KF = 1, B_KE = 4, B_SF = 7, B_SE = 8, B_VF = 9, B_VE = 11, B_PF = 13,
+                B_OD = 15, B_FL = 19, B_FIN = 20, NBAR = 22;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + S::OFF_BAR + NBAR * 8);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + S::OFF_BAR + NBAR * 8 + 16);
-  float *m_s = reinterpret_cast<float *>(smem + S::OFF_M);
+  // A row's maximum as a tile left it, with the tile: one 8-byte word, which the
+  // next tile's thread of the row polls.
+  volatile unsigned long long *m_s =
+      reinterpret_cast<volatile unsigned long long *>(smem + S::OFF_M);
   float *l_s = reinterpret_cast<float *>(smem + S::OFF_L);
 
+  if (threadIdx.x < ROWS) m_s[threadIdx.x] = ~0ull;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NBAR; ++i)
-      mbar_init(bar(i), i == B_SE || i == B_FL ? 8 : i >= B_PF && i < B_OD ? 4 : 1);
+      mbar_init(bar(i), i == B_SE || i == B_FL ? 8 : i >= B_PF && i < B_OD ? 4 : 1);  // warps
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -222,21 +227,24 @@ __global__ void __launch_bounds__(THREADS, 1)
           tma_load_3d(qb + c * S::Q_CHUNK, &tmQh, c * 64, g * p.G, t0, bar(B_Q));
           tma_load_3d(qb + S::Q_BYTES + c * S::Q_CHUNK, &tmQl, c * 64, g * p.G, t0, bar(B_Q));
         }
-        int n = 0;
-        for (; n < npair; ++n) {
-          if (!mbar_wait(bar(B_KE), (n & 1) ^ 1, abort_flag)) break;
-          mbar_expect_tx(bar(B_KF), 2 * S::K_BYTES);
+        // K in units of a pair's lo, then its hi, through a ring of three: the next
+        // lo is there when a pair's scores begin, its hi follows into the place of
+        // the present lo, which the first third of the MMAs has read.
+        int u = 0;
+        for (; u < 2 * npair; ++u) {
+          const int s = u % 3;
+          if (!mbar_wait(bar(B_KE + s), ((u / 3) & 1) ^ 1, abort_flag)) break;
+          mbar_expect_tx(bar(B_KF + s), S::K_BYTES);
           // (rows past this head's are read with an odd last tile, and not used)
-          const int krow = g * p.Lp + (kt0 + 2 * n) * BK;
-          for (int c = 0; c < S::NC; ++c) {
-            tma_load_2d(kb + c * S::K_CHUNK, &tmKh, c * 64, krow, bar(B_KF));
-            tma_load_2d(kb + S::K_BYTES + c * S::K_CHUNK, &tmKl, c * 64, krow, bar(B_KF));
-          }
+          const int krow = g * p.Lp + (kt0 + (u & ~1)) * BK;
+          for (int c = 0; c < S::NC; ++c)
+            tma_load_2d(kb + s * S::K_BYTES + c * S::K_CHUNK, u & 1 ? &tmKh : &tmKl, c * 64, krow,
+                        bar(B_KF + s));
         }
-        if (n < npair) {
+        if (u < 2 * npair) {
           fail();
           mbar_drain(bar(B_Q), 0);
-          if (n > 0) mbar_drain(bar(B_KF), (n - 1) & 1);
+          for (int k = u > 3 ? u - 3 : 0; k < u; ++k) mbar_drain(bar(B_KF + k % 3), (k / 3) & 1);
         }
       }
       __syncwarp();
@@ -262,31 +270,40 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ---------------- S issuer ----------------
       if (lane == 0) {
         const uint32_t qh = smem_u32(smem + S::OFF_Q), ql = qh + S::Q_BYTES;
-        const uint32_t kh = smem_u32(smem + S::OFF_K), kl = kh + S::K_BYTES;
+        const uint32_t kb = smem_u32(smem + S::OFF_K);
         constexpr uint32_t id_s = idesc_f16(ROWS, PK);
         bool ok = mbar_wait(bar(B_Q), 0, abort_flag);
         for (int n = 0; ok && n < npair; ++n) {
-          // The scores of two tiles, over those that the softmax warps have read.
-          if (n >= 1 ? !mbar_wait2(bar(B_KF), n & 1, bar(B_SE), (n - 1) & 1, abort_flag)
-                     : !mbar_wait(bar(B_KF), 0, abort_flag)) {
+          // The scores of two tiles, over those that the softmax warps have read;
+          // small products first.
+          const int ul = 2 * n, uh = 2 * n + 1;
+          const uint32_t kl = kb + ul % 3 * S::K_BYTES, kh = kb + uh % 3 * S::K_BYTES;
+          const int full = bar(B_KF + ul % 3), par = (ul / 3) & 1;
+          if (n >= 1 ? !mbar_wait2(full, par, bar(B_SE), (n - 1) & 1, abort_flag)
+                     : !mbar_wait(full, par, abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          uint32_t acc = 0;
-#pragma unroll
-          for (int pass = 0; pass < 3; ++pass) {  // small products first
-            const uint32_t a = pass == 1 ? ql : qh, b = pass == 0 ? kl : kh;
+          auto pass = [&](uint32_t a, uint32_t b, uint32_t acc) {
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               const uint32_t off = (k & 3) * 32;
               mma_f16(tmem + S::COL_S, smem_desc(a + (k >> 2) * S::Q_CHUNK + off),
-                      smem_desc(b + (k >> 2) * S::K_CHUNK + off), id_s, acc);
-              acc = 1;
+                      smem_desc(b + (k >> 2) * S::K_CHUNK + off), id_s, k ? 1u : acc);
             }
+          };
+          pass(qh, kl, 0);
+          mma_commit(bar(B_KE + ul % 3));
+          if (!mbar_wait(bar(B_KF + uh % 3), (uh / 3) & 1, abort_flag)) {
+            ok = false;
+            break;
           }
+          tc_fence_after();
+          pass(ql, kh, 1);
+          pass(qh, kh, 1);
           mma_commit(bar(B_SF));
-          mma_commit(bar(B_KE));
+          mma_commit(bar(B_KE + uh % 3));
         }
         if (!ok) fail();
         mma_commit(bar(B_FIN));
@@ -352,15 +369,31 @@ __global__ void __launch_bounds__(THREADS, 1)
     // tot * f1 and the window's sums, times f2
     auto take_window = [&](float f1, float f2) {
 #pragma unroll
-      for (int c = 0; c < H; c += 16) {
-        uint32_t o[16], ol[16];
-        tmem_ld16(t_o + c, o);
-        tmem_ld16(t_ol + c, ol);
+      for (int c = 0; c < H; c += 32) {
+        uint32_t o[32], ol[32];
+        tmem_ld32(t_o + c, o);
+        tmem_ld32(t_ol + c, ol);
         tmem_wait_ld();
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
+        for (int k = 0; k < 32; ++k)
           tot[c + k] = fmaf(tot[c + k], f1, __uint_as_float(o[k]) + __uint_as_float(ol[k])) * f2;
       }
+    };
+    // The row's maximum as tile j left it (bounded as the other waits).
+    auto max_of = [&](int j, float &m) {
+      unsigned long long w = m_s[r];
+      if (__any_sync(0xffffffffu, (uint32_t)(w >> 32) != (uint32_t)j)) {
+        const uint64_t begin = globaltimer();
+        bool here;
+        do {
+          w = m_s[r];
+          here = (uint32_t)(w >> 32) == (uint32_t)j;
+        } while (!__all_sync(0xffffffffu, here) &&
+                 !__any_sync(0xffffffffu, *abort_flag || globaltimer() - begin > 2000000000ull));
+        if (!__all_sync(0xffffffffu, here)) return false;
+      }
+      m = __uint_as_float((uint32_t)w);
+      return true;
     };
     auto wait_od = [&](int j) {  // P.V of tile j is done
       return mbar_wait_warp(bar(B_OD + (j & 3)), (j >> 2) & 1, abort_flag);
@@ -400,20 +433,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       mt = mt == -INFINITY ? mt : mt * rf;
       // The maximum as the previous tile left it, raised if need be, passed on.
       float m = -INFINITY;
-      if (i > 0) {
-        if (!mbar_wait_warp(bar(B_MX + ((i - 1) & 1)), ((i - 1) >> 1) & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
-        m = m_s[r];
+      if (i > 0 && !max_of(i - 1, m)) {
+        ok = false;
+        break;
       }
       const bool resc = mt > m + kRescaleLog2;
       const float alpha = resc ? ex2(m - mt) : 1.0f;  // 0 from no keys yet
       const float sync = m != mine ? ex2(mine - m) : 1.0f;  // 0 from no keys yet
       if (resc) m = mt;
-      m_s[r] = m;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(B_MX + grp));
+      m_s[r] = ((unsigned long long)(uint32_t)i << 32) | __float_as_uint(m);
       mine = m;
       l *= sync * alpha;
       // A pair whose first tile begins a window: the last one's sums are taken
@@ -497,20 +525,17 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     // The last maximum, both groups' sums relative to it, and the last P.V.
     float m = -INFINITY;
-    if (ok && !mbar_wait_warp(bar(B_MX + ((nkt - 1) & 1)), ((nkt - 1) >> 1) & 1, abort_flag))
-      ok = false;
-    if (ok) {
-      m = m_s[r];
-      if (m != mine) {
-        const float f = ex2(mine - m);
-        l *= f;
+    if (ok && !max_of(nkt - 1, m)) ok = false;
+    if (ok && m != mine) {
+      const float f = ex2(mine - m);
+      l *= f;
 #pragma unroll
-        for (int k = 0; k < H; ++k) tot[k] *= f;
-      }
-      l_s[grp * ROWS + r] = l;
+      for (int k = 0; k < H; ++k) tot[k] *= f;
     }
     if (ok && !wait_od(nkt - 1)) ok = false;
     if (!ok && lane == 0) fail();
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // the maxima are read
+    l_s[grp * ROWS + r] = l;
     asm volatile("bar.sync 1, 256;" ::: "memory");
     if (ok) {
       tc_fence_after();
