@@ -516,9 +516,16 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
   }
 }
 
-// Splits of a token merged in order: grid (Hq, T), a thread per dim.
+// Splits of a token merged: grid (Hq, T).  A warp takes every eighth split, a lane
+// four dims (D = 64: half a warp a split), all its loads in flight; the warps'
+// sums are then added in order.
+constexpr int kCombineWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(D) k_kv4_combine(const __grid_constant__ Kv4AttnArgs a) {
+__global__ void __launch_bounds__(kCombineWarps * 32)
+    k_kv4_combine(const __grid_constant__ Kv4AttnArgs a) {
+  constexpr int LPR = D / 4, GROUPS = kCombineWarps * 32 / LPR;  // splits read at once
+  __shared__ float4 o_s[GROUPS][LPR];
+  __shared__ float l_s[GROUPS], m_s[kCombineWarps];
   pdl_trigger();
   pdl_wait();
   const Token tk = token_of(a, blockIdx.y);
@@ -528,17 +535,39 @@ __global__ void __launch_bounds__(D) k_kv4_combine(const __grid_constant__ Kv4At
   const size_t slot = ((size_t)blockIdx.y * a.n_q_heads + blockIdx.x) * a.nsplit;
   const float2 *ml = reinterpret_cast<const float2 *>(a.part) + slot;
   const float *po = a.part + (size_t)gridDim.y * a.n_q_heads * a.nsplit * 2 + slot * D;
+  const int grp = threadIdx.x / LPR, c = threadIdx.x % LPR;
   float M = -INFINITY;
-  for (int i = 0; i < ns; ++i) M = fmaxf(M, ml[i].x);
+  for (int i = threadIdx.x; i < ns; i += blockDim.x) M = fmaxf(M, ml[i].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  if ((threadIdx.x & 31) == 0) m_s[threadIdx.x >> 5] = M;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kCombineWarps; ++w) M = fmaxf(M, m_s[w]);
   const float Mu = M == -INFINITY ? 0.0f : M;
-  float L = 0.0f, o = 0.0f;
-  for (int i = 0; i < ns; ++i) {
+  float L = 0.0f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = grp; i < ns; i += GROUPS) {
     const float2 x = ml[i];
+    const float4 y = *reinterpret_cast<const float4 *>(po + (size_t)i * D + 4 * c);
     const float f = ex2(x.x - Mu);
     L = fmaf(x.y, f, L);
-    o = fmaf(po[(size_t)i * D + threadIdx.x], f, o);
+    o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y);
+    o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
   }
-  a.out[((size_t)tk.row * a.n_q_heads + blockIdx.x) * D + threadIdx.x] = L == 0.0f ? 0.0f : o / L;
+  o_s[grp][c] = o;
+  if (c == 0) l_s[grp] = L;
+  __syncthreads();
+  if (grp) return;
+  for (int i = 1; i < GROUPS; ++i) {
+    const float4 y = o_s[i][c];
+    o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
+    L += l_s[i];
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  *reinterpret_cast<float4 *>(a.out + ((size_t)tk.row * a.n_q_heads + blockIdx.x) * D + 4 * c) =
+      make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 template <int D>
@@ -550,7 +579,7 @@ cudaError_t launch(Kv4AttnArgs a, cudaStream_t s) {
   e = launch_pdl(k_attn_kv4<D>, dim3(a.nsplit, a.kv.n_kv_heads, a.T), dim3(kWarps * 32),
                  Shape<D>::SMEM, s, a);
   if (e != cudaSuccess || a.nsplit == 1) return e;
-  return launch_pdl(k_kv4_combine<D>, dim3(a.n_q_heads, a.T), dim3(D), 0, s, a);
+  return launch_pdl(k_kv4_combine<D>, dim3(a.n_q_heads, a.T), dim3(kCombineWarps * 32), 0, s, a);
 }
 
 }  // namespace

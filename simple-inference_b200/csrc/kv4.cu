@@ -46,146 +46,180 @@ __device__ __forceinline__ int kv4_run_of(const Kv4Runs &r, int t) {
   return lo;
 }
 
-// One warp writes one row: lane = dim within each block of 32.  The codes of
-// four neighbouring lanes make a half-word, which lane 4g stores for its g.
+// A warp takes whole rows: lane j of the D/4 lanes of a row holds dims 4j ..
+// 4j + 3, one 16-byte load, which is one half-word of the row (block b = j / 8,
+// group g = j % 8), so a block's eight lanes find its extreme by three exchanges
+// and no code moves between lanes.  At D = 64 a warp takes two rows at once.
 template <int D>
-__device__ __forceinline__ void kv4_store_row(const float (&x)[D / 32], uint8_t *codes,
-                                              uint16_t *scales, int lane) {
+__device__ __forceinline__ void kv4_store_row(const float4 x, uint8_t *codes, uint16_t *scales,
+                                              int j) {
   constexpr int NB = D / 32;
-  uint32_t hw[NB];
-  uint16_t sc[NB];
+  const float v[4] = {x.x, x.y, x.z, x.w};
+  // The largest magnitude as bits (a NaN is largest of all), and the first value
+  // that has it.
+  uint32_t a[4], am = 0;
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    const uint32_t a = __float_as_uint(fabsf(x[b]));
-    const uint32_t amax = __reduce_max_sync(0xffffffffu, a);
-    const int first = __ffs(__ballot_sync(0xffffffffu, a == amax)) - 1;
-    const float m = __shfl_sync(0xffffffffu, x[b], first);
-    const float d = __fmul_rn(m, -0.125f);  // m / -8, exact
-    const float id = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
-    int q = __float2int_rz(__fadd_rn(__fmul_rn(x[b], id), 8.5f));
-    q = min(max(q, 0), 15);
-    uint32_t v = (uint32_t)q;
-    v |= __shfl_down_sync(0xffffffffu, v, 1) << 4;
-    v |= __shfl_down_sync(0xffffffffu, v, 2) << 8;
-    hw[b] = v & 0xffffu;
-    sc[b] = f32_to_f16(d);
+  for (int i = 0; i < 4; ++i) {
+    a[i] = __float_as_uint(fabsf(v[i]));
+    am = max(am, a[i]);
   }
-  if ((lane & 3) == 0) {
-    uint32_t *dst = reinterpret_cast<uint32_t *>(codes + (lane >> 2) * 2 * NB);
 #pragma unroll
-    for (int b = 0; b < NB; b += 2) dst[b / 2] = hw[b] | (hw[b + 1] << 16);
+  for (int o = 1; o < 8; o <<= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, o));
+  float own = v[3];
+#pragma unroll
+  for (int i = 2; i >= 0; --i)
+    if (a[i] == am) own = v[i];
+  const bool has = a[0] == am || a[1] == am || a[2] == am || a[3] == am;
+  const int lane = threadIdx.x & 31, base = lane & ~7;
+  const uint32_t who = (__ballot_sync(0xffffffffu, has) >> base) & 0xffu;
+  const float m = __shfl_sync(0xffffffffu, own, base + __ffs(who) - 1);
+  const float d = __fmul_rn(m, -0.125f);  // m / -8, exact
+  const float id = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int q = __float2int_rz(__fadd_rn(__fmul_rn(v[i], id), 8.5f));
+    w |= (uint32_t)min(max(q, 0), 15) << (4 * i);
   }
-  if (lane == 0) {
-    uint32_t *dst = reinterpret_cast<uint32_t *>(scales);
-#pragma unroll
-    for (int b = 0; b < NB; b += 2) dst[b / 2] = sc[b] | ((uint32_t)sc[b + 1] << 16);
+  const int b = j >> 3, g = j & 7;
+  if (codes) {
+    reinterpret_cast<uint16_t *>(codes)[g * NB + b] = (uint16_t)w;
+    if (g == 0) scales[b] = f32_to_f16(d);
   }
 }
 
-// One warp per row: grid (tokens, ceil(units / 8)); units are the query heads
-// (rotated into q_out; none without q_out), then the K rows, then the V rows.
-// With tables the K rows and queries are rotated first (rope_kv.cu's
-// arithmetic).  A position without a page, or whose page other sequences hold
-// too, is not written and recorded as SI_ERR_INVALID.
+// CTAs of four warps, grid (tokens, ceil(units / kUnits)): a unit is a query head
+// (rotated into q_out; none without q_out), then the K rows, then the V rows of
+// the token; a warp loads its units before it works on them.  With tables the K
+// rows and queries are rotated first (rope_kv.cu's arithmetic).  A position
+// without a page, or whose page other sequences hold too, is not written and
+// recorded as SI_ERR_INVALID.
+constexpr int kUnits = 16;
+
 template <int D>
-__global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ Kv4AppendArgs a) {
+__global__ void __launch_bounds__(128) k_kv4_append(const __grid_constant__ Kv4AppendArgs a) {
   pdl_trigger();
   pdl_wait();
-  constexpr int NB = D / 32, HALF = D / 2;
-  const int t = blockIdx.x, lane = threadIdx.x & 31;
-  const int nq = a.q_out ? a.n_q_heads : 0, Hkv = a.kv.n_kv_heads;
-  const int u = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (u >= nq + 2 * Hkv) return;
+  constexpr int HALF = D / 2, LPR = D / 4, RPW = 32 / LPR;  // lanes per row, rows per warp
+  constexpr int N = kUnits / (4 * RPW);                     // row loads per warp
+  const int t = blockIdx.x, lane = threadIdx.x & 31, j = lane % LPR;
+  const int nq = a.q_out ? a.n_q_heads : 0, Hkv = a.kv.n_kv_heads, units = nq + 2 * Hkv;
   int seq, pos, row = t;
   if (a.tok_ctx) {
     seq = t;
     pos = a.tok_ctx[t] - 1;
   } else {
-    const int r = kv4_run_of(a.runs, a.runs.row0[0] + t);
     row = a.runs.row0[0] + t;
+    const int r = kv4_run_of(a.runs, row);
     seq = a.runs.seq[r];
     pos = a.runs.pos[r] + row - a.runs.row0[r];
   }
-  const bool is_v = u >= nq + Hkv;
-  const int head = u < nq ? u : (u - nq) % Hkv;
-  const float *src = u < nq ? a.q + (size_t)row * a.ldq + (size_t)u * D
-                            : (is_v ? a.v : a.k) + (size_t)row * a.ldkv + (size_t)head * D;
-  float x[NB];
+  const int u0 = blockIdx.y * kUnits + (threadIdx.x >> 5) * (N * RPW) + lane / LPR;
+  float4 x[N];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) x[b] = src[32 * b + lane];
-  if (a.cos_tab && !is_v) {
-    if (pos < 0 || pos >= a.max_positions) return;  // never read outside the tables
-    const float *ct = a.cos_tab + (size_t)pos * HALF, *st = a.sin_tab + (size_t)pos * HALF;
-#pragma unroll
-    for (int b = 0; b < NB / 2; ++b) {
-      const float c = ct[32 * b + lane], s = st[32 * b + lane];
-      const float x0 = x[b], x1 = x[b + NB / 2];
-      x[b] = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, s));
-      x[b + NB / 2] = __fadd_rn(__fmul_rn(x1, c), __fmul_rn(x0, s));
+  for (int k = 0; k < N; ++k) {
+    const int u = u0 + k * RPW;
+    x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (u < units) {
+      const int head = u < nq ? u : (u - nq) % Hkv;
+      const float *src = u < nq ? a.q + (size_t)row * a.ldq + (size_t)u * D
+                                : (u >= nq + Hkv ? a.v : a.k) + (size_t)row * a.ldkv + (size_t)head * D;
+      x[k] = a.vec ? *reinterpret_cast<const float4 *>(src + 4 * j)
+                   : make_float4(src[4 * j], src[4 * j + 1], src[4 * j + 2], src[4 * j + 3]);
     }
-  }
-  if (u < nq) {
-    float *q = a.q_out + ((size_t)row * a.n_q_heads + u) * D;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) q[32 * b + lane] = x[b];
-    return;
   }
   int page = 0;
-  uint8_t *g = kv4_group(a.kv, seq, pos, head, &page);
-  if (!g || a.kv.refs[page] != 1) {
-    if (lane == 0) raise_error(a.err, 1);
-    return;
+  uint8_t *grp = kv4_group(a.kv, seq, pos, 0, &page);
+  if (grp && a.kv.refs[page] != 1) grp = nullptr;
+  if (!grp && threadIdx.x == 0 && blockIdx.y == 0) raise_error(a.err, 1);
+  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (a.cos_tab) {
+    if (pos < 0 || pos >= a.max_positions) return;  // never read outside the tables
+    const int i = (4 * j) % HALF;
+    c = *reinterpret_cast<const float4 *>(a.cos_tab + (size_t)pos * HALF + i);
+    s = *reinterpret_cast<const float4 *>(a.sin_tab + (size_t)pos * HALF + i);
   }
+  const size_t head_bytes = (size_t)(a.kv.page_len / kKv4Group) * kv4_group_bytes(D);
   const int r16 = pos % kKv4Group;
-  g += is_v ? kv4_group_bytes(D) / 2 : 0;
-  kv4_store_row<D>(x, g + r16 * (D / 2),
-                   reinterpret_cast<uint16_t *>(g + kKv4Group * (D / 2)) + r16 * NB, lane);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int u = u0 + k * RPW;
+    const bool is_v = u >= nq + Hkv;
+    if (a.cos_tab) {
+      float4 y;  // the other half of the pair
+      y.x = __shfl_xor_sync(0xffffffffu, x[k].x, LPR / 2);
+      y.y = __shfl_xor_sync(0xffffffffu, x[k].y, LPR / 2);
+      y.z = __shfl_xor_sync(0xffffffffu, x[k].z, LPR / 2);
+      y.w = __shfl_xor_sync(0xffffffffu, x[k].w, LPR / 2);
+      if (!is_v) {
+        auto rot = [&](float own, float other, float c, float s) {
+          return j < LPR / 2 ? __fsub_rn(__fmul_rn(own, c), __fmul_rn(other, s))
+                             : __fadd_rn(__fmul_rn(own, c), __fmul_rn(other, s));
+        };
+        x[k] = make_float4(rot(x[k].x, y.x, c.x, s.x), rot(x[k].y, y.y, c.y, s.y),
+                           rot(x[k].z, y.z, c.z, s.z), rot(x[k].w, y.w, c.w, s.w));
+      }
+    }
+    if (u < nq)
+      *reinterpret_cast<float4 *>(a.q_out + ((size_t)row * a.n_q_heads + u) * D + 4 * j) = x[k];
+    uint8_t *codes = nullptr;
+    if (grp && u >= nq && u < units)
+      codes = grp + (u - nq) % Hkv * head_bytes + (is_v ? kv4_group_bytes(D) / 2 : 0);
+    kv4_store_row<D>(x[k], codes ? codes + r16 * (D / 2) : nullptr,
+                     codes ? reinterpret_cast<uint16_t *>(codes + kKv4Group * (D / 2)) + r16 * (D / 32)
+                           : nullptr,
+                     j);
+  }
 }
 
-// Rows back to fp32, one warp per row: grid (tokens, ceil(2 Hkv / 8)).  A
-// half-word's four values are one 16-byte store; the warp covers the row.  A
+// Rows back to fp32, laid out as above: grid (tokens, ceil(2 Hkv / kUnits)).  A
 // position without a page reads as zeros and is recorded.
 template <int D>
-__global__ void __launch_bounds__(256) k_kv4_read(const __grid_constant__ Kv4ReadArgs a) {
+__global__ void __launch_bounds__(128) k_kv4_read(const __grid_constant__ Kv4ReadArgs a) {
   pdl_trigger();
   pdl_wait();
-  constexpr int NB = D / 32;
-  const int lane = threadIdx.x & 31, Hkv = a.kv.n_kv_heads;
-  const int u = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (u >= 2 * Hkv) return;
-  const bool is_v = u >= Hkv;
-  float *out = is_v ? a.v : a.k;
-  if (!out) return;
-  const int row = a.runs.row0[0] + blockIdx.x, head = u % Hkv;
-  const int r = kv4_run_of(a.runs, row);
+  constexpr int NB = D / 32, LPR = D / 4, RPW = 32 / LPR, N = kUnits / (4 * RPW);
+  const int lane = threadIdx.x & 31, j = lane % LPR, Hkv = a.kv.n_kv_heads;
+  const int row = a.runs.row0[0] + blockIdx.x, r = kv4_run_of(a.runs, row);
   const int pos = a.runs.pos[r] + row - a.runs.row0[r];
-  const uint8_t *g = kv4_group(a.kv, a.runs.seq[r], pos, head, nullptr);
-  if (!g && lane == 0) raise_error(a.err, 1);
-  out += ((size_t)row * Hkv + head) * D;
-  const int r16 = pos % kKv4Group;
-  if (g) g += is_v ? kv4_group_bytes(D) / 2 : 0;
+  const uint8_t *grp = kv4_group(a.kv, a.runs.seq[r], pos, 0, nullptr);
+  if (!grp && threadIdx.x == 0 && blockIdx.y == 0) raise_error(a.err, 1);
+  const size_t head_bytes = (size_t)(a.kv.page_len / kKv4Group) * kv4_group_bytes(D);
+  const int r16 = pos % kKv4Group, b = j >> 3, g = j & 7;
+  const int u0 = blockIdx.y * kUnits + (threadIdx.x >> 5) * (N * RPW) + lane / LPR;
+  uint32_t w[N];
+  float sc[N];
 #pragma unroll
-  for (int i = 0; i < D / 4; i += 32) {
-    const int h = i + lane;
-    if (h >= D / 4) break;  // D = 64: 16 half-words
-    const int b = h % NB, gg = h / NB;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (g) {
-      const uint32_t w = reinterpret_cast<const uint16_t *>(g + r16 * (D / 2))[h];
-      const float s = f16_to_f32(
-          reinterpret_cast<const uint16_t *>(g + kKv4Group * (D / 2))[r16 * NB + b]);
-      o = make_float4(s * (float)((int)(w & 15) - 8), s * (float)((int)((w >> 4) & 15) - 8),
-                      s * (float)((int)((w >> 8) & 15) - 8), s * (float)((int)(w >> 12) - 8));
+  for (int k = 0; k < N; ++k) {
+    const int u = u0 + k * RPW;
+    w[k] = 0x8888u;
+    sc[k] = 0.0f;
+    if (grp && u < 2 * Hkv) {
+      const uint8_t *p = grp + u % Hkv * head_bytes + (u >= Hkv ? kv4_group_bytes(D) / 2 : 0);
+      w[k] = reinterpret_cast<const uint16_t *>(p + r16 * (D / 2))[g * NB + b];
+      sc[k] = f16_to_f32(reinterpret_cast<const uint16_t *>(p + kKv4Group * (D / 2))[r16 * NB + b]);
     }
-    *reinterpret_cast<float4 *>(out + 32 * b + 4 * gg) = o;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int u = u0 + k * RPW;
+    if (u >= 2 * Hkv) continue;
+    float *out = u >= Hkv ? a.v : a.k;
+    if (!out) continue;
+    *reinterpret_cast<float4 *>(out + ((size_t)row * Hkv + u % Hkv) * D + 4 * j) =
+        make_float4(sc[k] * (float)((int)(w[k] & 15) - 8), sc[k] * (float)((int)((w[k] >> 4) & 15) - 8),
+                    sc[k] * (float)((int)((w[k] >> 8) & 15) - 8), sc[k] * (float)((int)(w[k] >> 12) - 8));
   }
 }
 
 // Bookkeeping: entries and reference counts from kernel parameters (the host's
 // tables may change again at once), and page copies in the same launch: the
-// last CTA writes the entries, the others copy kCopyBytes each of a page.
+// last kWriters CTAs write the entries, the others copy kCopyBytes each of a
+// page.  The words are read through a generic pointer: as constants, whose lanes
+// read different addresses, they would come one at a time.
 constexpr int kCopyThreads = 256;
 constexpr int kCopyBytes = kCopyThreads * 16 * 4;
+constexpr int kWriters = 4;
 
 template <int WORDS>
 __global__ void __launch_bounds__(kCopyThreads)
@@ -193,19 +227,22 @@ __global__ void __launch_bounds__(kCopyThreads)
   pdl_trigger();
   pdl_wait();
   const int pieces = (int)((u.page_bytes + kCopyBytes - 1) / kCopyBytes);
-  if (blockIdx.x == gridDim.x - 1) {
-    for (int j = threadIdx.x >> 5; j < u.n_spans; j += kCopyThreads / 32) {
-      int *to = u.tables + u.word[3 * j];
-      const int n = u.word[3 * j + 1], from = u.word[3 * j + 2];
+  const int *word = u.word;
+  asm volatile("" : "+l"(word));
+  if (blockIdx.x >= gridDim.x - kWriters) {
+    const int w0 = blockIdx.x - (gridDim.x - kWriters), t0 = w0 * kCopyThreads + threadIdx.x;
+    for (int j = t0 >> 5; j < u.n_spans; j += kWriters * kCopyThreads / 32) {
+      int *to = u.tables + word[3 * j];
+      const int n = word[3 * j + 1], from = word[3 * j + 2];
       for (int i = threadIdx.x & 31; i < n; i += 32) to[i] = from < 0 ? -1 : u.tables[from + i];
     }
-    const int *w = u.word + 3 * u.n_spans;
-    for (int i = threadIdx.x; i < u.n_table; i += kCopyThreads) u.tables[w[2 * i]] = w[2 * i + 1];
+    const int *w = word + 3 * u.n_spans;
+    for (int i = t0; i < u.n_table; i += kWriters * kCopyThreads) u.tables[w[2 * i]] = w[2 * i + 1];
     w += 2 * u.n_table;
-    for (int i = threadIdx.x; i < u.n_refs; i += kCopyThreads) u.refs[w[2 * i]] = w[2 * i + 1];
+    for (int i = t0; i < u.n_refs; i += kWriters * kCopyThreads) u.refs[w[2 * i]] = w[2 * i + 1];
     return;
   }
-  const int *w = u.word + 3 * u.n_spans + 2 * (u.n_table + u.n_refs) +
+  const int *w = word + 3 * u.n_spans + 2 * (u.n_table + u.n_refs) +
                  2 * (blockIdx.x / pieces);
   const size_t off = (size_t)(blockIdx.x % pieces) * kCopyBytes;
   const uint8_t *src = u.pool + (size_t)w[0] * u.page_bytes + off;
@@ -229,22 +266,25 @@ __global__ void __launch_bounds__(kCopyThreads)
 cudaError_t launch_kv4_append(const Kv4AppendArgs &a, cudaStream_t s) {
   if (a.T <= 0) return cudaSuccess;
   const int units = (a.q_out ? a.n_q_heads : 0) + 2 * a.kv.n_kv_heads;
-  const dim3 grid(a.T, (units + 7) / 8);
-  return a.kv.head_dim == 128 ? launch_pdl(k_kv4_append<128>, grid, dim3(256), 0, s, a)
-                              : launch_pdl(k_kv4_append<64>, grid, dim3(256), 0, s, a);
+  const dim3 grid(a.T, (units + kUnits - 1) / kUnits);
+  Kv4AppendArgs b = a;
+  b.vec = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
+            reinterpret_cast<uintptr_t>(a.v) | 4 * a.ldq | 4 * a.ldkv) & 15) == 0;
+  return a.kv.head_dim == 128 ? launch_pdl(k_kv4_append<128>, grid, dim3(128), 0, s, b)
+                              : launch_pdl(k_kv4_append<64>, grid, dim3(128), 0, s, b);
 }
 
 cudaError_t launch_kv4_read(const Kv4ReadArgs &a, cudaStream_t s) {
   if (a.T <= 0) return cudaSuccess;
-  const dim3 grid(a.T, (2 * a.kv.n_kv_heads + 7) / 8);
-  return a.kv.head_dim == 128 ? launch_pdl(k_kv4_read<128>, grid, dim3(256), 0, s, a)
-                              : launch_pdl(k_kv4_read<64>, grid, dim3(256), 0, s, a);
+  const dim3 grid(a.T, (2 * a.kv.n_kv_heads + kUnits - 1) / kUnits);
+  return a.kv.head_dim == 128 ? launch_pdl(k_kv4_read<128>, grid, dim3(128), 0, s, a)
+                              : launch_pdl(k_kv4_read<64>, grid, dim3(128), 0, s, a);
 }
 
 template <int WORDS>
 static cudaError_t update(const Kv4Update<WORDS> &u, cudaStream_t s) {
   const int pieces = (int)((u.page_bytes + kCopyBytes - 1) / kCopyBytes);
-  return launch_pdl(k_kv4_update<WORDS>, dim3(u.n_copies * pieces + 1), dim3(kCopyThreads), 0, s,
+  return launch_pdl(k_kv4_update<WORDS>, dim3(u.n_copies * pieces + kWriters), dim3(kCopyThreads), 0, s,
                     u);
 }
 cudaError_t launch_kv4_update(const Kv4Update<kKv4SmallWords> &u, cudaStream_t s) {

@@ -236,6 +236,7 @@ struct Kv4AppendArgs {
   const float *cos_tab, *sin_tab;  // rotate K (and q) by position, or null
   int max_positions;
   int *err;
+  int vec;               // set by the launch: 16-byte loads
 };
 cudaError_t launch_kv4_append(const Kv4AppendArgs &a, cudaStream_t s);
 struct Kv4ReadArgs {
