@@ -42,6 +42,7 @@
 // takes about 800 instructions, of them 290 for unpacking the codes and 64
 // matrix instructions.
 #include <algorithm>
+#include <atomic>
 
 #include "si_common.cuh"
 #include "si_kernels.cuh"
@@ -56,6 +57,7 @@ constexpr int kMinSplit = kWarps * kTile;  // a split has at least one tile per 
 constexpr int kStages = 2;
 constexpr int kHeads = 8;                  // query heads of a KV group, at most
 constexpr int kCtasPerSm = 3;
+constexpr int kMaxCluster = 8;             // splits that are merged within the kernel
 constexpr float kStaleMax = 4.0f;          // log2 units a score may lie above the maximum
 
 template <int D>
@@ -70,8 +72,9 @@ struct Shape {
   static constexpr int RING = kWarps * kStages * TILE;
   static constexpr int MERGE = kWarps * kHeads * (OROW + 2) * 4;
   static constexpr int Q = NB * 2 * 32 * 16;         // query operand
-  static constexpr int AMAX = NB * kHeads * 4;
-  static constexpr int SMEM = Q + AMAX + (RING > MERGE ? RING : MERGE);
+  static constexpr int AMAX = (NB > 2 ? NB : 2) * kHeads * 4;  // later (m, l) per head
+  static constexpr int BARS = kWarps * kStages * 8;
+  static constexpr int SMEM = Q + AMAX + BARS + (RING > MERGE ? RING : MERGE);
 };
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x, relative error below 2^-22
@@ -118,6 +121,50 @@ __device__ __forceinline__ float half_at(const uint32_t *w, int i) {
 }
 __device__ __forceinline__ float pow2(int e) {  // 2^e, 0 below the normal range
   return e < -126 ? 0.0f : __int_as_float((e + 127) << 23);
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+// The whole warp waits for a stage's copies, 2 s at most.
+__device__ __forceinline__ bool wait_tile(uint32_t bar, uint32_t parity) {
+  bool ok = mbar_try(bar, parity);
+  if (!ok) {
+    const uint64_t t0 = globaltimer();
+    while (!(ok = mbar_try(bar, parity)) && globaltimer() - t0 < 2000000000ull) {}
+  }
+  return __all_sync(0xffffffffu, ok) != 0;
+}
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(const void *p, int cta) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(cta));
+  return r;
+}
+__device__ __forceinline__ float2 cluster_ld2(const float2 *p, int cta) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(cluster_addr(p, cta))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_ld4(const float *p, int cta) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr(p, cta))
+               : "memory");
+  return v;
 }
 
 struct Token {
@@ -175,7 +222,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
   extern __shared__ __align__(16) uint8_t smem_all[];
   uint4 *q_s = reinterpret_cast<uint4 *>(smem_all);                  // [NB][2][32 lanes]
   float *amax_s = reinterpret_cast<float *>(smem_all + S::Q);        // [NB][8 heads]
-  uint8_t *smem = smem_all + S::Q + S::AMAX;
+  uint8_t *smem = smem_all + S::Q + S::AMAX + S::BARS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;  // operand row (head) and column group
   pdl_trigger();
@@ -190,6 +237,16 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
   const int ntiles = (k1 - k0 + kTile - 1) / kTile;
   const int mine = ntiles > warp ? (ntiles - warp + kWarps - 1) / kWarps : 0;
 
+  // This warp's part of the query (see below), asked for before the tables.
+  float x[8] = {};
+  if (warp < NB && g < G) {
+    const float *q = a.q + ((size_t)tk.row * a.n_q_heads + (size_t)kvh * G + g) * D + 32 * warp + 8 * t;
+    const float4 u = *reinterpret_cast<const float4 *>(q);
+    const float4 v = *reinterpret_cast<const float4 *>(q + 4);
+    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+    x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+  }
+
   // Group addresses of this warp's tiles, 16 tiles at a time: lane j holds the
   // pool index of group j & 1 of tile j / 2 of the batch, -1 past the keys or
   // where the table has no page (which is recorded).
@@ -197,6 +254,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
   const int *table = a.kv.tables + (size_t)tk.seq * a.kv.max_pages;
   uint8_t *ring = smem + warp * (kStages * S::TILE);
   int gidx = -1;
+  const uint32_t bars = smem_u32(smem_all + S::Q + S::AMAX) + warp * (kStages * 8);
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) mbar_init(bars + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
   uint32_t okb = 0;  // group validity of the tiles in flight, 2 bits each
   auto issue = [&](int n) {
     if ((n & 15) == 0) {
@@ -215,37 +279,22 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
     const int g1 = __shfl_sync(0xffffffffu, gidx, (2 * n + 1) & 31);
     const int sh = (n & 15) * 2;
     okb = (okb & ~(3u << sh)) | ((uint32_t)(g0 >= 0) << sh) | ((uint32_t)(g1 >= 0) << (sh + 1));
-    const uint8_t *p0 = a.kv.pool + (size_t)(uint32_t)g0 * S::GB;
-    const uint8_t *p1 = a.kv.pool + (size_t)(uint32_t)g1 * S::GB;
-    const uint32_t dst = smem_u32(ring + (n % kStages) * S::TILE);
-#pragma unroll
-    for (int i = 0; i < (S::CHUNKS + 31) / 32; ++i) {
-      const int c = lane + 32 * i;
-      const bool second = c >= S::CHUNKS / 2;
-      const uint8_t *src = second ? p1 + (c - S::CHUNKS / 2) * 16 : p0 + c * 16;
-      if (c < S::CHUNKS && (second ? g1 : g0) >= 0)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c * 16), "l"(src)
-                     : "memory");
+    if (lane == 0) {
+      const uint32_t bar = bars + 8 * (n % kStages), dst = smem_u32(ring + (n % kStages) * S::TILE);
+      mbar_expect_tx(bar, (g0 >= 0 ? S::GB : 0) + (g1 >= 0 ? S::GB : 0));
+      if (g0 >= 0) bulk_load(dst, a.kv.pool + (size_t)(uint32_t)g0 * S::GB, S::GB, bar);
+      if (g1 >= 0) bulk_load(dst + S::GB, a.kv.pool + (size_t)(uint32_t)g1 * S::GB, S::GB, bar);
     }
   };
 #pragma unroll
   for (int n = 0; n < kStages - 1; ++n) {
     if (n < mine) issue(n);
-    asm volatile("cp.async.commit_group;" ::: "memory");
   }
 
   // The query operand: head g's values of dims 32b + 8t + 0..7, scaled and
   // split, block b by warp b.
   float sc;  // score in log2 units per unit of the accumulators
   {
-    float x[8] = {};
-    if (warp < NB && g < G) {
-      const float *q = a.q + ((size_t)tk.row * a.n_q_heads + (size_t)kvh * G + g) * D + 32 * warp + 8 * t;
-      const float4 u = *reinterpret_cast<const float4 *>(q);
-      const float4 v = *reinterpret_cast<const float4 *>(q + 4);
-      x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-      x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-    }
     if (warp < NB) {
       float am = 0.0f;
 #pragma unroll
@@ -288,9 +337,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
 
   for (int n = 0; n < mine; ++n) {
     if (n + kStages - 1 < mine) issue(n + kStages - 1);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-    __syncwarp();
+    if (!wait_tile(bars + 8 * (n % kStages), (n / kStages) & 1)) {
+      // The copies that are still under way are given as long again, then the
+      // warp stops.
+      if (lane == 0) raise_error(a.err, 6 /* SI_ERR_TIMEOUT */);
+      if (n + 1 < mine) wait_tile(bars + 8 * ((n + 1) % kStages), ((n + 1) / kStages) & 1);
+      break;
+    }
     uint8_t *st = ring + (n % kStages) * S::TILE;
     const int lim = k1 - (k0 + (warp + kWarps * n) * kTile);  // keys of this tile, >= 1
     const uint32_t ok2 = (okb >> ((n & 15) * 2)) & 3u;
@@ -306,6 +359,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
           reinterpret_cast<uint32_t *>(srow)[i] = 0;
           reinterpret_cast<uint32_t *>(srow + S::V_OFF)[i] = 0;
         }
+        fence_proxy_async();  // before the stage's next copy
       }
       __syncwarp();
     }
@@ -317,50 +371,52 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
 
     // Scores: n-tile (grp, nt) column c is key 16 grp + 8 nt + c / 2 + 4 (c & 1).
     float s[8];
+    {
+      uint32_t w[4][NB], d0[4][NB / 2], d1[4][NB / 2];
 #pragma unroll
-    for (int grp = 0; grp < 2; ++grp) {
-      const uint8_t *gp = st + grp * S::GB;
-      uint32_t w[2][NB], d0[2][NB / 2], d1[2][NB / 2];
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
+      for (int i = 0; i < 4; ++i) {  // n-tile (grp, nt) = (i / 2, i % 2)
+        const uint8_t *gp = st + (i >> 1) * S::GB;
+        const int nt = i & 1;
         const uint8_t *kr = gp + (8 * nt + (g >> 1) + 4 * (g & 1)) * (D / 2) + t * (4 * NB);
-        const uint8_t *sp = gp + S::S_OFF + (8 * nt + t) * (2 * NB);
+        const uint8_t *dp = gp + S::S_OFF + (8 * nt + t) * (2 * NB);
         if constexpr (NB == 4) {
           const uint4 r = *reinterpret_cast<const uint4 *>(kr);
-          w[nt][0] = __byte_perm(r.x, r.z, 0x5410);
-          w[nt][1] = __byte_perm(r.x, r.z, 0x7632);
-          w[nt][2] = __byte_perm(r.y, r.w, 0x5410);
-          w[nt][3] = __byte_perm(r.y, r.w, 0x7632);
-          const uint2 r0 = *reinterpret_cast<const uint2 *>(sp);
-          const uint2 r1 = *reinterpret_cast<const uint2 *>(sp + 4 * (2 * NB));
-          d0[nt][0] = r0.x; d0[nt][1] = r0.y; d1[nt][0] = r1.x; d1[nt][1] = r1.y;
+          w[i][0] = __byte_perm(r.x, r.z, 0x5410);
+          w[i][1] = __byte_perm(r.x, r.z, 0x7632);
+          w[i][2] = __byte_perm(r.y, r.w, 0x5410);
+          w[i][3] = __byte_perm(r.y, r.w, 0x7632);
+          const uint2 r0 = *reinterpret_cast<const uint2 *>(dp);
+          const uint2 r1 = *reinterpret_cast<const uint2 *>(dp + 4 * (2 * NB));
+          d0[i][0] = r0.x; d0[i][1] = r0.y; d1[i][0] = r1.x; d1[i][1] = r1.y;
         } else {
           const uint2 r = *reinterpret_cast<const uint2 *>(kr);
-          w[nt][0] = __byte_perm(r.x, r.y, 0x5410);
-          w[nt][1] = __byte_perm(r.x, r.y, 0x7632);
-          d0[nt][0] = *reinterpret_cast<const uint32_t *>(sp);
-          d1[nt][0] = *reinterpret_cast<const uint32_t *>(sp + 4 * (2 * NB));
+          w[i][0] = __byte_perm(r.x, r.y, 0x5410);
+          w[i][1] = __byte_perm(r.x, r.y, 0x7632);
+          d0[i][0] = *reinterpret_cast<const uint32_t *>(dp);
+          d1[i][0] = *reinterpret_cast<const uint32_t *>(dp + 4 * (2 * NB));
         }
       }
-      float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      float2 s2[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s2[i] = make_float2(0.f, 0.f);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const uint4 qa = q_s[(b * 2) * 32 + lane], qb = q_s[(b * 2 + 1) * 32 + lane];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
+        for (int i = 0; i < 4; ++i) {
           const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
           float c[4];
-          const uint32_t x = w[nt][b], h = x >> 8;
+          const uint32_t x = w[i][b], h = x >> 8;
           mma16816(c, qa.x, qa.y, qa.z, qa.w, codes_lo(x, one_k), codes_hi(x, one_k), zero);
           mma16816(c, qb.x, qb.y, qb.z, qb.w, codes_lo(h, one_k), codes_hi(h, one_k), c);
-          s2[nt] = fma2(make_float2(half_at(d0[nt], b), half_at(d1[nt], b)),
-                        add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), s2[nt]);
+          s2[i] = fma2(make_float2(half_at(d0[i], b), half_at(d1[i], b)),
+                       add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), s2[i]);
         }
       }
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        s[grp * 4 + nt * 2] = s2[nt].x * sc;
-        s[grp * 4 + nt * 2 + 1] = s2[nt].y * sc;
+      for (int i = 0; i < 4; ++i) {
+        s[2 * i] = s2[i].x * sc;
+        s[2 * i + 1] = s2[i].y * sc;
       }
     }
     if (!full) {
@@ -460,7 +516,6 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
     }
     __syncwarp();  // the stage may be refilled
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
   __syncthreads();
@@ -468,6 +523,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
   // Merge of the warps over the ring's memory.
   float *ow = reinterpret_cast<float *>(smem);
   float2 *ml = reinterpret_cast<float2 *>(smem + kWarps * kHeads * S::OROW * 4);
+  float2 *cta_ml = reinterpret_cast<float2 *>(amax_s);  // [8 heads]
   {
     const float f0 = mine ? ldexpf(1.0f, -(sp + dexp)) : 0.0f, f1 = f0 * 0.0625f;
     float *o = ow + (warp * kHeads + g) * S::OROW + 8 * t;
@@ -484,6 +540,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
     if (t == 0) ml[warp * kHeads + g] = make_float2(m, l);
   }
   __syncthreads();
+  // The CTA's sums over its warps go to the output (one split), to warp 0's place
+  // for the cluster's merge, or to the scratch.
   for (int i = threadIdx.x; i < G * (D / 4); i += kWarps * 32) {
     const int h = i / (D / 4), c = i % (D / 4);
     float M = -INFINITY;
@@ -506,6 +564,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
       const float inv = L == 0.0f ? 0.0f : 1.0f / L;
       *reinterpret_cast<float4 *>(a.out + ((size_t)tk.row * a.n_q_heads + head) * D + 4 * c) =
           make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    } else if (a.cluster) {
+      *reinterpret_cast<float4 *>(ow + h * S::OROW + 4 * c) = o;  // read by this thread alone
+      if (c == 0) cta_ml[h] = make_float2(M, L);
     } else {
       const size_t slot = ((size_t)blockIdx.z * a.n_q_heads + head) * a.nsplit + split;
       float2 *pml = reinterpret_cast<float2 *>(a.part);
@@ -514,6 +575,36 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
       *reinterpret_cast<float4 *>(po + slot * D + 4 * c) = o;
     }
   }
+  if (ns == 1 || !a.cluster) return;
+  // The splits of a token are one cluster: each CTA merges its share of the output
+  // from the others' shared memory, in the order of the splits.
+  cluster_sync_all();
+  for (int i = split * (kWarps * 32) + threadIdx.x; i < G * (D / 4); i += ns * (kWarps * 32)) {
+    const int h = i / (D / 4), c = i % (D / 4);
+    float2 x[kMaxCluster];
+    float M = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      x[r] = r < ns ? cluster_ld2(cta_ml + h, r) : make_float2(-INFINITY, 0.0f);
+      M = fmaxf(M, x[r].x);
+    }
+    const float Mu = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      if (r >= ns) break;
+      const float f = ex2(x[r].x - Mu);
+      const float4 y = cluster_ld4(ow + h * S::OROW + 4 * c, r);
+      L = fmaf(x[r].y, f, L);
+      o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y);
+      o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    *reinterpret_cast<float4 *>(a.out + ((size_t)tk.row * a.n_q_heads + (size_t)kvh * G + h) * D +
+                                4 * c) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  }
+  cluster_sync_all();  // no CTA leaves while another may still read its sums
 }
 
 // Splits of a token merged: grid (Hq, T).  A warp takes every eighth split, a lane
@@ -572,13 +663,42 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
 
 template <int D>
 cudaError_t launch(Kv4AttnArgs a, cudaStream_t s) {
-  a.one_k = 0x64006400u;
-  cudaError_t e = cudaFuncSetAttribute(k_attn_kv4<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       Shape<D>::SMEM);
+  // Once per device: more shared memory than a kernel has by default.
+  static std::atomic<unsigned long long> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(k_attn_kv4<D>, dim3(a.nsplit, a.kv.n_kv_heads, a.T), dim3(kWarps * 32),
-                 Shape<D>::SMEM, s, a);
-  if (e != cudaSuccess || a.nsplit == 1) return e;
+  if (!((ready.load() >> (dev & 63)) & 1)) {
+    e = cudaFuncSetAttribute(k_attn_kv4<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Shape<D>::SMEM);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  a.one_k = 0x64006400u;
+  a.cluster = a.nsplit > 1 && a.nsplit <= kMaxCluster;
+  const dim3 grid(a.nsplit, a.kv.n_kv_heads, a.T);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = Shape<D>::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
+  if ((unsigned long long)grid.x * grid.y * grid.z <= kPdlMaxCtas) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+  }
+  if (a.cluster) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = a.nsplit;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  count_launch();
+  e = cudaLaunchKernelEx(&cfg, k_attn_kv4<D>, a);
+  if (e != cudaSuccess || a.nsplit == 1 || a.cluster) return e;
   return launch_pdl(k_kv4_combine<D>, dim3(a.n_q_heads, a.T), dim3(kCombineWarps * 32), 0, s, a);
 }
 
@@ -600,7 +720,7 @@ int kv4_pick_splits(int T, int n_kv_heads, long long keys, int longest) {
 }
 
 size_t kv4_part_floats(int T, int n_q_heads, int head_dim, int nsplit) {
-  return nsplit > 1 ? (size_t)T * n_q_heads * nsplit * (head_dim + 2) : 0;
+  return nsplit > kMaxCluster ? (size_t)T * n_q_heads * nsplit * (head_dim + 2) : 0;
 }
 
 cudaError_t launch_attention_kv4(const Kv4AttnArgs &a, cudaStream_t s) {

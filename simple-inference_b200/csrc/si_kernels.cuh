@@ -270,8 +270,9 @@ struct Kv4AttnArgs {
   const float *q;      // rows [.][Hq][D]
   float *out;          // rows [.][Hq][D]
   int nsplit;          // kv4_pick_splits()
-  uint32_t one_k;      // set by the launch
-  float *part;         // kv4_part_floats() of device memory when nsplit > 1
+  uint32_t one_k;      // set by the launch, as the next
+  int cluster;         // the splits of a token are one cluster and merge in it
+  float *part;         // kv4_part_floats() of device memory
   int *err;
 };
 // Splits of the key axis for T tokens that attend `keys` keys in all, `longest`
