@@ -43,6 +43,7 @@
 // matrix instructions.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "si_common.cuh"
 #include "si_kernels.cuh"
@@ -191,10 +192,12 @@ __device__ __forceinline__ Token token_of(const Kv4AttnArgs &a, int t) {
   if (k.seq < 0 || k.seq >= a.kv.n_seqs) k.len = 0;
   return k;
 }
-// Keys per split of a token of `len` keys, and the splits it needs.
-__device__ __forceinline__ int split_keys(int len, int nsplit) {
+// Keys per split of a token of `len` keys: an even share, so that a token's
+// splits, which are one cluster, end together.
+__host__ __device__ __forceinline__ int split_keys(int len, int nsplit) {
   const int per = (len + nsplit - 1) / nsplit;
-  return max(kMinSplit, (per + kTile - 1) / kTile * kTile);
+  const int up = (per + kTile - 1) / kTile * kTile;
+  return up > kMinSplit ? up : kMinSplit;
 }
 // Two fp32 operations per instruction, each rounded on its own.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -704,23 +707,54 @@ cudaError_t launch(Kv4AttnArgs a, cudaStream_t s) {
 
 }  // namespace
 
-int kv4_pick_splits(int T, int n_kv_heads, long long keys, int longest) {
-  // One wave of CTAs over the whole call (a split of the longest token per
-  // slot that the others leave), a split no shorter than one tile per warp.
-  const long long slots = 148 * kCtasPerSm;
-  long long per = (keys * n_kv_heads + slots - 1) / slots;
-  per = std::max<long long>(kMinSplit, (per + kTile - 1) / kTile * kTile);
-  if (T * n_kv_heads < slots && longest > per) {
-    const long long fit = slots / ((long long)T * n_kv_heads);  // equal lengths: whole splits
-    const long long even = (longest + fit - 1) / fit;
-    if (keys >= (long long)T * longest - T) per = std::max(per, (even + kTile - 1) / kTile * kTile);
+// The number of splits that takes the least time by this count, in keys of one
+// slot: with all CTAs at once, the longest split; else what the slots have to do on
+// average plus half a split at the end, or whole waves where lengths are equal.  A
+// CTA costs some 300 keys by itself, the merge kernel for more than kMaxCluster
+// splits 600.  (7B, 64 of 0 to 8191 keys: 130, 82, 81, 78, 84, 82, 93 us for 1 to 6
+// and 8 splits; 72B, 8 x 4096: 51, 38, 30, 24, 22, 20, 28 us.)
+constexpr int kSlots = 148 * kCtasPerSm;  // CTAs that run at once
+constexpr int kCtaKeys = 300, kMergeKeys = 600;
+
+void kv4_pick_splits(Kv4AttnArgs &a) {
+  const int Hkv = a.kv.n_kv_heads;
+  if (a.tok_ctx) {
+    // Lengths up to the cache's are possible: enough splits for one wave.
+    const int most = a.kv.max_pages * a.kv.page_len;
+    a.nsplit = std::max(1, std::min(kSlots / (a.T * Hkv), (most + kMinSplit - 1) / kMinSplit));
+    return;
   }
-  const long long ns = (longest + per - 1) / per;
-  return ns < 1 ? 1 : (int)ns;
+  double keys = 0;
+  int longest = 1;
+  for (int i = 0; i < a.runs.n; ++i) {
+    const int c = a.runs.row0[i + 1] - a.runs.row0[i], len = a.runs.pos[i] + c;
+    keys += (double)c * len;
+    longest = std::max(longest, len);
+  }
+  const double even = keys * Hkv / kSlots;
+  const int most = (longest + kMinSplit - 1) / kMinSplit;
+  const int wave = kSlots / std::max(1, std::min(kSlots, a.T * Hkv));
+  double best = 0;
+  auto consider = [&](int ns) {
+    double n = 0;
+    for (int i = 0; i < a.runs.n; ++i) {
+      const int c = a.runs.row0[i + 1] - a.runs.row0[i], len = a.runs.pos[i] + c;
+      n += (double)c * std::max(1, std::min(ns, (len + kMinSplit - 1) / kMinSplit));
+    }
+    const double waves = n * Hkv / kSlots, piece = split_keys(longest, ns);
+    double cost = waves <= 1 ? piece : std::min(std::ceil(waves) * piece, even + piece / 2);
+    cost += kCtaKeys * std::max(1.0, waves) + (ns > kMaxCluster ? kMergeKeys : 0);
+    if (best == 0 || cost < 0.97 * best) {
+      best = cost;
+      a.nsplit = ns;
+    }
+  };
+  for (int ns = 1; ns <= std::min(most, kMaxCluster); ++ns) consider(ns);
+  if (most > kMaxCluster && wave > kMaxCluster) consider(std::min(most, wave));
 }
 
-size_t kv4_part_floats(int T, int n_q_heads, int head_dim, int nsplit) {
-  return nsplit > kMaxCluster ? (size_t)T * n_q_heads * nsplit * (head_dim + 2) : 0;
+size_t kv4_part_floats(const Kv4AttnArgs &a) {
+  return a.nsplit > kMaxCluster ? (size_t)a.T * a.n_q_heads * a.nsplit * (a.kv.head_dim + 2) : 0;
 }
 
 cudaError_t launch_attention_kv4(const Kv4AttnArgs &a, cudaStream_t s) {

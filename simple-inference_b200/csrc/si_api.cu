@@ -1498,8 +1498,8 @@ static si_status kv4_attend(si_ctx *ctx, si_kv4 *kv, int n_q_heads, const float 
   if (tok_ctx) {
     a.tok_ctx = tok_ctx;
     a.T = T;
-    a.nsplit = si::kv4_pick_splits(T, kv->d.n_kv_heads, (long long)T * kv->max_ctx, kv->max_ctx);
-    SI_TRY(ctx->kv4.reserve(si::kv4_part_floats(T, n_q_heads, D, a.nsplit) * sizeof(float)));
+    si::kv4_pick_splits(a);
+    SI_TRY(ctx->kv4.reserve(si::kv4_part_floats(a) * sizeof(float)));
     a.part = static_cast<float *>(ctx->kv4.p);
     SI_CUDA(si::launch_attention_kv4(a, ctx->stream));
     return SI_OK;
@@ -1518,16 +1518,8 @@ static si_status kv4_attend(si_ctx *ctx, si_kv4 *kv, int n_q_heads, const float 
       [&](const si::Kv4Runs &p, int tokens) -> si_status {
         a.runs = p;
         a.T = tokens;
-        long long keys = 0;
-        int longest = 0;
-        for (int i = 0; i < p.n; ++i) {
-          const int c = p.row0[i + 1] - p.row0[i];
-          keys += (long long)c * (p.pos[i] + 1) + (long long)c * (c - 1) / 2;
-          longest = std::max(longest, p.pos[i] + c);
-        }
-        a.nsplit = si::kv4_pick_splits(tokens, kv->d.n_kv_heads, keys, longest);
-        SI_TRY(ctx->kv4.reserve(si::kv4_part_floats(tokens, n_q_heads, D, a.nsplit) *
-                                sizeof(float)));
+        si::kv4_pick_splits(a);
+        SI_TRY(ctx->kv4.reserve(si::kv4_part_floats(a) * sizeof(float)));
         a.part = static_cast<float *>(ctx->kv4.p);
         SI_CUDA(si::launch_attention_kv4(a, ctx->stream));
         return SI_OK;

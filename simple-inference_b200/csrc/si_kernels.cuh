@@ -275,10 +275,9 @@ struct Kv4AttnArgs {
   float *part;         // kv4_part_floats() of device memory
   int *err;
 };
-// Splits of the key axis for T tokens that attend `keys` keys in all, `longest`
-// of them the most.
-int kv4_pick_splits(int T, int n_kv_heads, long long keys, int longest);
-size_t kv4_part_floats(int T, int n_q_heads, int head_dim, int nsplit);
+// Sets the splits of the key axis of a call (its tokens and lengths given).
+void kv4_pick_splits(Kv4AttnArgs &a);
+size_t kv4_part_floats(const Kv4AttnArgs &a);
 cudaError_t launch_attention_kv4(const Kv4AttnArgs &a, cudaStream_t s);
 // A run of T consecutive tokens of sequence seq from position prefix on, on the
 // tensor cores (attention_kv4_tc.cu).
