@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
   // Group addresses of this warp's tiles, 16 tiles at a time: lane j holds the
   // pool index of group j & 1 of tile j / 2 of the batch, -1 past the keys or
   // where the table has no page (which is recorded).
-  const int gpp = a.kv.page_len / kKv4Group;
+  const int gpp = a.kv.gpp;
   const int *table = a.kv.tables + (size_t)tk.seq * a.kv.max_pages;
   uint8_t *ring = smem + warp * (kStages * S::TILE);
   int gidx = -1;
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
       const int key = k0 + (warp + kWarps * (n + (lane >> 1))) * kTile + (lane & 1) * kKv4Group;
       gidx = -1;
       if (key < k1) {
-        const int gi = key / kKv4Group, pi = gi / gpp;
+        const int gi = key / kKv4Group, pi = a.kv.page_of(gi);
         const int page = table[pi];
         if (page >= 0 && page < a.kv.n_pages)
           gidx = (page * a.kv.n_kv_heads + kvh) * gpp + (gi - pi * gpp);

@@ -604,13 +604,13 @@ __global__ void __launch_bounds__(256) k_kv4_absmax(const __grid_constant__ Kv4V
   pdl_trigger();
   pdl_wait();
   constexpr int NB = D / 32, GB = kv4_group_bytes(D);
-  const int head = blockIdx.y, gpp = kv.page_len / kKv4Group;
+  const int head = blockIdx.y, gpp = kv.gpp;
   const int *table = kv.tables + (size_t)seq * kv.max_pages;
   uint32_t mk = 0, mv = 0;
   const int pos = blockIdx.x * 256 + threadIdx.x;
-  const int gi = pos / kKv4Group, page = pos < L ? table[gi / gpp] : -1;
+  const int gi = pos / kKv4Group, pi = kv.page_of(gi), page = pos < L ? table[pi] : -1;
   if (page >= 0 && page < kv.n_pages) {
-    const uint8_t *g = kv.pool + (((size_t)page * kv.n_kv_heads + head) * gpp + gi % gpp) * GB +
+    const uint8_t *g = kv.pool + (((size_t)page * kv.n_kv_heads + head) * gpp + gi - pi * gpp) * GB +
                        kKv4Group * (D / 2) + (pos % kKv4Group) * (2 * NB);
     // (infinite and NaN scales, 0x7c00 and above, do not count)
 #pragma unroll
@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
     return;
   }
   const int head = blockIdx.x / (a.Lp / BK), p0 = blockIdx.x % (a.Lp / BK) * BK;
-  const int gpp = a.kv.page_len / kKv4Group;
+  const int gpp = a.kv.gpp;
   const int *table = a.kv.tables + (size_t)a.seq * a.kv.max_pages;
   const float ck = ldexpf(1.0f, operand_shift(a.bits[2 * head]));
   const float cv = ldexpf(1.0f, operand_shift(a.bits[2 * head + 1]));
@@ -696,10 +696,10 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
     uint32_t wk = 0x8888u, wv = 0x8888u;
     float sk = 0.0f, sv = 0.0f;
     if (pos < a.L) {
-      const int gi = pos / kKv4Group, page = table[gi / gpp], r = pos % kKv4Group;
+      const int gi = pos / kKv4Group, pi = a.kv.page_of(gi), page = table[pi], r = pos % kKv4Group;
       if (page >= 0 && page < a.kv.n_pages) {
         const uint8_t *g =
-            a.kv.pool + (((size_t)page * a.kv.n_kv_heads + head) * gpp + gi % gpp) * GB;
+            a.kv.pool + (((size_t)page * a.kv.n_kv_heads + head) * gpp + gi - pi * gpp) * GB;
         const uint16_t *c = reinterpret_cast<const uint16_t *>(g + r * (D / 2)) + hw;
         const uint16_t *s = reinterpret_cast<const uint16_t *>(g + kKv4Group * (D / 2)) + r * NB + b;
         wk = c[0];

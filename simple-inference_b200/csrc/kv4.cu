@@ -23,18 +23,19 @@
 namespace si {
 namespace {
 
-// The row (16-position group, row in it) of position pos of sequence seq, or
-// null where the table has no page there.
-__device__ __forceinline__ uint8_t *kv4_group(const Kv4View &kv, int seq, int pos, int head,
-                                              int *page_out) {
-  if (seq < 0 || seq >= kv.n_seqs || pos < 0 || pos / kv.page_len >= kv.max_pages) return nullptr;
-  const int page = kv.tables[(size_t)seq * kv.max_pages + pos / kv.page_len];
+// The group of position pos of sequence seq for KV head 0, or null where the
+// table has no page there.
+__device__ __forceinline__ uint8_t *kv4_group(const Kv4View &kv, int seq, int pos, int *page_out) {
+  if (seq < 0 || seq >= kv.n_seqs || pos < 0 || pos >= kKv4MaxCtx) return nullptr;
+  const int group = pos >> 4, i = kv.page_of(group);
+  if (i >= kv.max_pages) return nullptr;
+  const int page = kv.tables[(size_t)seq * kv.max_pages + i];
   if (page < 0 || page >= kv.n_pages) return nullptr;
-  if (page_out) *page_out = page;
-  const int gpp = kv.page_len / kKv4Group;
-  const size_t g = ((size_t)page * kv.n_kv_heads + head) * gpp + pos % kv.page_len / kKv4Group;
+  *page_out = page;
+  const size_t g = (size_t)page * kv.n_kv_heads * kv.gpp + (group - i * kv.gpp);
   return kv.pool + g * kv4_group_bytes(kv.head_dim);
 }
+static_assert(kKv4Group == 16, "positions are split by shifts");
 
 __device__ __forceinline__ int kv4_run_of(const Kv4Runs &r, int t) {
   int lo = 0, hi = r.n;  // the last run with row0 <= t
@@ -96,7 +97,7 @@ __device__ __forceinline__ void kv4_store_row(const float4 x, uint8_t *codes, ui
 // recorded as SI_ERR_INVALID.
 constexpr int kUnits = 16;
 
-template <int D>
+template <int D, bool VEC>
 __global__ void __launch_bounds__(128) k_kv4_append(const __grid_constant__ Kv4AppendArgs a) {
   pdl_trigger();
   pdl_wait();
@@ -115,21 +116,22 @@ __global__ void __launch_bounds__(128) k_kv4_append(const __grid_constant__ Kv4A
     pos = a.runs.pos[r] + row - a.runs.row0[r];
   }
   const int u0 = blockIdx.y * kUnits + (threadIdx.x >> 5) * (N * RPW) + lane / LPR;
+  const float *qr = nq ? a.q + (size_t)row * a.ldq + 4 * j : nullptr;
+  const float *kr = a.k + (size_t)row * a.ldkv + 4 * j, *vr = a.v + (size_t)row * a.ldkv + 4 * j;
   float4 x[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const int u = u0 + k * RPW;
     x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (u < units) {
-      const int head = u < nq ? u : (u - nq) % Hkv;
-      const float *src = u < nq ? a.q + (size_t)row * a.ldq + (size_t)u * D
-                                : (u >= nq + Hkv ? a.v : a.k) + (size_t)row * a.ldkv + (size_t)head * D;
-      x[k] = a.vec ? *reinterpret_cast<const float4 *>(src + 4 * j)
-                   : make_float4(src[4 * j], src[4 * j + 1], src[4 * j + 2], src[4 * j + 3]);
+      const float *src = u < nq ? qr + u * D : u < nq + Hkv ? kr + (u - nq) * D
+                                                            : vr + (u - nq - Hkv) * D;
+      if constexpr (VEC) x[k] = *reinterpret_cast<const float4 *>(src);
+      else x[k] = make_float4(src[0], src[1], src[2], src[3]);
     }
   }
   int page = 0;
-  uint8_t *grp = kv4_group(a.kv, seq, pos, 0, &page);
+  uint8_t *grp = kv4_group(a.kv, seq, pos, &page);
   if (grp && a.kv.refs[page] != 1) grp = nullptr;
   if (!grp && threadIdx.x == 0 && blockIdx.y == 0) raise_error(a.err, 1);
   float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -139,8 +141,8 @@ __global__ void __launch_bounds__(128) k_kv4_append(const __grid_constant__ Kv4A
     c = *reinterpret_cast<const float4 *>(a.cos_tab + (size_t)pos * HALF + i);
     s = *reinterpret_cast<const float4 *>(a.sin_tab + (size_t)pos * HALF + i);
   }
-  const size_t head_bytes = (size_t)(a.kv.page_len / kKv4Group) * kv4_group_bytes(D);
-  const int r16 = pos % kKv4Group;
+  const size_t head_bytes = (size_t)a.kv.gpp * kv4_group_bytes(D);
+  const int r16 = pos & 15;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const int u = u0 + k * RPW;
@@ -164,7 +166,8 @@ __global__ void __launch_bounds__(128) k_kv4_append(const __grid_constant__ Kv4A
       *reinterpret_cast<float4 *>(a.q_out + ((size_t)row * a.n_q_heads + u) * D + 4 * j) = x[k];
     uint8_t *codes = nullptr;
     if (grp && u >= nq && u < units)
-      codes = grp + (u - nq) % Hkv * head_bytes + (is_v ? kv4_group_bytes(D) / 2 : 0);
+      codes = is_v ? grp + (u - nq - Hkv) * head_bytes + kv4_group_bytes(D) / 2
+                   : grp + (u - nq) * head_bytes;
     kv4_store_row<D>(x[k], codes ? codes + r16 * (D / 2) : nullptr,
                      codes ? reinterpret_cast<uint16_t *>(codes + kKv4Group * (D / 2)) + r16 * (D / 32)
                            : nullptr,
@@ -182,10 +185,11 @@ __global__ void __launch_bounds__(128) k_kv4_read(const __grid_constant__ Kv4Rea
   const int lane = threadIdx.x & 31, j = lane % LPR, Hkv = a.kv.n_kv_heads;
   const int row = a.runs.row0[0] + blockIdx.x, r = kv4_run_of(a.runs, row);
   const int pos = a.runs.pos[r] + row - a.runs.row0[r];
-  const uint8_t *grp = kv4_group(a.kv, a.runs.seq[r], pos, 0, nullptr);
+  int page;
+  const uint8_t *grp = kv4_group(a.kv, a.runs.seq[r], pos, &page);
   if (!grp && threadIdx.x == 0 && blockIdx.y == 0) raise_error(a.err, 1);
-  const size_t head_bytes = (size_t)(a.kv.page_len / kKv4Group) * kv4_group_bytes(D);
-  const int r16 = pos % kKv4Group, b = j >> 3, g = j & 7;
+  const size_t head_bytes = (size_t)a.kv.gpp * kv4_group_bytes(D);
+  const int r16 = pos & 15, b = j >> 3, g = j & 7;
   const int u0 = blockIdx.y * kUnits + (threadIdx.x >> 5) * (N * RPW) + lane / LPR;
   uint32_t w[N];
   float sc[N];
@@ -195,7 +199,8 @@ __global__ void __launch_bounds__(128) k_kv4_read(const __grid_constant__ Kv4Rea
     w[k] = 0x8888u;
     sc[k] = 0.0f;
     if (grp && u < 2 * Hkv) {
-      const uint8_t *p = grp + u % Hkv * head_bytes + (u >= Hkv ? kv4_group_bytes(D) / 2 : 0);
+      const uint8_t *p =
+          u < Hkv ? grp + u * head_bytes : grp + (u - Hkv) * head_bytes + kv4_group_bytes(D) / 2;
       w[k] = reinterpret_cast<const uint16_t *>(p + r16 * (D / 2))[g * NB + b];
       sc[k] = f16_to_f32(reinterpret_cast<const uint16_t *>(p + kKv4Group * (D / 2))[r16 * NB + b]);
     }
@@ -204,9 +209,9 @@ __global__ void __launch_bounds__(128) k_kv4_read(const __grid_constant__ Kv4Rea
   for (int k = 0; k < N; ++k) {
     const int u = u0 + k * RPW;
     if (u >= 2 * Hkv) continue;
-    float *out = u >= Hkv ? a.v : a.k;
+    float *out = u < Hkv ? a.k : a.v;
     if (!out) continue;
-    *reinterpret_cast<float4 *>(out + ((size_t)row * Hkv + u % Hkv) * D + 4 * j) =
+    *reinterpret_cast<float4 *>(out + ((size_t)row * Hkv + (u < Hkv ? u : u - Hkv)) * D + 4 * j) =
         make_float4(sc[k] * (float)((int)(w[k] & 15) - 8), sc[k] * (float)((int)((w[k] >> 4) & 15) - 8),
                     sc[k] * (float)((int)((w[k] >> 8) & 15) - 8), sc[k] * (float)((int)(w[k] >> 12) - 8));
   }
@@ -267,11 +272,11 @@ cudaError_t launch_kv4_append(const Kv4AppendArgs &a, cudaStream_t s) {
   if (a.T <= 0) return cudaSuccess;
   const int units = (a.q_out ? a.n_q_heads : 0) + 2 * a.kv.n_kv_heads;
   const dim3 grid(a.T, (units + kUnits - 1) / kUnits);
-  Kv4AppendArgs b = a;
-  b.vec = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
+  const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
             reinterpret_cast<uintptr_t>(a.v) | 4 * a.ldq | 4 * a.ldkv) & 15) == 0;
-  return a.kv.head_dim == 128 ? launch_pdl(k_kv4_append<128>, grid, dim3(128), 0, s, b)
-                              : launch_pdl(k_kv4_append<64>, grid, dim3(128), 0, s, b);
+  auto *kern = a.kv.head_dim == 128 ? (vec ? k_kv4_append<128, true> : k_kv4_append<128, false>)
+                                    : (vec ? k_kv4_append<64, true> : k_kv4_append<64, false>);
+  return launch_pdl(kern, grid, dim3(128), 0, s, a);
 }
 
 cudaError_t launch_kv4_read(const Kv4ReadArgs &a, cudaStream_t s) {

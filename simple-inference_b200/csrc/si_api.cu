@@ -247,6 +247,8 @@ struct si_kv4 {
     v.head_dim = d.head_dim;
     v.n_seqs = pages->n_seqs();
     v.max_pages = pages->max_pages();
+    v.gpp = page_len / si::kKv4Group;
+    v.gpp_recip = v.gpp == 1 ? 0u : (uint32_t)(((1ull << 32) + v.gpp - 1) / v.gpp);
     return v;
   }
 };
@@ -1120,7 +1122,7 @@ extern "C" SI_API si_status si_kv4_create(si_ctx *ctx, const si_dims *d, int n_s
     *out = nullptr;
     SI_CHECK(page_len >= si::kKv4Group && page_len <= 4096 && page_len % si::kKv4Group == 0,
              "page_len must be a multiple of %d up to 4096", si::kKv4Group);
-    SI_CHECK(max_ctx <= (1 << 30), "max_ctx out of range");
+    SI_CHECK(max_ctx <= si::kKv4MaxCtx - 4096, "max_ctx out of range");
     const int64_t max_pages = ((int64_t)max_ctx + page_len - 1) / page_len;
     SI_CHECK(max_pages * n_seqs < (1ll << 30), "too many table entries");
     SI_CHECK((int64_t)n_pages * d->n_kv_heads * (page_len / si::kKv4Group) < (1ll << 31),

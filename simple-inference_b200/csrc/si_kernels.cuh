@@ -214,7 +214,15 @@ struct Kv4View {
   const int *tables;  // [n_seqs][max_pages] page of each stretch of page_len positions, or -1
   const int *refs;    // [n_pages] table entries that hold the page
   int n_pages, page_len, n_kv_heads, head_dim, n_seqs, max_pages;
+  int gpp;              // groups per page, at most 256
+  uint32_t gpp_recip;   // ceil(2^32 / gpp), 0 for gpp 1
+  // The page of a group of 16 positions: the quotient by gpp, exact for group
+  // numbers below 2^24 (kKv4MaxCtx positions) since gpp_recip * gpp - 2^32 < 256.
+  __device__ __forceinline__ int page_of(int group) const {
+    return gpp == 1 ? group : (int)__umulhi((uint32_t)group, gpp_recip);
+  }
 };
+constexpr int kKv4MaxCtx = 1 << 27;
 // Ragged tokens by value: run i is rows [row0[i], row0[i + 1]) of the call's
 // row-wise tensors, at positions pos[i], pos[i] + 1, ... of sequence seq[i].
 constexpr int kKv4MaxRuns = 256;
@@ -236,7 +244,6 @@ struct Kv4AppendArgs {
   const float *cos_tab, *sin_tab;  // rotate K (and q) by position, or null
   int max_positions;
   int *err;
-  int vec;               // set by the launch: 16-byte loads
 };
 cudaError_t launch_kv4_append(const Kv4AppendArgs &a, cudaStream_t s);
 struct Kv4ReadArgs {
