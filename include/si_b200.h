@@ -522,12 +522,14 @@ SI_API si_status si_kv4_read_dev(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs
 /* Attention of queries q [T][Hq][D] (RoPE applied; 16-byte aligned, as out)
  * over the cache: the token at position p attends positions 0 .. p of its
  * sequence, whose pages must cover it.  A run at pos -1 begins with a token
- * that attends nothing; its row of out is zeros (padding of a batch).  Runs of
- * 16 tokens and more go through the prefill kernels over their keys unpacked
- * once (the kernel follows si_ctx_set_exact_attention), shorter ones read the
- * packed cache directly.  fp32 in and out; no product's input is rounded to
- * fewer than 22 bits.  Sums follow the split of the work, so a token's result
- * may differ in its last bits between calls with other runs. */
+ * that attends nothing; its row of out is zeros (padding of a batch).  Runs with
+ * enough work go through a prompt kernel on the tensor cores (with
+ * si_ctx_set_exact_attention the fp32 one over their keys unpacked), the others
+ * read the packed cache token by token.  fp32 in and out, within about 1e-6 of
+ * the 64-bit result.  Sums follow the split of the work, so a token's result may
+ * differ in its last bits between calls with other runs.  A position whose V
+ * holds infinities or NaN makes whole rows NaN that attend it in the prompt
+ * kernel, the affected dims in the other. */
 SI_API si_status si_attention_kv4_dev(si_ctx *ctx, si_kv4 *kv, const si_dims *dims,
                                       const float *q_dev, const si_kv4_run *runs, int n,
                                       float *out_dev);

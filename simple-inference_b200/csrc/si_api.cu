@@ -1103,9 +1103,18 @@ static const si::Kv4Run *as_runs(const si_kv4_run *r) {
   return reinterpret_cast<const si::Kv4Run *>(r);
 }
 
-// Attention of a run of at least this many tokens goes through the prefill
-// kernels over the run's keys unpacked once.
-constexpr int kKv4PrefillMin = 16;
+// Whether a run's attention goes through the prompt kernel.  That costs about 30 us
+// a run before it starts (its operands are made first, over all keys) and then a
+// fifth of what the decode kernel takes per token and key; measured at 16 to 256
+// tokens on 500 to 8000 positions, the two meet near (tokens - 8) * keys * KV heads =
+// 500,000 at head_dim 128 (7B, 2000 positions: 64 tokens 35 against 38 us, 128 56
+// against 40 us; 72B, 8000: 16 tokens 52 against 56 us, 32 101 against 64 us), a
+// half more at 64, whose decode tiles take two thirds of the time.
+static bool kv4_prompt_run(const si_kv4 *kv, const si_kv4_run &r) {
+  if (r.pos < 0 || r.count < 16) return false;
+  const double keys = r.pos + 0.5 * r.count;
+  return (r.count - 8) * keys * kv->d.n_kv_heads * (kv->d.head_dim + 64) / 192 >= 5e5;
+}
 
 extern "C" SI_API size_t si_kv4_page_bytes(const si_dims *d, int page_len) {
   if (check_dims(d) != SI_OK || page_len <= 0 || page_len % si::kKv4Group) return 0;
@@ -1507,11 +1516,11 @@ static si_status kv4_attend(si_ctx *ctx, si_kv4 *kv, int n_q_heads, const float 
     return SI_OK;
   }
   const std::vector<int> rows = kv4_rows(runs, n);
-  // Few tokens a run: one token at a time over the packed cache.
+  // Decode tokens, short and early prompts: one token at a time.
   std::vector<si_kv4_run> few;
   std::vector<int> few_rows;
   for (int i = 0; i < n; ++i)
-    if (runs[i].count > 0 && (runs[i].count < kKv4PrefillMin || runs[i].pos < 0)) {
+    if (runs[i].count > 0 && !kv4_prompt_run(kv, runs[i])) {
       few.push_back(runs[i]);
       few_rows.push_back(rows[i]);
     }
@@ -1527,7 +1536,7 @@ static si_status kv4_attend(si_ctx *ctx, si_kv4 *kv, int n_q_heads, const float 
         return SI_OK;
       }));
   for (int i = 0; i < n; ++i) {
-    if (runs[i].count < kKv4PrefillMin || runs[i].pos < 0) continue;
+    if (!kv4_prompt_run(kv, runs[i])) continue;
     if (!ctx->exact_attention) {
       si::Kv4PromptArgs pa{};
       pa.kv = a.kv;

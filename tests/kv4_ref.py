@@ -20,7 +20,8 @@ def quantise(x):
 def values(codes, scales):
     """What codes stand for, in 64 bits."""
     c = codes.reshape(*codes.shape[:-1], -1, 32).astype(np.float64) - 8
-    return (c * scales.astype(np.float64)[..., None]).reshape(codes.shape)
+    with np.errstate(invalid="ignore"):
+        return (c * scales.astype(np.float64)[..., None]).reshape(codes.shape)
 
 
 def group_bytes(D):
