@@ -91,7 +91,7 @@ struct Params {
   float *out;   // rows [T][Hq][D]
   float *part;  // with splits: (m, l) [T][Hq][nsplit], then O [T][Hq][nsplit][D]
   int *err;
-  const float *rowf;  // [T][Hq]: takes a row's scores to log2 units
+  const float *rowf;  // [T][Hq]: with K's power of two takes a row's scores to log2 units
   const int *bits;    // [Hkv][2]: largest |scale| of K and V as fp16 bits
 };
 
@@ -356,7 +356,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int tok = t0 + tl;
     const bool valid = r < rows && tok < p.T;
     const int pos = valid ? p.prefix + tok : -1;  // a padding row attends nothing
-    const float rf = valid ? p.rowf[(size_t)tok * p.Hq + (size_t)g * p.G + hh] : 0.0f;
+    const int kshift = operand_shift(p.bits[2 * g]), vshift = operand_shift(p.bits[2 * g + 1]);
+    // (kept above zero: a masked score times it stays -inf)
+    const float rf =
+        valid ? fmaxf(ldexpf(p.rowf[(size_t)tok * p.Hq + (size_t)g * p.G + hh], -kshift), 1.2e-38f)
+              : 0.0f;
     const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16);
     constexpr int H = D / 2;   // this group keeps dims [grp * H, grp * H + H) of the sums
     const uint32_t t_o = t_row + S::COL_O + grp * H, t_ol = t_row + S::COL_OL + grp * H;
@@ -540,7 +544,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (ok) {
       tc_fence_after();
       l = l_s[r] + l_s[ROWS + r];
-      const float back = ldexpf(1.0f, -operand_shift(p.bits[2 * g + 1]));
+      const float back = ldexpf(1.0f, -vshift);
       const size_t head = (size_t)g * p.G + hh;
       float *orow = p.out + ((size_t)tok * p.Hq + head) * D;
       float f = back;
@@ -596,11 +600,11 @@ __global__ void __launch_bounds__(D) k_kv4_tc_combine(const Params p) {
 }
 
 // ---- operands from the cache (layout in kv4.cu) ----------------------------
-// Largest |scale| of K and of V over positions [0, L) of one KV head, as fp16
-// bits: grid (pieces of 256 positions, Hkv); bits [Hkv][2] start at 0.
+// Largest |scale| of K and of V of each piece of 256 positions below L of each KV
+// head, as fp16 bits: grid (pieces, Hkv), part [Hkv][pieces].
 template <int D>
 __global__ void __launch_bounds__(256) k_kv4_absmax(const __grid_constant__ Kv4View kv, int seq,
-                                                    int L, int *__restrict__ bits) {
+                                                    int L, uint2 *__restrict__ part) {
   pdl_trigger();
   pdl_wait();
   constexpr int NB = D / 32, GB = kv4_group_bytes(D);
@@ -623,9 +627,15 @@ __global__ void __launch_bounds__(256) k_kv4_absmax(const __grid_constant__ Kv4V
   }
   mk = __reduce_max_sync(0xffffffffu, max(mk & 0xffffu, mk >> 16));
   mv = __reduce_max_sync(0xffffffffu, max(mv & 0xffffu, mv >> 16));
-  if ((threadIdx.x & 31) == 0) {
-    atomicMax(bits + 2 * head, (int)mk);
-    atomicMax(bits + 2 * head + 1, (int)mv);
+  __shared__ uint2 w_s[8];
+  if ((threadIdx.x & 31) == 0) w_s[threadIdx.x >> 5] = make_uint2(mk, mv);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) {
+      mk = max(mk, w_s[i].x);
+      mv = max(mv, w_s[i].y);
+    }
+    part[(size_t)head * gridDim.x + blockIdx.x] = make_uint2(mk, mv);
   }
 }
 
@@ -633,18 +643,19 @@ __global__ void __launch_bounds__(256) k_kv4_absmax(const __grid_constant__ Kv4V
 // take (64 positions, KV head) of the cache, the others eight query rows each.
 //
 // Q: q * scale, times the power of two that puts the row's largest value just
-// below 2^14, split; rowf undoes it and the K operand's.  One warp per (token,
-// head) row.
+// below 2^14, split; rowf undoes it.  One warp per (token, head) row.
 // K as [Hkv][Lp][D] and V transposed as [Hkv][D][Lp], hi and lo halves, zero
-// past L: a thread per half-word of four codes; V goes through shared memory for
+// past L: every CTA first finds its head's largest scales among the pieces' (a
+// head's first one writes them down for the attention); a thread per half-word of four codes; V goes through shared memory for
 // the transpose, its 16-byte pieces XORed by the position's octet so that the
 // reads along positions meet different banks.
 struct SplitArgs {
   Kv4View kv;
-  int seq, L, Lp, q_rows, Hq, G;
+  int seq, L, Lp, pieces, q_rows;
   float scale;
   const float *q;
-  const int *bits;
+  const uint2 *part;  // [Hkv][pieces] largest |scale| of K and V, as fp16 bits
+  int *bits;          // [Hkv][2]
   __half *qh, *ql, *kh, *kl, *vh, *vl;
   float *rowf;
   int *err;
@@ -679,17 +690,30 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
       reinterpret_cast<uint32_t *>(a.qh)[at] = pack_h2(hu, hv);
       reinterpret_cast<uint32_t *>(a.ql)[at] = pack_h2(u - hu, v - hv);
     }
-    // (kept above zero: a masked score times it stays -inf)
-    if (lane == 0)
-      a.rowf[row] =
-          fmaxf(ldexpf(1.0f, -e - operand_shift(a.bits[2 * (row % a.Hq / a.G)])), 1.2e-38f);
+    if (lane == 0) a.rowf[row] = ldexpf(1.0f, -e);
     return;
   }
   const int head = blockIdx.x / (a.Lp / BK), p0 = blockIdx.x % (a.Lp / BK) * BK;
   const int gpp = a.kv.gpp;
   const int *table = a.kv.tables + (size_t)a.seq * a.kv.max_pages;
-  const float ck = ldexpf(1.0f, operand_shift(a.bits[2 * head]));
-  const float cv = ldexpf(1.0f, operand_shift(a.bits[2 * head + 1]));
+  __shared__ uint2 w_s[8];
+  uint2 mx = make_uint2(0, 0);
+  for (int i = threadIdx.x; i < a.pieces; i += blockDim.x) {
+    const uint2 x = a.part[(size_t)head * a.pieces + i];
+    mx = make_uint2(max(mx.x, x.x), max(mx.y, x.y));
+  }
+  mx.x = __reduce_max_sync(0xffffffffu, mx.x);
+  mx.y = __reduce_max_sync(0xffffffffu, mx.y);
+  if ((threadIdx.x & 31) == 0) w_s[threadIdx.x >> 5] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) mx = make_uint2(max(mx.x, w_s[i].x), max(mx.y, w_s[i].y));
+  if (p0 == 0 && threadIdx.x == 0) {
+    a.bits[2 * head] = (int)mx.x;
+    a.bits[2 * head + 1] = (int)mx.y;
+  }
+  const float ck = ldexpf(1.0f, operand_shift((int)mx.x));
+  const float cv = ldexpf(1.0f, operand_shift((int)mx.y));
   for (int e = threadIdx.x; e < BK * (D / 4); e += blockDim.x) {
     const int pp = e / (D / 4), hw = e % (D / 4), pos = p0 + pp;
     const int b = hw % NB, d = 32 * b + 4 * (hw / NB);
@@ -751,7 +775,7 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
 
 // Where the pieces of the scratch lie.
 struct Scratch {
-  size_t qh, ql, kh, kl, vh, vl, bits, rowf, part, bytes;
+  size_t qh, ql, kh, kl, vh, vl, bits, pieces, rowf, part, bytes;
   int nsplit;
 };
 static Scratch carve(const Kv4PromptArgs &a) {
@@ -767,7 +791,8 @@ static Scratch carve(const Kv4PromptArgs &a) {
   s.vh = s.kl + kv;
   s.vl = s.vh + kv;
   s.bits = s.vl + kv;
-  s.rowf = s.bits + up(2 * Hkv * sizeof(int));
+  s.pieces = s.bits + up(2 * Hkv * sizeof(int));
+  s.rowf = s.pieces + up(Hkv * ((L + 255) / 256) * sizeof(uint2));
   s.part = s.rowf + up((size_t)a.T * a.n_q_heads * sizeof(float));
   // Splits of the keys where the row tiles alone leave SMs idle; a split has
   // eight tiles at least.
@@ -792,12 +817,12 @@ cudaError_t launch(const Kv4PromptArgs &a, char *base, const Scratch &sc, cudaSt
   float *rowf = reinterpret_cast<float *>(base + sc.rowf);
   const float scale = 1.4426950408889634f / sqrtf((float)D);
   const int rows = a.T * Hq;
-  cudaError_t e = cudaMemsetAsync(bits, 0, 2 * Hkv * sizeof(int), s);
+  uint2 *part = reinterpret_cast<uint2 *>(base + sc.pieces);
+  const int pieces = (L + 255) / 256;
+  cudaError_t e = launch_pdl(k_kv4_absmax<D>, dim3(pieces, Hkv), dim3(256), 0, s, a.kv, a.seq, L,
+                             part);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(k_kv4_absmax<D>, dim3((L + 255) / 256, Hkv), dim3(256), 0, s, a.kv, a.seq, L,
-                 bits);
-  if (e != cudaSuccess) return e;
-  SplitArgs sa{a.kv, a.seq, L, Lp, rows, Hq, G, scale, a.q, bits, qh, ql, kh, kl, vh, vl, rowf,
+  SplitArgs sa{a.kv, a.seq, L, Lp, pieces, rows, scale, a.q, part, bits, qh, ql, kh, kl, vh, vl, rowf,
                a.err};
   e = launch_pdl(k_split<D>, dim3(Lp / BK * Hkv + (rows + 7) / 8), dim3(256), 0, s, sa);
   if (e != cudaSuccess) return e;
