@@ -217,8 +217,8 @@ __global__ void __launch_bounds__(128) k_kv4_read(const __grid_constant__ Kv4Rea
   }
 }
 
-// Bookkeeping: entries and reference counts from kernel parameters (the host's
-// tables may change again at once), and page copies in the same launch: the
+// Bookkeeping: table entries from kernel parameters (the host's tables may change
+// again at once), the reference counts that follow them, and page copies in the same launch: the
 // last kWriters CTAs write the entries, the others copy kCopyBytes each of a
 // page.  The words are read through a generic pointer: as constants, whose lanes
 // read different addresses, they would come one at a time.
@@ -236,19 +236,23 @@ __global__ void __launch_bounds__(kCopyThreads)
   asm volatile("" : "+l"(word));
   if (blockIdx.x >= gridDim.x - kWriters) {
     const int w0 = blockIdx.x - (gridDim.x - kWriters), t0 = w0 * kCopyThreads + threadIdx.x;
+    auto set = [&](int *entry, int page) {
+      const int old = *entry;
+      *entry = page;
+      if (old >= 0) atomicSub(u.refs + old, 1);
+      if (page >= 0) atomicAdd(u.refs + page, 1);
+    };
     for (int j = t0 >> 5; j < u.n_spans; j += kWriters * kCopyThreads / 32) {
       int *to = u.tables + word[3 * j];
       const int n = word[3 * j + 1], from = word[3 * j + 2];
-      for (int i = threadIdx.x & 31; i < n; i += 32) to[i] = from < 0 ? -1 : u.tables[from + i];
+      for (int i = threadIdx.x & 31; i < n; i += 32)
+        set(to + i, from == -1 ? -1 : from >= 0 ? u.tables[from + i] : word[-2 - from + i]);
     }
     const int *w = word + 3 * u.n_spans;
-    for (int i = t0; i < u.n_table; i += kWriters * kCopyThreads) u.tables[w[2 * i]] = w[2 * i + 1];
-    w += 2 * u.n_table;
-    for (int i = t0; i < u.n_refs; i += kWriters * kCopyThreads) u.refs[w[2 * i]] = w[2 * i + 1];
+    for (int i = t0; i < u.n_table; i += kWriters * kCopyThreads) set(u.tables + w[2 * i], w[2 * i + 1]);
     return;
   }
-  const int *w = word + 3 * u.n_spans + 2 * (u.n_table + u.n_refs) +
-                 2 * (blockIdx.x / pieces);
+  const int *w = word + 3 * u.n_spans + 2 * u.n_table + 2 * (blockIdx.x / pieces);
   const size_t off = (size_t)(blockIdx.x % pieces) * kCopyBytes;
   const uint8_t *src = u.pool + (size_t)w[0] * u.page_bytes + off;
   uint8_t *dst = u.pool + (size_t)w[1] * u.page_bytes + off;
@@ -293,6 +297,9 @@ static cudaError_t update(const Kv4Update<WORDS> &u, cudaStream_t s) {
                     u);
 }
 cudaError_t launch_kv4_update(const Kv4Update<kKv4SmallWords> &u, cudaStream_t s) {
+  return update(u, s);
+}
+cudaError_t launch_kv4_update(const Kv4Update<kKv4MediumWords> &u, cudaStream_t s) {
   return update(u, s);
 }
 cudaError_t launch_kv4_update(const Kv4Update<kKv4LargeWords> &u, cudaStream_t s) {

@@ -1215,42 +1215,54 @@ static si_status kv4_push(si_ctx *ctx, si_kv4 *kv) {
   u.refs = kv->refs;
   u.pool = kv->pool;
   u.page_bytes = kv->page_bytes;
-  size_t s = 0, t = 0, r = 0, c = 0;
+  size_t s = 0, t = 0, c = 0;
+  int done = 0;  // of span s, as far as its pages fit the launches before
   do {
-    int *w = u.word, *const end = u.word + WORDS;
-    u.n_spans = u.n_table = u.n_refs = u.n_copies = 0;
-    for (; s < e.spans.size() && end - w >= 3; ++s, ++u.n_spans) {
-      *w++ = e.spans[s].to;
-      *w++ = e.spans[s].n;
-      *w++ = e.spans[s].from;
+    // Spans from the front, their pages from the back.
+    int *w = u.word, *end = u.word + WORDS;
+    u.n_spans = u.n_table = u.n_copies = 0;
+    while (s < e.spans.size() && end - w >= 4) {
+      const si::Kv4Span &x = e.spans[s];
+      int n = x.n - done, from = x.from < 0 ? -1 : x.from + done;
+      if (x.from >= si::Kv4Span::kLiteral) {
+        n = (int)std::min<ptrdiff_t>(n, end - w - 3);
+        end -= n;
+        std::copy_n(e.literal.data() + (from - si::Kv4Span::kLiteral), n, end);
+        from = -2 - (int)(end - u.word);
+      }
+      *w++ = x.to + done;
+      *w++ = n;
+      *w++ = from;
+      ++u.n_spans;
+      done += n;
+      if (done == x.n) {
+        ++s;
+        done = 0;
+      }
     }
     for (; t < e.table.size() && end - w >= 2; ++t, ++u.n_table) {
       *w++ = e.table[t].first;
       *w++ = e.table[t].second;
-    }
-    for (; r < e.touched.size() && end - w >= 2; ++r, ++u.n_refs) {
-      *w++ = e.touched[r];
-      *w++ = kv->pages->refs(e.touched[r]);
     }
     for (; c < e.copies.size() && end - w >= 2; ++c, ++u.n_copies) {
       *w++ = e.copies[c].first;
       *w++ = e.copies[c].second;
     }
     SI_CUDA(si::launch_kv4_update(u, ctx->stream));
-  } while (s < e.spans.size() || t < e.table.size() || r < e.touched.size() ||
-           c < e.copies.size());
+  } while (s < e.spans.size() || t < e.table.size() || c < e.copies.size());
   return SI_OK;
 }
 
 // Queues a change of the pages on the context's stream.
 static si_status kv4_flush(si_ctx *ctx, si_kv4 *kv) {
   si::Kv4Edits &e = kv->edits;
-  const size_t n = 3 * e.spans.size() + 2 * (e.table.size() + e.touched.size() + e.copies.size());
+  const size_t n = 3 * e.spans.size() + e.literal.size() + 2 * (e.table.size() + e.copies.size());
   si_status st = SI_OK;
   if (n)
-    st = n <= si::kKv4SmallWords ? kv4_push<si::kKv4SmallWords>(ctx, kv)
-                                 : kv4_push<si::kKv4LargeWords>(ctx, kv);
-  kv->pages->done(&e);
+    st = n <= si::kKv4SmallWords    ? kv4_push<si::kKv4SmallWords>(ctx, kv)
+         : n <= si::kKv4MediumWords ? kv4_push<si::kKv4MediumWords>(ctx, kv)
+                                    : kv4_push<si::kKv4LargeWords>(ctx, kv);
+  e.clear();
   return st;
 }
 

@@ -255,19 +255,22 @@ struct Kv4ReadArgs {
 };
 cudaError_t launch_kv4_read(const Kv4ReadArgs &a, cudaStream_t s);
 // word: n_spans triples (to, n, from) of table entries that become the entries
-// from `from` on, or -1; n_table pairs (entry, page), n_refs pairs (page, count),
-// n_copies pairs (from, to), taken when the launch is queued.  The small form
-// keeps a decode step's few words from carrying 28 KB of kernel parameters.
-constexpr int kKv4SmallWords = 960, kKv4LargeWords = 7168;
+// from `from` on, -1 (from -1) or the words word[-2 - from ..] (from below); n_table
+// pairs (entry, page); n_copies pairs (page, page); all taken when the launch is
+// queued.  refs follows: a changed entry's old page loses a count, its new one
+// gains one.  Three sizes, since a launch takes its parameters in whole: 28 KB cost
+// some 5 us more than the small one.
+constexpr int kKv4SmallWords = 960, kKv4MediumWords = 3328, kKv4LargeWords = 7168;
 template <int WORDS>
 struct Kv4Update {
   int *tables, *refs;
   uint8_t *pool;
   size_t page_bytes;
-  int n_spans, n_table, n_refs, n_copies;
+  int n_spans, n_table, n_copies;
   int word[WORDS];
 };
 cudaError_t launch_kv4_update(const Kv4Update<kKv4SmallWords> &u, cudaStream_t s);
+cudaError_t launch_kv4_update(const Kv4Update<kKv4MediumWords> &u, cudaStream_t s);
 cudaError_t launch_kv4_update(const Kv4Update<kKv4LargeWords> &u, cudaStream_t s);
 struct Kv4AttnArgs {
   Kv4View kv;

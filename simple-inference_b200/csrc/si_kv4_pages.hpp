@@ -20,24 +20,26 @@ struct Kv4Run {  // `count` consecutive tokens of sequence seq from position pos
   int seq, pos, count;
 };
 
-// Table entries [to, to + n) become entries [from, from + n), or -1 where from
-// is -1.
+// Table entries [to, to + n) become entries [from, from + n); -1 where from is
+// kNone; or, where from is kLiteral + i, the pages literal[i .. i + n).
 struct Kv4Span {
+  static constexpr int kNone = -1, kLiteral = 1 << 30;  // (tables have fewer entries)
   int to, n, from;
 };
 
-// What a change asks of the device.  Copies never chain: no destination of a
-// change is a source of the same change, and no destination occurs twice; the
-// same holds of the table's entries and spans.
+// What a change asks of the device, where the reference counts follow the table:
+// an entry that changes lets its old page go and holds its new one.  Copies never
+// chain: no destination of a change is a source of the same change, and no
+// destination occurs twice; the same holds of the table's entries and spans.
 struct Kv4Edits {
   std::vector<Kv4Span> spans;
+  std::vector<int> literal;
   std::vector<std::pair<int, int>> table;  // (entry, page)
-  std::vector<int> touched;                // pages whose reference count changed, each once
   std::vector<std::pair<int, int>> copies; // (from page, to page)
   void clear() {
     spans.clear();
+    literal.clear();
     table.clear();
-    touched.clear();
     copies.clear();
   }
 };
@@ -46,7 +48,7 @@ class Kv4Pages {
  public:
   Kv4Pages(int n_seqs, int max_pages, int n_pages, int page_len)
       : n_seqs_(n_seqs), max_pages_(max_pages), page_len_(page_len), n_free_(n_pages),
-        count_(n_seqs, 0), refs_(n_pages, 0), mark_(n_pages, 0),
+        count_(n_seqs, 0), refs_(n_pages, 0),
         table_((size_t)n_seqs * max_pages, -1) {}
 
   int n_pages() const { return (int)refs_.size(); }
@@ -87,12 +89,6 @@ class Kv4Pages {
 
   bool seq_ok(int seq) { return (seq >= 0 && seq < n_seqs_) || no("sequence out of range"); }
 
-  // Called with a change's edits once they are done with.
-  void done(Kv4Edits *e) {
-    for (int pg : e->touched) mark_[pg] = 0;
-    e->clear();
-  }
-
   // Positions [pos, pos + count) of every run get pages that no other
   // sequence holds: missing pages (from the sequence's first missing one) are
   // taken, a shared page is replaced by a copy of it.
@@ -132,13 +128,18 @@ class Kv4Pages {
       for (int p = p0; p < std::min(p1 + 1, count_[x.seq]); ++p) {
         const int old = table_[at(x.seq, p)];
         if (refs_[old] <= 1) continue;
-        const int pg = take(e);
+        const int pg = take();
         e->copies.push_back({old, pg});
-        drop(old, e);
+        drop(old);
         put(x.seq, p, pg, e);
       }
-      for (int p = count_[x.seq]; p <= p1; ++p) put(x.seq, p, take(e), e);
-      count_[x.seq] = std::max(count_[x.seq], p1 + 1);
+      if (p1 >= count_[x.seq]) {
+        const int n = p1 + 1 - count_[x.seq];
+        int *row = literal(x.seq, count_[x.seq], n, e);
+        for (int p = 0; p < n; ++p) row[p] = take();
+        copy_literal(x.seq, count_[x.seq], row, n);
+        count_[x.seq] = p1 + 1;
+      }
     }
     return true;
   }
@@ -158,12 +159,15 @@ class Kv4Pages {
     for (int64_t i = 0; i < total; ++i)
       if (pages[i] < 0 || pages[i] >= n_pages()) return no("page out of range");
     for (int i = 0; i < n; ++i) {
+      if (counts[i] == 0) continue;
+      int *row = literal(seqs[i], 0, counts[i], e);
+      int taken = 0;
       for (int p = 0; p < counts[i]; ++p) {
-        const int pg = *pages++;
-        if (refs_[pg] == 0) --n_free_;
-        hold(pg, e);
-        put(seqs[i], p, pg, e);
+        const int pg = row[p] = *pages++;
+        taken += refs_[pg]++ == 0;
       }
+      n_free_ -= taken;
+      copy_literal(seqs[i], 0, row, counts[i]);
       count_[seqs[i]] = counts[i];
     }
     return true;
@@ -185,15 +189,13 @@ class Kv4Pages {
     if (need > n_free_) return no("not enough free pages");
     for (int i = 0; i < n; ++i) {
       const int whole = lens[i] / page_len_;
-      for (int p = 0; p < whole; ++p) {
-        const int pg = table_[at(src[i], p)];
-        hold(pg, e);
-        table_[at(dst[i], p)] = pg;
-      }
+      const int *from = table_.data() + at(src[i], 0);
+      int *to = table_.data() + at(dst[i], 0);
+      for (int p = 0; p < whole; ++p) ++refs_[to[p] = from[p]];
       if (whole) e->spans.push_back({(int)at(dst[i], 0), whole, (int)at(src[i], 0)});
       count_[dst[i]] = whole;
       if (lens[i] % page_len_) {
-        const int pg = take(e);
+        const int pg = take();
         e->copies.push_back({table_[at(src[i], whole)], pg});
         put(dst[i], whole, pg, e);
         count_[dst[i]] = whole + 1;
@@ -215,10 +217,10 @@ class Kv4Pages {
       if (n == 0) continue;
       int *row = table_.data() + at(seqs[i], count_[seqs[i]] - n);
       for (int p = 0; p < n; ++p) {
-        drop(row[p], e);
+        drop(row[p]);
         row[p] = -1;
       }
-      e->spans.push_back({(int)(row - table_.data()), n, -1});
+      e->spans.push_back({(int)(row - table_.data()), n, Kv4Span::kNone});
       count_[seqs[i]] -= n;
     }
     return true;
@@ -237,8 +239,6 @@ class Kv4Pages {
       refs_[hole] = refs_[pg];
       refs_[pg] = 0;
       e->copies.push_back({pg, hole});
-      touch(pg, e);
-      touch(hole, e);
       ++hole;
     }
     if (!e->copies.empty())
@@ -260,28 +260,28 @@ class Kv4Pages {
     why_ = why;
     return false;
   }
-  int take(Kv4Edits *e) {  // the lowest free page; the caller has checked that there is one
+  int take() {  // the lowest free page; the caller has checked that there is one
     while (refs_[first_free_]) ++first_free_;
     const int pg = first_free_++;
     --n_free_;
-    hold(pg, e);
+    refs_[pg] = 1;
     return pg;
   }
-  void touch(int pg, Kv4Edits *e) {
-    if (mark_[pg]) return;
-    mark_[pg] = 1;
-    e->touched.push_back(pg);
-  }
-  void hold(int pg, Kv4Edits *e) {
-    ++refs_[pg];
-    touch(pg, e);
-  }
-  void drop(int pg, Kv4Edits *e) {
+  void drop(int pg) {
     if (--refs_[pg] == 0) {
       ++n_free_;
       first_free_ = std::min(first_free_, pg);
     }
-    touch(pg, e);
+  }
+  // Room for n pages of seq from its p-th on, and the same into the table.
+  int *literal(int seq, int p, int n, Kv4Edits *e) {
+    const int i = (int)e->literal.size();
+    e->literal.resize(i + n);
+    e->spans.push_back({(int)at(seq, p), n, Kv4Span::kLiteral + i});
+    return e->literal.data() + i;
+  }
+  void copy_literal(int seq, int p, const int *row, int n) {
+    std::copy(row, row + n, table_.data() + at(seq, p));
   }
   void put(int seq, int p, int pg, Kv4Edits *e) {
     table_[at(seq, p)] = pg;
@@ -290,9 +290,7 @@ class Kv4Pages {
 
   int n_seqs_, max_pages_, page_len_, n_free_;
   int first_free_ = 0;  // no free page lies below
-  std::vector<int> count_, refs_;
-  std::vector<char> mark_;  // pages in the present change's `touched`
-  std::vector<int> table_;
+  std::vector<int> count_, refs_, table_;
   std::string why_;
 };
 

@@ -58,10 +58,9 @@ int main() {
     for (auto &c : e.spans) printf(" %d %d %d", c.to, c.n, c.from);
     printf(" T %zu", e.table.size());
     for (auto &c : e.table) printf(" %d %d", c.first, c.second);
-    printf(" R %zu", e.touched.size());
-    for (int p : e.touched) printf(" %d %d", p, k.refs(p));
+    printf(" L %zu", e.literal.size());
+    for (int p : e.literal) printf(" %d", p);
     printf("\n");
-    k.done(&e);
     fflush(stdout);
   }
 }
@@ -77,6 +76,9 @@ def driver(tmp_path_factory):
                     "-fno-sanitize-recover=all", "-D_GLIBCXX_ASSERTIONS", "-I",
                     os.path.join(PKG, "csrc"), str(d / "t.cpp"), "-o", exe], check=True)
     return exe
+
+
+LITERAL = 1 << 30  # Kv4Span::kLiteral
 
 
 class Model:
@@ -103,7 +105,7 @@ class Model:
         at, parts = 3, {}
         while at < len(out):
             key, n = out[at], int(out[at + 1])
-            k = 3 if key == "S" else 2
+            k = {"S": 3, "L": 1}.get(key, 2)
             v = list(map(int, out[at + 2:at + 2 + k * n]))
             parts[key] = [tuple(v[i:i + k]) for i in range(0, k * n, k)]
             at += 2 + k * n
@@ -113,28 +115,26 @@ class Model:
             return ok, used, free
         froms, tos = {a for a, _ in parts["C"]}, [b for _, b in parts["C"]]
         assert not froms & set(tos) and len(tos) == len(set(tos)), "copies chain or collide"
-        assert len({t for t, _ in parts["R"]}) == len(parts["R"]), "a count is written twice"
         written = [t + i for t, n, _ in parts["S"] for i in range(n)] + [t for t, _ in parts["T"]]
-        sources = {f + i for _, n, f in parts["S"] if f >= 0 for i in range(n)}
+        sources = {f + i for _, n, f in parts["S"] if 0 <= f < LITERAL for i in range(n)}
         assert len(written) == len(set(written)) and not sources & set(written), "entries collide"
-        for t, n, f in parts["S"]:
-            self.table[t:t + n] = [-1] * n if f < 0 else self.table[f:f + n]
         for a, b in parts["C"]:
             assert self.refs[b] == 0, "copied over a page that was in use"
             self.pool[b] = list(self.pool[a])
+        lit = [p for p, in parts["L"]]
+        for t, n, f in parts["S"]:
+            self.table[t:t + n] = ([-1] * n if f < 0 else lit[f - LITERAL:f - LITERAL + n]
+                                   if f >= LITERAL else self.table[f:f + n])
         for t, pg in parts["T"]:
             self.table[t] = pg
-        for pg, r in parts["R"]:
-            self.refs[pg] = r
+        self.refs = [0] * self.N
+        for t in self.table:
+            if t >= 0:
+                self.refs[t] += 1
         return ok, used, free
 
     def check(self, free):
-        held = [0] * self.N
-        for t in self.table:
-            if t >= 0:
-                held[t] += 1
-        assert held == self.refs
-        assert free == held.count(0)
+        assert free == self.refs.count(0)
         for s in range(self.S):
             row = self.table[s * self.P:(s + 1) * self.P]
             n = sum(t >= 0 for t in row)
