@@ -13,7 +13,7 @@
 //     goes into the other operand or the result.  (The masked word by itself,
 //     the subnormal n 2^-24, would save both steps, but the instruction aligns
 //     its products by the operands' nominal exponents and loses the low bits:
-//     2.5e-6 relative error against 2e-7.);
+//     2.5e-6 relative error against 2e-7);
 //   * a query is scaled by a power of two so that its largest value is just
 //     below 2^15 and split into two halves, hi = fp16(q), lo = fp16(q - hi).
 //     The instruction has 16 rows and a KV group at most 8 heads: hi is rows
@@ -32,15 +32,19 @@
 //     output is rarely rescaled.
 //
 // Work split.  A CTA of four warps takes one (token, KV head, split of the
-// keys); a warp walks every fourth tile of 32 keys of its split on its own, its
-// tiles staged by cp.async into a private ring (a tile is two contiguous
-// groups of 16 positions with their scales), so there is no barrier between
-// the warps until the merge.  The query operand is made once per CTA and read
-// from shared memory, which leaves registers for three CTAs per SM.
+// keys); a warp walks every fourth tile of 32 keys of its split on its own.  A
+// tile is two contiguous groups of 16 positions with their scales, which one lane
+// brings by two bulk copies into the warp's private ring of two, so there is no
+// barrier between the warps until the merge.  The query operand is made once per
+// CTA and read from shared memory, which leaves registers for three CTAs per SM
+// (four with spills: 58 against 55 us).  Up to eight splits of a token are one
+// thread-block cluster and merge through distributed shared memory (72B, 8 x 4096
+// keys: 23.2 -> 19.7 us); more go through scratch and a second kernel.
 //
-// Bound by instruction issue, not by the cache's bytes: a tile of 4608 bytes
-// takes about 800 instructions, of them 290 for unpacking the codes and 64
-// matrix instructions.
+// Bound by instruction issue, not by the cache's bytes: a tile of 4608 bytes takes
+// 860 instructions, some 350 of them to bring the codes into the operands, at 2.6 a
+// cycle and SM.  72B heads on B200: 131071 keys 52.6 us (2.9 TB/s; the copies
+// alone 35.5 us), 8 x 4096 keys 19.3 us.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -66,7 +70,6 @@ struct Shape {
   static constexpr int NB = D / 32;
   static constexpr int GB = kv4_group_bytes(D);
   static constexpr int TILE = 2 * GB;
-  static constexpr int CHUNKS = TILE / 16;
   static constexpr int S_OFF = kKv4Group * (D / 2);  // K scales in a group
   static constexpr int V_OFF = GB / 2;               // V codes in a group
   static constexpr int OROW = D + 4;                 // merge row, one 16-byte step of padding
@@ -290,9 +293,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
     }
   };
 #pragma unroll
-  for (int n = 0; n < kStages - 1; ++n) {
+  for (int n = 0; n < kStages - 1; ++n)
     if (n < mine) issue(n);
-  }
 
   // The query operand: head g's values of dims 32b + 8t + 0..7, scaled and
   // split, block b by warp b.
@@ -511,7 +513,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
             x >>= 8;
             y >>= 8;
           }
-          mma16816(acc[b * 4 + j], h01, l01, h23, l23, codes_lo(x, one_k), codes_lo(y, one_k), acc[b * 4 + j]);
+          mma16816(acc[b * 4 + j], h01, l01, h23, l23, codes_lo(x, one_k), codes_lo(y, one_k),
+                   acc[b * 4 + j]);
           mma16816(acc[b * 4 + j + 1], h01, l01, h23, l23, codes_hi(x, one_k), codes_hi(y, one_k),
                    acc[b * 4 + j + 1]);
         }

@@ -33,17 +33,21 @@
 // Warp roles (384 threads): warp 0 loads Q and K, warp 2 V (TMA), warp 1 issues
 // the MMAs of the scores, warp 3 those of P.V (a thread's wait on a barrier takes
 // some 300 cycles even when it is open, during which the other one's MMAs run),
-// warps 4-7 and 8-11 are two softmax groups, one for each tile of a
-// pair.  The scores of pair n + 1 follow as soon as both groups have read those of
-// pair n, so the tensor pipe has work while the softmax of pair n runs.  Shared memory is what
-// bounds this: an MMA of 128 x 128 x 16 reads 8 KB of it in 64 cycles, all that
-// there is, beside the copies that bring K and V.  (P through shared memory, in one
-// buffer, and one issuing warp: 417 us for 509 tokens of 72B on 7680, against 322.)  The
-// running maximum is handed from tile to tile through shared memory, by a tagged
-// word per row (a barrier's wait took 300 to 800 cycles there); it is only
-// raised by a score more than 2^8 above it.  Every wait is bounded (about 2 s;
-// SI_ERR_TIMEOUT in the context's error word); on expiry every role stops, the
-// CTA's own copies and MMAs in flight are waited for (bounded) and TMEM is freed.
+// warps 4-7 and 8-11 are two softmax groups, one for each tile of a pair.  The
+// scores of pair n + 1 follow as soon as both groups have read those of pair n, so
+// the tensor pipe has work while the softmax of pair n runs.  The running maximum
+// is handed from tile to tile through shared memory, by a tagged word per row (a
+// barrier's wait took 300 to 800 cycles there); it is only raised by a score more
+// than 2^8 above it.  Every wait is bounded (about 2 s; SI_ERR_TIMEOUT in the
+// context's error word); on expiry every role stops, the CTA's own copies and MMAs
+// in flight are waited for (bounded) and TMEM is freed.
+//
+// Bound by the tensor pipe and shared memory together: an MMA of 128 x 128 x 16
+// takes 64 cycles and reads 8 KB of shared memory, all that there is in that time,
+// 4 KB with P from TMEM; a pair of tiles takes about 3900 cycles, 3100 of them MMAs.
+// 72B heads, 509 tokens on 7680 positions: P through shared memory and one issuing
+// warp 417 us, P from TMEM 362, windows taken at the next pair 337, keys a third
+// ahead 322 (three MMAs a product: 400 TFLOP/s are 1200); 7B, a prompt of 2048: 107.
 #include <algorithm>
 
 #include "si_common.cuh"
