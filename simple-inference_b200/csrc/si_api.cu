@@ -1438,7 +1438,8 @@ static si_status kv4_covered(const si_kv4 *kv, const si_kv4_run *runs, int n, in
   for (int i = 0; i < n; ++i) {
     SI_CHECK(kv->pages->seq_ok(runs[i].seq), "%s", kv->pages->why().c_str());
     SI_CHECK(runs[i].pos >= lowest && runs[i].count >= 0 &&
-                 (int64_t)runs[i].pos + runs[i].count <= kv->pages->covered(runs[i].seq),
+                 (int64_t)runs[i].pos + runs[i].count <=
+                     std::min<int64_t>(kv->max_ctx, kv->pages->covered(runs[i].seq)),
              "positions [%d, %d + %d) outside the pages of sequence %d", runs[i].pos, runs[i].pos,
              runs[i].count, runs[i].seq);
   }

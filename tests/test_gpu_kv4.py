@@ -154,6 +154,23 @@ def test_append_writes_the_rule_and_the_layout(si_ctx, heads, page):
     c.kv.free()
 
 
+def test_rows_that_are_not_16_byte_aligned(si_ctx):
+    c = Cache(si_ctx, (14, 2, 64), 1, 40, 16, seed=21)
+    k = c.rng.standard_normal((33, 2, 64)).astype(np.float32)
+    v = c.rng.standard_normal((33, 2, 64)).astype(np.float32)
+    buf = torch.zeros(2, 33 * 128 + 1, device="cuda")
+    buf[0, 1:], buf[1, :-1] = up(k).view(-1), up(v).view(-1)
+    torch.cuda.synchronize()
+    c.kv.append(buf[0, 1:], buf[1], [(0, 0, 33)])
+    ko, vo = (torch.zeros(33, 2, 64, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    c.kv.read([(0, 0, 33)], ko, vo)
+    si_ctx.status()
+    for x, y in ((k, ko), (v, vo)):
+        np.testing.assert_array_equal(y.cpu().numpy(), ref.values(*ref.quantise(x)).astype(np.float32))
+    c.kv.free()
+
+
 def test_append_of_many_runs(si_ctx):
     """More runs than one launch takes, one token each."""
     c = Cache(si_ctx, (1, 1, 64), 700, 3, 16, seed=2)
@@ -283,7 +300,7 @@ def test_sharp_and_flat_softmax(si_ctx):
 # few tokens (the key axis split over CTAs) and a ragged last tile of rows and keys.
 PROMPTS = [((28, 4, 128), 0, 530), ((64, 8, 128), 520, 131), ((12, 2, 128), 2500, 131),
            ((14, 2, 64), 3200, 131), ((64, 8, 128), 7990, 17), ((4, 4, 128), 9000, 24),
-           ((8, 1, 128), 6001, 129)]
+           ((8, 1, 128), 6001, 129), ((6, 2, 128), 4001, 71)]
 
 
 @pytest.mark.parametrize("heads,prefix,count", PROMPTS)
@@ -391,6 +408,91 @@ def test_large_page_changes(si_ctx):
     c.kv.read([(2, p, k) for _, p, k in spots], ko, vo)
     si_ctx.status()
     np.testing.assert_array_equal(vo.cpu().numpy(), want)
+    c.kv.free()
+
+
+def test_pool_beyond_four_gigabytes(si_ctx):
+    """Pages at the end of a pool of 5.9 GB: written, read, attended by both kernels,
+    copied and moved."""
+    heads, P = (64, 8, 128), 128
+    dims = dims_of(*heads)
+    n_pages = 40000
+    assert n_pages * sib200.kv4_page_bytes(dims, P) > 5 << 30
+    c = Cache.__new__(Cache)
+    c.ctx, (c.hq, c.hkv, c.D), c.dims, c.P, c.n_pages = si_ctx, heads, dims, P, n_pages
+    c.kv = si_ctx.kv4(dims, 2, 1024, n_pages, P)
+    c.rng = np.random.default_rng(22)
+    c.k = [np.zeros((1024, 8, 128)) for _ in range(2)]
+    c.v = [np.zeros((1024, 8, 128)) for _ in range(2)]
+    c.kv.assign([0], [8], np.arange(n_pages - 8, n_pages)[::-1])
+    c.random([(0, 0, 1000)])
+    runs = [(0, 999, 1), (0, 868, 131)]
+    q = c.rng.standard_normal((132, 64, 128))
+    got = c.attend(q, runs)
+    c.check(got, q, runs, every=40)
+    c.kv.fork([0], [1], [1000])        # the last page is copied to the front
+    c.k[1], c.v[1] = c.k[0], c.v[0]
+    one = [(1, 999, 1)]
+    first = c.attend(q[:1], one)
+    c.check(first, q[:1], one)
+    assert c.kv.compact() == 9
+    np.testing.assert_array_equal(c.attend(q[:1], one), first)
+    ko, vo = (torch.zeros(1000, 8, 128, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    c.kv.read([(0, 0, 1000)], ko, vo)
+    si_ctx.status()
+    np.testing.assert_array_equal(vo.cpu().numpy(), c.v[0][:1000].astype(np.float32))
+    c.kv.free()
+
+
+def test_captured_calls_share_the_workspace(si_ctx):
+    """Two graphs of append and attention calls (tokens, and a prompt with tokens) over
+    the same workspaces, replayed in turn with new inputs, against eager calls."""
+    c = Cache(si_ctx, (12, 2, 128), 3, 3000, 64, seed=23)
+    lens = [2700, 900, 64]
+    c.random([(s, 0, n) for s, n in enumerate(lens)])
+    runs_a = [(0, 2699, 1), (1, 899, 1), (2, -1, 1)]
+    runs_b = [(0, 2560, 140), (1, 880, 20)]
+    qa, qb = torch.zeros(3, 12, 128, device="cuda"), torch.zeros(160, 12, 128, device="cuda")
+    new = torch.zeros(2, 2, 2, 128, device="cuda")
+    oa, ob = torch.zeros_like(qa), torch.zeros_like(qb)
+    torch.cuda.synchronize()
+
+    def call_a():
+        c.kv.append(new[0], new[1], [(0, 2699, 1), (1, 899, 1)])
+        si_ctx.attention_kv4(c.kv, c.dims, qa, runs_a, oa)
+
+    def call_b():
+        si_ctx.attention_kv4(c.kv, c.dims, qb, runs_b, ob)
+
+    call_a()
+    call_b()
+    ga, gb = si_ctx.capture(call_a), si_ctx.capture(call_b)
+    g = torch.Generator("cuda").manual_seed(5)
+    for _ in range(3):
+        for t in (qa, qb, new):
+            t.normal_(generator=g)
+        torch.cuda.synchronize()
+        ga.launch()
+        gb.launch()
+        ga.launch()
+        si_ctx.status()
+        a, b = oa.clone(), ob.clone()
+        oa.zero_()
+        ob.zero_()
+        torch.cuda.synchronize()
+        call_a()
+        call_b()
+        si_ctx.status()
+        assert torch.equal(a, oa) and torch.equal(b, ob)
+        kq = ref.values(*ref.quantise(new[0].cpu().numpy()))
+        vq = ref.values(*ref.quantise(new[1].cpu().numpy()))
+        for i, (s, p) in enumerate(((0, 2699), (1, 899))):
+            c.k[s][p], c.v[s][p] = kq[i], vq[i]
+        c.check(a.cpu().numpy(), qa.cpu().numpy(), runs_a)
+        c.check(b.cpu().numpy(), qb.cpu().numpy(), runs_b, every=39)
+    ga.free()
+    gb.free()
     c.kv.free()
 
 
@@ -621,6 +723,9 @@ def test_refusals(si_ctx):
     no(kv.append, t, t, [(0, 0, -1)])
     no(kv.reserve, [(0, 60, 1)])
     no(kv.read, [(0, 20, 13)], t, t)                    # past its pages
+    kv.reserve([(0, 32, 28)])
+    no(kv.read, [(0, 60, 1)], t, t)                     # past max_ctx, within its last page
+    kv.release([0], [20])
     no(kv.read, [(1, 0, 1)], t, t)
     no(kv.read, [(0, -1, 2)], t, t)
     no(kv.read, [(0, 0, 1)], t.view(-1)[1:], t)         # not 16-byte aligned
