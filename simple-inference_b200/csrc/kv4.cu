@@ -47,62 +47,81 @@ __device__ __forceinline__ int kv4_run_of(const Kv4Runs &r, int t) {
   return lo;
 }
 
-// A warp takes whole rows: lane j of the D/4 lanes of a row holds dims 4j ..
-// 4j + 3, one 16-byte load, which is one half-word of the row (block b = j / 8,
-// group g = j % 8), so a block's eight lanes find its extreme by three exchanges
-// and no code moves between lanes.  At D = 64 a warp takes two rows at once.
-template <int D>
-__device__ __forceinline__ void kv4_store_row(const float4 x, uint8_t *codes, uint16_t *scales,
-                                              int j) {
-  constexpr int NB = D / 32;
-  const float v[4] = {x.x, x.y, x.z, x.w};
-  // The largest magnitude as bits (a NaN is largest of all), and the first value
-  // that has it.
-  uint32_t a[4], am = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    a[i] = __float_as_uint(fabsf(v[i]));
-    am = max(am, a[i]);
-  }
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, o));
-  float own = v[3];
-#pragma unroll
-  for (int i = 2; i >= 0; --i)
-    if (a[i] == am) own = v[i];
-  const bool has = a[0] == am || a[1] == am || a[2] == am || a[3] == am;
-  const int lane = threadIdx.x & 31, base = lane & ~7;
-  const uint32_t who = (__ballot_sync(0xffffffffu, has) >> base) & 0xffu;
-  const float m = __shfl_sync(0xffffffffu, own, base + __ffs(who) - 1);
-  const float d = __fmul_rn(m, -0.125f);  // m / -8, exact
-  const float id = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int q = __float2int_rz(__fadd_rn(__fmul_rn(v[i], id), 8.5f));
-    w |= (uint32_t)min(max(q, 0), 15) << (4 * i);
-  }
-  const int b = j >> 3, g = j & 7;
-  if (codes) {
-    reinterpret_cast<uint16_t *>(codes)[g * NB + b] = (uint16_t)w;
-    if (g == 0) scales[b] = f32_to_f16(d);
-  }
+// The later of two values of a row, in their order, if its magnitude is larger (as
+// bits: a NaN is largest of all), else the first.
+__device__ __forceinline__ float larger(float first, float later) {
+  return __float_as_uint(fabsf(later)) > __float_as_uint(fabsf(first)) ? later : first;
 }
 
-// CTAs of four warps, grid (tokens, ceil(units / kUnits)): a unit is a query head
+// A warp takes whole rows: lane j of the D/4 lanes of a row holds dims 4j ..
+// 4j + 3, one 16-byte load, which is one half-word of the row (block b = j / 8,
+// group g = j % 8), so no code moves between lanes.  At D = 64 a warp takes two
+// rows at once.  The N rows of a lane are quantised together: the eight lanes of a
+// block halve the rows they hold at each exchange, so that lane g ends with the
+// extreme of row g % N, divides once and stores one scale (one row after the
+// other, with everything in every lane: 19 us for 4099 tokens of 72B; together
+// 17).  Row k is row r16 of the half-group dst(k), null for one that is not stored.
+template <int D, int N, typename Dst>
+__device__ __forceinline__ void kv4_store_rows(const float4 (&x)[N], int j, int r16, Dst dst) {
+  static_assert(N == 2 || N == 4, "rows of a lane");
+  constexpr int NB = D / 32;
+  const int b = j >> 3, g = j & 7;
+  float m[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    m[k] = larger(larger(larger(x[k].x, x[k].y), x[k].z), x[k].w);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    const bool up = g & o;  // the other lane's values come before this one's
+#pragma unroll
+    for (int k = 0; k < (o < N ? N / (2 * o) : 1); ++k) {
+      float own = m[k], send = m[k];
+      if (o < N) {  // of rows 2k and 2k + 1 of those still held, keep one
+        own = up ? m[2 * k + 1] : m[2 * k];
+        send = up ? m[2 * k] : m[2 * k + 1];
+      }
+      const float other = __shfl_xor_sync(0xffffffffu, send, o);
+      m[k] = larger(up ? other : own, up ? own : other);
+    }
+  }
+  const float d = __fmul_rn(m[0], -0.125f);  // m / -8, exact
+  const float id = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float r = __shfl_sync(0xffffffffu, id, (threadIdx.x & 24) + k);
+    // The code in the last bits of 2^23 + code, rounded towards zero; what is no
+    // number gives 0.
+    auto code = [r](float v) {
+      const float t = fminf(fmaxf(__fadd_rn(__fmul_rn(v, r), 8.5f), 0.0f), 15.5f);
+      return __float_as_uint(__fadd_rz(t, 8388608.0f));
+    };
+    const uint32_t w = code(x[k].x) + (code(x[k].y) << 4) + (code(x[k].z) << 8) +
+                       (code(x[k].w) << 12);
+    if (uint8_t *half = dst(k))
+      reinterpret_cast<uint16_t *>(half + r16 * (D / 2))[g * NB + b] = (uint16_t)w;
+  }
+  if (g < N)
+    if (uint8_t *half = dst(g))
+      reinterpret_cast<uint16_t *>(half + kKv4Group * (D / 2))[r16 * NB + b] = f32_to_f16(d);
+}
+
+// CTAs of kWarps warps, grid (tokens, ceil(units / kUnits)): a unit is a query head
 // (rotated into q_out; none without q_out), then the K rows, then the V rows of
-// the token; a warp loads its units before it works on them.  With tables the K
-// rows and queries are rotated first (rope_kv.cu's arithmetic).  A position
-// without a page, or whose page other sequences hold too, is not written and
-// recorded as SI_ERR_INVALID.
-constexpr int kUnits = 16;
+// the token; a warp loads its kRows units before it works on them.  Bound by the
+// latency of the loads and the warps that an SM holds: rows written and read back,
+// 4099 tokens of 72B, 28 us with four warps of four rows, 31 with two rows each or
+// in eight warps, 30 with two warps of eight, 35 with a whole token per warp (their
+// bytes alone would take 12).  With tables the K rows and queries are rotated first
+// (rope_kv.cu's arithmetic).  A position without a page, or whose page other
+// sequences hold too, is not written and recorded as SI_ERR_INVALID.
+constexpr int kWarps = 4, kRows = 4, kUnits = kWarps * kRows;
 
 template <int D, bool VEC>
-__global__ void __launch_bounds__(128) k_kv4_append(const __grid_constant__ Kv4AppendArgs a) {
+__global__ void __launch_bounds__(32 * kWarps) k_kv4_append(const __grid_constant__ Kv4AppendArgs a) {
   pdl_trigger();
   pdl_wait();
   constexpr int HALF = D / 2, LPR = D / 4, RPW = 32 / LPR;  // lanes per row, rows per warp
-  constexpr int N = kUnits / (4 * RPW);                     // row loads per warp
+  constexpr int N = kRows / RPW;
   const int t = blockIdx.x, lane = threadIdx.x & 31, j = lane % LPR;
   const int nq = a.q_out ? a.n_q_heads : 0, Hkv = a.kv.n_kv_heads, units = nq + 2 * Hkv;
   int seq, pos, row = t;
@@ -142,7 +161,6 @@ __global__ void __launch_bounds__(128) k_kv4_append(const __grid_constant__ Kv4A
     s = *reinterpret_cast<const float4 *>(a.sin_tab + (size_t)pos * HALF + i);
   }
   const size_t head_bytes = (size_t)a.kv.gpp * kv4_group_bytes(D);
-  const int r16 = pos & 15;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const int u = u0 + k * RPW;
@@ -164,24 +182,27 @@ __global__ void __launch_bounds__(128) k_kv4_append(const __grid_constant__ Kv4A
     }
     if (u < nq)
       *reinterpret_cast<float4 *>(a.q_out + ((size_t)row * a.n_q_heads + u) * D + 4 * j) = x[k];
-    uint8_t *codes = nullptr;
-    if (grp && u >= nq && u < units)
-      codes = is_v ? grp + (u - nq - Hkv) * head_bytes + kv4_group_bytes(D) / 2
-                   : grp + (u - nq) * head_bytes;
-    kv4_store_row<D>(x[k], codes ? codes + r16 * (D / 2) : nullptr,
-                     codes ? reinterpret_cast<uint16_t *>(codes + kKv4Group * (D / 2)) + r16 * (D / 32)
-                           : nullptr,
-                     j);
   }
+  if (!__any_sync(0xffffffffu, u0 + (N - 1) * RPW >= nq)) return;  // queries alone
+  kv4_store_rows<D, N>(x, j, pos & 15, [&](int k) -> uint8_t * {
+    const int h = u0 + k * RPW - nq;
+    if (!grp || h < 0 || h >= 2 * Hkv) return nullptr;
+    return h < Hkv ? grp + h * head_bytes : grp + (h - Hkv) * head_bytes + kv4_group_bytes(D) / 2;
+  });
+}
+
+// Code i of a half-word less 8, exact: placed behind 2^23.
+__device__ __forceinline__ float code_at(uint32_t w, int i) {
+  return __uint_as_float(((w >> (4 * i)) & 15u) | 0x4b000000u) - 8388616.0f;
 }
 
 // Rows back to fp32, laid out as above: grid (tokens, ceil(2 Hkv / kUnits)).  A
 // position without a page reads as zeros and is recorded.
 template <int D>
-__global__ void __launch_bounds__(128) k_kv4_read(const __grid_constant__ Kv4ReadArgs a) {
+__global__ void __launch_bounds__(32 * kWarps) k_kv4_read(const __grid_constant__ Kv4ReadArgs a) {
   pdl_trigger();
   pdl_wait();
-  constexpr int NB = D / 32, LPR = D / 4, RPW = 32 / LPR, N = kUnits / (4 * RPW);
+  constexpr int NB = D / 32, LPR = D / 4, RPW = 32 / LPR, N = kRows / RPW;
   const int lane = threadIdx.x & 31, j = lane % LPR, Hkv = a.kv.n_kv_heads;
   const int row = a.runs.row0[0] + blockIdx.x, r = kv4_run_of(a.runs, row);
   const int pos = a.runs.pos[r] + row - a.runs.row0[r];
@@ -212,8 +233,8 @@ __global__ void __launch_bounds__(128) k_kv4_read(const __grid_constant__ Kv4Rea
     float *out = u < Hkv ? a.k : a.v;
     if (!out) continue;
     *reinterpret_cast<float4 *>(out + ((size_t)row * Hkv + (u < Hkv ? u : u - Hkv)) * D + 4 * j) =
-        make_float4(sc[k] * (float)((int)(w[k] & 15) - 8), sc[k] * (float)((int)((w[k] >> 4) & 15) - 8),
-                    sc[k] * (float)((int)((w[k] >> 8) & 15) - 8), sc[k] * (float)((int)(w[k] >> 12) - 8));
+        make_float4(sc[k] * code_at(w[k], 0), sc[k] * code_at(w[k], 1), sc[k] * code_at(w[k], 2),
+                    sc[k] * code_at(w[k], 3));
   }
 }
 
@@ -280,14 +301,14 @@ cudaError_t launch_kv4_append(const Kv4AppendArgs &a, cudaStream_t s) {
             reinterpret_cast<uintptr_t>(a.v) | 4 * a.ldq | 4 * a.ldkv) & 15) == 0;
   auto *kern = a.kv.head_dim == 128 ? (vec ? k_kv4_append<128, true> : k_kv4_append<128, false>)
                                     : (vec ? k_kv4_append<64, true> : k_kv4_append<64, false>);
-  return launch_pdl(kern, grid, dim3(128), 0, s, a);
+  return launch_pdl(kern, grid, dim3(32 * kWarps), 0, s, a);
 }
 
 cudaError_t launch_kv4_read(const Kv4ReadArgs &a, cudaStream_t s) {
   if (a.T <= 0) return cudaSuccess;
   const dim3 grid(a.T, (2 * a.kv.n_kv_heads + kUnits - 1) / kUnits);
-  return a.kv.head_dim == 128 ? launch_pdl(k_kv4_read<128>, grid, dim3(128), 0, s, a)
-                              : launch_pdl(k_kv4_read<64>, grid, dim3(128), 0, s, a);
+  return a.kv.head_dim == 128 ? launch_pdl(k_kv4_read<128>, grid, dim3(32 * kWarps), 0, s, a)
+                              : launch_pdl(k_kv4_read<64>, grid, dim3(32 * kWarps), 0, s, a);
 }
 
 template <int WORDS>

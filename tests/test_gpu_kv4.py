@@ -154,6 +154,30 @@ def test_append_writes_the_rule_and_the_layout(si_ctx, heads, page):
     c.kv.free()
 
 
+@pytest.mark.parametrize("heads", [(8, 1, 64), (9, 3, 64), (5, 5, 128), (64, 8, 128)])
+def test_ties_infinities_and_nan_of_every_row(si_ctx, heads):
+    """The first of a block's values of largest magnitude gives the sign of its scale,
+    whichever lane holds it; a block with a NaN reads as NaN, one with an infinity
+    as infinities and NaN."""
+    c = Cache(si_ctx, heads, 1, 64, 16, seed=12)
+    hq, hkv, D = heads
+    c.shuffle([64])
+    k = c.rng.choice([-1.0, 1.0, 0.25, -0.25], (64, hkv, D)).astype(np.float32)
+    v = c.rng.choice([-2.0, 2.0], (64, hkv, D)).astype(np.float32)
+    k[40:44, :, 5] = np.inf
+    k[42:44, :, 37] = -np.inf
+    v[50, :, D - 1] = np.nan
+    c.append([(0, 0, 64)], k, v)
+    gk, gv = (torch.empty((64, hkv, D), device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    c.kv.read([(0, 0, 64)], gk, gv)
+    si_ctx.status()
+    for got, rows in ((gk, k), (gv, v)):
+        with np.errstate(invalid="ignore"):
+            want = ref.values(*ref.quantise(rows)).astype(np.float32)
+        assert np.array_equal(got.cpu().numpy(), want, equal_nan=True)
+
+
 def test_rows_that_are_not_16_byte_aligned(si_ctx):
     c = Cache(si_ctx, (14, 2, 64), 1, 40, 16, seed=21)
     k = c.rng.standard_normal((33, 2, 64)).astype(np.float32)
