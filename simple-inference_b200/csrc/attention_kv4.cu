@@ -42,8 +42,8 @@
 // keys: 23.2 -> 19.7 us); more go through scratch and a second kernel.
 //
 // Bound by instruction issue, not by the cache's bytes: a tile of 4608 bytes takes
-// 860 instructions, some 350 of them to bring the codes into the operands, at 2.6 a
-// cycle and SM.  72B heads on B200: 131071 keys 52.6 us (2.9 TB/s; the copies
+// 818 instructions, some 350 of them to bring the codes into the operands, at 2.3 to
+// 2.6 a cycle and SM.  72B heads on B200: 131071 keys 52.5 us (2.9 TB/s; the copies
 // alone 35.5 us), 8 x 4096 keys 19.3 us.
 #include <algorithm>
 #include <atomic>

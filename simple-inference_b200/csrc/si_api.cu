@@ -80,9 +80,9 @@ extern "C" SI_API const char *si_last_error(void) { return g_last_error.c_str();
 struct DevBuf {
   void *p = nullptr;
   size_t bytes = 0;
-  // Once the context has captured a graph, memory that a captured kernel may
-  // hold stays until the context goes: growth sets it aside.
-  bool keep = false;
+  // What was here during a capture, a kernel of the graph may hold: growth sets it
+  // aside until the context goes.  What came later no graph holds, and it is freed.
+  bool held = false, capturing = false;
   std::vector<void *> kept;
   size_t kept_bytes = 0;
   void release() {
@@ -94,14 +94,15 @@ struct DevBuf {
   }
   si_status reserve(size_t n) {
     if (n <= bytes) return SI_OK;
-    if (keep && p) {
+    if (p && held) {
       kept.push_back(p);
       kept_bytes += bytes;
-      p = nullptr;
-      bytes = 0;
-    } else if (!keep) {
-      release();
+    } else if (p) {
+      cudaFree(p);
     }
+    p = nullptr;
+    bytes = 0;
+    held = capturing;
     cudaError_t e = cudaMalloc(&p, n);
     if (e != cudaSuccess) {
       p = nullptr;
@@ -402,13 +403,15 @@ extern "C" SI_API si_status si_graph_begin(si_ctx *ctx) {
   SI_TRY(set_device(ctx));
   SI_CUDA(cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal));
   for (DevBuf *b : {&ctx->work, &ctx->idx, &ctx->gemm, &ctx->hx, &ctx->hy, &ctx->attn, &ctx->kv4})
-    b->keep = true;
+    b->held = b->capturing = true;
   return SI_OK;
 }
 
 extern "C" SI_API si_status si_graph_end(si_ctx *ctx, si_graph **out) {
   SI_TRY(set_device(ctx));
   SI_CHECK(out, "null output handle");
+  for (DevBuf *b : {&ctx->work, &ctx->idx, &ctx->gemm, &ctx->hx, &ctx->hy, &ctx->attn, &ctx->kv4})
+    b->capturing = false;
   si_graph *g = new si_graph();
   cudaError_t e = cudaStreamEndCapture(ctx->stream, &g->graph);
   if (e == cudaSuccess) e = cudaGraphInstantiate(&g->exec, g->graph, 0);

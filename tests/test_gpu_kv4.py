@@ -469,6 +469,53 @@ def test_pool_beyond_four_gigabytes(si_ctx):
     c.kv.free()
 
 
+def test_workspaces_after_a_capture():
+    """A workspace that a graph holds outlives its growth; those that came after the
+    capture do not pile up."""
+    def filled(ctx):
+        c = Cache(ctx, (12, 2, 128), 1, 2048, 64, seed=24)
+        c.random([(0, 0, 2048)])
+        return c, torch.randn(2048, 12, 128, device="cuda", generator=torch.Generator("cuda").manual_seed(6))
+
+    def attend(c, q, count, out):
+        c.ctx.attention_kv4(c.kv, c.dims, q[:count], [(0, 2048 - count, count)], out)
+
+    counts = range(300, 2049, 76)
+    ctx = sib200.Context(0, max_positions=64, head_dim=128)
+    c, q = filled(ctx)
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    for count in counts:  # not all need less than the last: fewer rows split the keys
+        attend(c, q, count, out)
+    ctx.status()
+    need = ctx.scratch_bytes()
+    c.kv.free()
+    ctx.close()
+
+    ctx = sib200.Context(0, max_positions=64, head_dim=128)
+    c, q = filled(ctx)
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    attend(c, q, 200, out)
+    ctx.status()
+    want = out.clone()
+    torch.cuda.synchronize()
+    first = ctx.scratch_bytes()
+    graph = ctx.capture(lambda: attend(c, q, 200, out))
+    for count in counts:
+        attend(c, q, count, out)
+    ctx.status()
+    assert ctx.scratch_bytes() <= first + need
+    out.zero_()
+    torch.cuda.synchronize()
+    graph.launch()
+    ctx.status()
+    assert torch.equal(out, want)
+    graph.free()
+    c.kv.free()
+    ctx.close()
+
+
 def test_captured_calls_share_the_workspace(si_ctx):
     """Two graphs of append and attention calls (tokens, and a prompt with tokens) over
     the same workspaces, replayed in turn with new inputs, against eager calls."""
