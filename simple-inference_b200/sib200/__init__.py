@@ -190,6 +190,11 @@ def _p(x):
         return None
     if isinstance(x, int):
         return x
+    if type(x) is np.ndarray:
+        try:  # 0.3 us; x.ctypes.data takes 0.8 of a call's 6
+            return C.addressof(C.c_byte.from_buffer(x))
+        except (TypeError, ValueError, BufferError):  # read-only, empty or strided
+            return x.ctypes.data
     if hasattr(x, "data_ptr"):
         return x.data_ptr()
     return x.ctypes.data
