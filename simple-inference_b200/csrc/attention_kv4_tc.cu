@@ -214,6 +214,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_wait();  // the operands' kernels
   const uint32_t tmem = *tmem_slot;
   auto fail = [&]() {
     if (p.err) atomicCAS(p.err, 0, 6 /* SI_ERR_TIMEOUT */);
@@ -860,10 +861,8 @@ cudaError_t launch(const Kv4PromptArgs &a, char *base, const Scratch &sc, cudaSt
     return cudaFuncGetAttributes(&fa, k_attn_kv4_tc<D>) == cudaSuccess ? fa.numRegs : 0;
   }();
   if (regs < kRegs) return cudaErrorInvalidConfiguration;
-  count_launch();
-  k_attn_kv4_tc<D><<<dim3(p.ntiles_rows, Hkv, p.nsplit), THREADS, S::SMEM, s>>>(mQh, mQl, mKh, mKl,
-                                                                               mVh, mVl, p);
-  e = cudaGetLastError();
+  e = launch_pdl(k_attn_kv4_tc<D>, dim3(p.ntiles_rows, Hkv, p.nsplit), dim3(THREADS), S::SMEM, s, mQh,
+                 mQl, mKh, mKl, mVh, mVl, p);
   if (e != cudaSuccess || p.nsplit == 1) return e;
   return launch_pdl(k_kv4_tc_combine<D>, dim3(Hq, a.T), dim3(D), 0, s, p);
 }
