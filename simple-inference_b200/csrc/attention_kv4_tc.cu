@@ -154,13 +154,8 @@ __device__ __forceinline__ uint32_t pack_h2(float x, float y) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// x in two fp16 halves, two values per register.
-__device__ __forceinline__ void split_h2(float x, float y, uint32_t &hi, uint32_t &lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  hi = *reinterpret_cast<const uint32_t *>(&h);
-  lo = pack_h2(x - f.x, y - f.y);
-}
+__device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2 *>(&x); }
+__device__ __forceinline__ uint32_t h2bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -645,15 +640,21 @@ __global__ void __launch_bounds__(256) k_kv4_absmax(const __grid_constant__ Kv4V
 }
 
 // The split operands of Q, K and V, in one launch: the first Hkv * Lp / 64 CTAs
-// take (64 positions, KV head) of the cache, the others eight query rows each.
+// take (64 positions, KV head) of the cache, the others kQRows query rows each.
 //
 // Q: q * scale, times the power of two that puts the row's largest value just
-// below 2^14, split; rowf undoes it.  One warp per (token, head) row.
+// below 2^14, split; rowf undoes it.  A warp takes rows one by one, the loads of
+// four ahead of their arithmetic.
 // K as [Hkv][Lp][D] and V transposed as [Hkv][D][Lp], hi and lo halves, zero
 // past L: every CTA first finds its head's largest scales among the pieces' (a
-// head's first one writes them down for the attention); a thread per half-word of four codes; V goes through shared memory for
-// the transpose, its 16-byte pieces XORed by the position's octet so that the
-// reads along positions meet different banks.
+// head's first one writes them down for the attention).  A thread takes 16 bytes of
+// codes, four times eight neighbouring dims, by packed fp16 arithmetic: the rounded
+// product is hi, its exact remainder lo.  (The scale times the head's power of two
+// is an fp16 number again; of scales 2^-25 of the largest and less it loses bits
+// that lie below 2^-36 of the largest value.)  V goes through shared memory for the
+// transpose, two dims of eight positions per thread; the 16-byte pieces are XORed by
+// the position's octet and parity, so that neither side meets a bank twice.
+constexpr int kQRows = 32;
 struct SplitArgs {
   Kv4View kv;
   int seq, L, Lp, pieces, q_rows;
@@ -673,29 +674,52 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
   __shared__ __align__(16) __half sh[BK * D], sl[BK * D];
   const int kv_ctas = a.Lp / BK * a.kv.n_kv_heads;
   if ((int)blockIdx.x >= kv_ctas) {
-    constexpr int N = D / 32;  // values per lane
-    const int row = (blockIdx.x - kv_ctas) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (row >= a.q_rows) return;
-    float x[N], am = 0.0f;
+    constexpr int N = D / 32, R = kQRows / 8;  // values per lane, rows per warp
+    const int row0 = (blockIdx.x - kv_ctas) * kQRows + (threadIdx.x >> 5) * R, lane = threadIdx.x & 31;
+    float x[R][N];
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float2 v = *reinterpret_cast<const float2 *>(a.q + (size_t)row * D + lane * N + i);
-      x[i] = __fmul_rn(v.x, a.scale);
-      x[i + 1] = __fmul_rn(v.y, a.scale);
-      am = fmaxf(am, fmaxf(fabsf(x[i]), fabsf(x[i + 1])));
+    for (int r = 0; r < R; ++r) {
+      const float *src = a.q + (size_t)(row0 + r) * D + lane * N;
+      if (row0 + r >= a.q_rows) break;
+      if constexpr (N == 4) {
+        const float4 v = *reinterpret_cast<const float4 *>(src);
+        x[r][0] = v.x; x[r][1] = v.y; x[r][2] = v.z; x[r][3] = v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2 *>(src);
+        x[r][0] = v.x; x[r][1] = v.y;
+      }
     }
-    const int ex = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(am)) >> 23);
-    const int e = max(-126, min(127, 13 - (ex - 127)));
-    const float up = __int_as_float((e + 127) << 23);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float u = x[i] * up, v = x[i + 1] * up;
-      const float hu = bf16_part(u), hv = bf16_part(v);
-      const size_t at = ((size_t)row * D + lane * N + i) / 2;
-      reinterpret_cast<uint32_t *>(a.qh)[at] = pack_h2(hu, hv);
-      reinterpret_cast<uint32_t *>(a.ql)[at] = pack_h2(u - hu, v - hv);
+    for (int r = 0; r < R; ++r) {
+      const int row = row0 + r;
+      if (row >= a.q_rows) return;
+      float am = 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        x[r][i] = __fmul_rn(x[r][i], a.scale);
+        am = fmaxf(am, fabsf(x[r][i]));
+      }
+      const int ex = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(am)) >> 23);
+      const int e = max(-126, min(127, 13 - (ex - 127)));
+      const float up = __int_as_float((e + 127) << 23);
+      uint32_t h[N / 2], l[N / 2];
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const float u = x[r][i] * up, v = x[r][i + 1] * up;
+        const float hu = bf16_part(u), hv = bf16_part(v);
+        h[i / 2] = pack_h2(hu, hv);
+        l[i / 2] = pack_h2(u - hu, v - hv);
+      }
+      const size_t at = (size_t)row * D + lane * N;
+      if constexpr (N == 4) {
+        *reinterpret_cast<uint2 *>(a.qh + at) = make_uint2(h[0], h[1]);
+        *reinterpret_cast<uint2 *>(a.ql + at) = make_uint2(l[0], l[1]);
+      } else {
+        *reinterpret_cast<uint32_t *>(a.qh + at) = h[0];
+        *reinterpret_cast<uint32_t *>(a.ql + at) = l[0];
+      }
+      if (lane == 0) a.rowf[row] = ldexpf(1.0f, -e);
     }
-    if (lane == 0) a.rowf[row] = ldexpf(1.0f, -e);
     return;
   }
   const int head = blockIdx.x / (a.Lp / BK), p0 = blockIdx.x % (a.Lp / BK) * BK;
@@ -719,62 +743,90 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
   }
   const float ck = ldexpf(1.0f, operand_shift((int)mx.x));
   const float cv = ldexpf(1.0f, operand_shift((int)mx.y));
-  for (int e = threadIdx.x; e < BK * (D / 4); e += blockDim.x) {
-    const int pp = e / (D / 4), hw = e % (D / 4), pos = p0 + pp;
-    const int b = hw % NB, d = 32 * b + 4 * (hw / NB);
-    uint32_t wk = 0x8888u, wv = 0x8888u;
-    float sk = 0.0f, sv = 0.0f;
+  // (K or V, position, 16 bytes of its codes)
+  constexpr int PIECES = D / 32;
+  for (int e = threadIdx.x; e < 2 * BK * PIECES; e += blockDim.x) {
+    const bool is_v = e >= BK * PIECES;
+    const int pp = e / PIECES % BK, t = e % PIECES, pos = p0 + pp;
+    uint4 w = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+    uint32_t sc[NB / 2] = {};
+    bool bad[NB] = {};
     if (pos < a.L) {
       const int gi = pos / kKv4Group, pi = a.kv.page_of(gi), page = table[pi], r = pos % kKv4Group;
       if (page >= 0 && page < a.kv.n_pages) {
         const uint8_t *g =
             a.kv.pool + (((size_t)page * a.kv.n_kv_heads + head) * gpp + gi - pi * gpp) * GB;
-        const uint16_t *c = reinterpret_cast<const uint16_t *>(g + r * (D / 2)) + hw;
-        const uint16_t *s = reinterpret_cast<const uint16_t *>(g + kKv4Group * (D / 2)) + r * NB + b;
-        wk = c[0];
-        wv = c[GB / 4];
-        sk = f16_to_f32(s[0]) * ck;
-        sv = f16_to_f32(s[GB / 4]) * cv;
+        const uint8_t *scales = g + kKv4Group * (D / 2) + r * (2 * NB);
+        w = *reinterpret_cast<const uint4 *>(g + (is_v ? GB / 2 : 0) + r * (D / 2) + 16 * t);
         // A V scale that is no number must not reach the queries before it, whose
         // probability 0 would not mask it: its key's scores become NaN instead,
         // and with them the rows that attend it.
-        if ((s[GB / 4] & 0x7c00u) == 0x7c00u) {
-          sv = 0.0f;
-          sk = __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int i = 0; i < NB / 2; ++i) {
+          const uint32_t sv = reinterpret_cast<const uint32_t *>(scales + GB / 2)[i];
+          sc[i] = is_v ? sv : reinterpret_cast<const uint32_t *>(scales)[i];
+          bad[2 * i] = (sv & 0x7c00u) == 0x7c00u;
+          bad[2 * i + 1] = (sv & 0x7c000000u) == 0x7c000000u;
         }
       } else {
         raise_error(a.err, 1);
       }
     }
-    uint32_t kh2[2], kl2[2], vh2[2], vl2[2];
+    const uint32_t wq[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int c0 = (int)((wk >> (8 * i)) & 15u) - 8, c1 = (int)((wk >> (8 * i + 4)) & 15u) - 8;
-      const int e0 = (int)((wv >> (8 * i)) & 15u) - 8, e1 = (int)((wv >> (8 * i + 4)) & 15u) - 8;
-      split_h2(sk * (float)c0, sk * (float)c1, kh2[i], kl2[i]);
-      split_h2(sv * (float)e0, sv * (float)e1, vh2[i], vl2[i]);
+    for (int i = 0; i < 4; ++i) {
+      // Eight dims of block b: half-words of the groups 2k and 2k + 1 of this piece.
+      const int b = NB == 4 ? i : i >> 1, k = NB == 4 ? 0 : i & 1;
+      const int d = 32 * b + 8 * (NB == 4 ? t : 2 * t + k);
+      const uint32_t sel = (b & 1) ? 0x7632 : 0x5410;
+      const uint32_t c = NB == 4 ? __byte_perm(wq[b >> 1], wq[2 + (b >> 1)], sel)
+                                 : __byte_perm(wq[2 * k], wq[2 * k + 1], sel);
+      float f = f16_to_f32((uint16_t)(sc[b >> 1] >> (16 * (b & 1)))) * (is_v ? cv : ck);
+      if (bad[b]) f = is_v ? 0.0f : __int_as_float(0x7fffffff);
+      const __half2 f2 = __float2half2_rn(f);
+      uint32_t h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // dims j and j + 4: n - 8 by way of 1024 + n
+        const uint32_t m = ((c >> (4 * j)) & 0x000f000fu) | 0x64006400u;
+        const __half2 n = __hsub2(as_h2(m), __half2half2(__ushort_as_half(0x6408)));
+        const __half2 x = __hmul2_rn(f2, n);
+        h[j] = h2bits(x);
+        l[j] = h2bits(__hfma2(f2, n, __hneg2(x)));
+      }
+      const uint4 hi = make_uint4(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410),
+                                  __byte_perm(h[0], h[1], 0x7632), __byte_perm(h[2], h[3], 0x7632));
+      const uint4 lo = make_uint4(__byte_perm(l[0], l[1], 0x5410), __byte_perm(l[2], l[3], 0x5410),
+                                  __byte_perm(l[0], l[1], 0x7632), __byte_perm(l[2], l[3], 0x7632));
+      if (is_v) {
+        const int at = pp * D + (d ^ (8 * ((pp >> 3) ^ ((pp & 1) << 2))));
+        *reinterpret_cast<uint4 *>(sh + at) = hi;
+        *reinterpret_cast<uint4 *>(sl + at) = lo;
+      } else {
+        const size_t kd = ((size_t)head * a.Lp + pos) * D + d;
+        *reinterpret_cast<uint4 *>(a.kh + kd) = hi;
+        *reinterpret_cast<uint4 *>(a.kl + kd) = lo;
+      }
     }
-    const size_t kd = ((size_t)head * a.Lp + pos) * D + d;
-    *reinterpret_cast<uint2 *>(a.kh + kd) = make_uint2(kh2[0], kh2[1]);
-    *reinterpret_cast<uint2 *>(a.kl + kd) = make_uint2(kl2[0], kl2[1]);
-    const int at = pp * D + (d ^ ((pp >> 3) * 8));
-    *reinterpret_cast<uint2 *>(sh + at) = make_uint2(vh2[0], vh2[1]);
-    *reinterpret_cast<uint2 *>(sl + at) = make_uint2(vl2[0], vl2[1]);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < D * (BK / 8); e += blockDim.x) {  // a dim's eight positions
-    const int d = e / (BK / 8), o = e % (BK / 8);
-    uint32_t h[4], l[4];
+  for (int e = threadIdx.x; e < D / 2 * (BK / 8); e += blockDim.x) {  // two dims' eight positions
+    const int d = e / (BK / 8) * 2, o = e % (BK / 8);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r0 = (8 * o + 2 * j) * D + (d ^ (o * 8)), r1 = r0 + D;
-      const __half2 x = __halves2half2(sh[r0], sh[r1]), y = __halves2half2(sl[r0], sl[r1]);
-      h[j] = *reinterpret_cast<const uint32_t *>(&x);
-      l[j] = *reinterpret_cast<const uint32_t *>(&y);
+    for (int part = 0; part < 2; ++part) {
+      const __half *src = part ? sl : sh;
+      uint32_t x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        x[j] = *reinterpret_cast<const uint32_t *>(src + (8 * o + j) * D + (d ^ (8 * (o ^ ((j & 1) << 2)))));
+      const size_t vd = ((size_t)head * D + d) * a.Lp + p0 + 8 * o;
+      __half *dst = part ? a.vl : a.vh;
+      *reinterpret_cast<uint4 *>(dst + vd) =
+          make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410),
+                     __byte_perm(x[4], x[5], 0x5410), __byte_perm(x[6], x[7], 0x5410));
+      *reinterpret_cast<uint4 *>(dst + vd + a.Lp) =
+          make_uint4(__byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632),
+                     __byte_perm(x[4], x[5], 0x7632), __byte_perm(x[6], x[7], 0x7632));
     }
-    const size_t vd = ((size_t)head * D + d) * a.Lp + p0 + 8 * o;
-    *reinterpret_cast<uint4 *>(a.vh + vd) = make_uint4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<uint4 *>(a.vl + vd) = make_uint4(l[0], l[1], l[2], l[3]);
   }
 }
 
@@ -829,7 +881,7 @@ cudaError_t launch(const Kv4PromptArgs &a, char *base, const Scratch &sc, cudaSt
   if (e != cudaSuccess) return e;
   SplitArgs sa{a.kv, a.seq, L, Lp, pieces, rows, scale, a.q, part, bits, qh, ql, kh, kl, vh, vl, rowf,
                a.err};
-  e = launch_pdl(k_split<D>, dim3(Lp / BK * Hkv + (rows + 7) / 8), dim3(256), 0, s, sa);
+  e = launch_pdl(k_split<D>, dim3(Lp / BK * Hkv + (rows + kQRows - 1) / kQRows), dim3(256), 0, s, sa);
   if (e != cudaSuccess) return e;
 
   CUtensorMap mQh, mQl, mKh, mKl, mVh, mVl;
