@@ -852,12 +852,12 @@ static Scratch carve(const Kv4PromptArgs &a) {
   s.rowf = s.pieces + up(Hkv * ((L + 255) / 256) * sizeof(uint2));
   s.part = s.rowf + up((size_t)a.T * a.n_q_heads * sizeof(float));
   // Splits of the keys where the row tiles alone leave SMs idle; a split has
-  // eight tiles at least.
+  // four tiles at least (72B, 64 tokens on 1436: 33 us, with eight 37, with two 33).
   const int TQ = ROWS / G;
   const long long ctas = (long long)((a.T + TQ - 1) / TQ) * Hkv;
   const long long tiles = (long long)(Lp / BK);
   s.nsplit = (int)std::max<long long>(
-      1, std::min<long long>({148 / ctas, tiles / 8, (long long)kMaxSplits}));
+      1, std::min<long long>({148 / ctas, tiles / 4, (long long)kMaxSplits}));
   s.bytes = s.part + (s.nsplit > 1 ? (size_t)a.T * a.n_q_heads * s.nsplit * (D + 2) * 4 : 0);
   return s;
 }
