@@ -572,31 +572,66 @@ __global__ void __launch_bounds__(THREADS, 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
-// Splits of a token merged in order: grid (Hq, T), a thread per dim.
+// Splits of a row merged: a warp per (token, head), a lane D / 32 dims and one
+// split's maximum and sum; the first splits' sums are asked for before the weights
+// are known.
+static_assert(kMaxSplits <= 32, "a split per lane");
 template <int D>
-__global__ void __launch_bounds__(D) k_kv4_tc_combine(const Params p) {
+__global__ void __launch_bounds__(256) k_kv4_tc_combine(const Params p) {
   pdl_trigger();
   pdl_wait();
-  const int t = blockIdx.y;
+  constexpr int N = D / 32, AHEAD = 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const size_t row = (size_t)blockIdx.x * 8 + warp;
+  const int t = (int)(row / p.Hq);
+  if (t >= p.T) return;
   const int last_tok = min(p.T, (t / p.TQ + 1) * p.TQ) - 1;
   const int all_kt = (p.prefix + last_tok + 1 + BK - 1) / BK;
   const int per = (all_kt + p.nsplit - 1) / p.nsplit;
   const int ns = (all_kt + per - 1) / per;
   if (ns == 1) return;  // already written
-  const size_t row = (size_t)t * p.Hq + blockIdx.x, slot = row * p.nsplit;
-  const float2 *ml = reinterpret_cast<const float2 *>(p.part) + slot;
-  const float *po = p.part + (size_t)p.T * p.Hq * p.nsplit * 2 + slot * D;
-  float M = -INFINITY;
-  for (int i = 0; i < ns; ++i) M = fmaxf(M, ml[i].x);
-  const float Mu = M == -INFINITY ? 0.0f : M;
-  float L = 0.0f, o = 0.0f;
-  for (int i = 0; i < ns; ++i) {
-    const float2 x = ml[i];
-    const float f = ex2(x.x - Mu);
-    L = fmaf(x.y, f, L);
-    o = fmaf(po[(size_t)i * D + threadIdx.x], f, o);
+  const size_t slot = row * p.nsplit;
+  const float *po = p.part + (size_t)p.T * p.Hq * p.nsplit * 2 + slot * D + lane * N;
+  float v[AHEAD][N], o[N] = {};
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (i0 + i < ns) {
+        const float *src = po + (size_t)(i0 + i) * D;
+        if constexpr (N == 4) {
+          const float4 x = *reinterpret_cast<const float4 *>(src);
+          v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
+        } else {
+          const float2 x = *reinterpret_cast<const float2 *>(src);
+          v[i][0] = x.x; v[i][1] = x.y;
+        }
+      }
+  };
+  load(0);
+  float2 ml = make_float2(-INFINITY, 0.0f);
+  if (lane < ns) ml = reinterpret_cast<const float2 *>(p.part)[slot + lane];
+  float M = ml.x;
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+  const float f = ex2(ml.x - (M == -INFINITY ? 0.0f : M));
+  float L = ml.y * f;
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
+  for (int i0 = 0; i0 < ns; i0 += AHEAD) {
+    if (i0) load(i0);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const float w = __shfl_sync(0xffffffffu, f, (i0 + i) & 31);
+      if (i0 + i < ns)
+#pragma unroll
+        for (int k = 0; k < N; ++k) o[k] = fmaf(v[i][k], w, o[k]);
+    }
   }
-  p.out[row * D + threadIdx.x] = L == 0.0f ? 0.0f : o / L;
+#pragma unroll
+  for (int k = 0; k < N; ++k) o[k] = L == 0.0f ? 0.0f : o[k] / L;
+  float *dst = p.out + row * D + lane * N;
+  if constexpr (N == 4) *reinterpret_cast<float4 *>(dst) = make_float4(o[0], o[1], o[2], o[3]);
+  else *reinterpret_cast<float2 *>(dst) = make_float2(o[0], o[1]);
 }
 
 // ---- operands from the cache (layout in kv4.cu) ----------------------------
@@ -916,7 +951,7 @@ cudaError_t launch(const Kv4PromptArgs &a, char *base, const Scratch &sc, cudaSt
   e = launch_pdl(k_attn_kv4_tc<D>, dim3(p.ntiles_rows, Hkv, p.nsplit), dim3(THREADS), S::SMEM, s, mQh,
                  mQl, mKh, mKl, mVh, mVl, p);
   if (e != cudaSuccess || p.nsplit == 1) return e;
-  return launch_pdl(k_kv4_tc_combine<D>, dim3(Hq, a.T), dim3(D), 0, s, p);
+  return launch_pdl(k_kv4_tc_combine<D>, dim3((rows + 7) / 8), dim3(256), 0, s, p);
 }
 
 }  // namespace k4tc
