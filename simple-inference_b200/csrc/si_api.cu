@@ -1106,17 +1106,18 @@ static const si::Kv4Run *as_runs(const si_kv4_run *r) {
   return reinterpret_cast<const si::Kv4Run *>(r);
 }
 
-// Whether a run's attention goes through the prompt kernel.  That costs about 30 us
+// Whether a run's attention goes through the prompt kernel.  That costs some 20 us
 // a run before it starts (its operands are made first, over all keys) and then a
-// fifth of what the decode kernel takes per token and key; measured at 16 to 256
+// fifth of what the decode kernel takes per token and key; measured at 16 to 128
 // tokens on 500 to 8000 positions, the two meet near (tokens - 8) * keys * KV heads =
-// 500,000 at head_dim 128 (7B, 2000 positions: 64 tokens 35 against 38 us, 128 56
-// against 40 us; 72B, 8000: 16 tokens 52 against 56 us, 32 101 against 64 us), a
-// half more at 64, whose decode tiles take two thirds of the time.
+// 330,000 at head_dim 128 (7B, 2000 positions: 32 tokens 18 against 27 us, 64 34
+// against 29 us; 72B, 2000: 16 tokens 18 against 27 us, 32 34 against 28 us), a
+// half more at 64, whose decode tiles take two thirds of the time (0.5B, 2000: 64
+// tokens 13 against 20 us, 128 24.5 against 23.7 us).
 static bool kv4_prompt_run(const si_kv4 *kv, const si_kv4_run &r) {
   if (r.pos < 0 || r.count < 16) return false;
   const double keys = r.pos + 0.5 * r.count;
-  return (r.count - 8) * keys * kv->d.n_kv_heads * (kv->d.head_dim + 64) / 192 >= 5e5;
+  return (r.count - 8) * keys * kv->d.n_kv_heads * (kv->d.head_dim + 64) / 192 >= 3.3e5;
 }
 
 extern "C" SI_API size_t si_kv4_page_bytes(const si_dims *d, int page_len) {
