@@ -156,18 +156,22 @@ class Kv4Pages {
       seen[seqs[i]] = 1;
       total += counts[i];
     }
-    for (int64_t i = 0; i < total; ++i)
-      if (pages[i] < 0 || pages[i] >= n_pages()) return no("page out of range");
-    for (int i = 0; i < n; ++i) {
+    const unsigned limit = n_pages();
+    bool bad = false;
+    for (int64_t i = 0; i < total; ++i) bad |= (unsigned)pages[i] >= limit;
+    if (bad) return no("page out of range");
+    e->literal.reserve(e->literal.size() + total);
+    e->spans.reserve(e->spans.size() + n);
+    int *__restrict refs = refs_.data();
+    int taken = 0;
+    for (int64_t i = 0; i < total; ++i) taken += refs[pages[i]]++ == 0;
+    n_free_ -= taken;
+    for (int i = 0; i < n; pages += counts[i++]) {
       if (counts[i] == 0) continue;
-      int *row = literal(seqs[i], 0, counts[i], e);
-      int taken = 0;
-      for (int p = 0; p < counts[i]; ++p) {
-        const int pg = row[p] = *pages++;
-        taken += refs_[pg]++ == 0;
-      }
-      n_free_ -= taken;
-      copy_literal(seqs[i], 0, row, counts[i]);
+      const int at0 = (int)at(seqs[i], 0);
+      e->spans.push_back({at0, counts[i], Kv4Span::kLiteral + (int)e->literal.size()});
+      e->literal.insert(e->literal.end(), pages, pages + counts[i]);
+      std::copy(pages, pages + counts[i], table_.data() + at0);
       count_[seqs[i]] = counts[i];
     }
     return true;
@@ -216,10 +220,16 @@ class Kv4Pages {
       const int n = count_[seqs[i]] - (int)std::min<int64_t>(count_[seqs[i]], stay);
       if (n == 0) continue;
       int *row = table_.data() + at(seqs[i], count_[seqs[i]] - n);
-      for (int p = 0; p < n; ++p) {
-        drop(row[p]);
-        row[p] = -1;
+      int *__restrict refs = refs_.data();
+      int freed = 0, lowest = first_free_;
+      for (int p = 0; p < n; ++p) {  // (the page lists are in any order: no branches)
+        const int pg = row[p], left = --refs[pg];
+        freed += left == 0;
+        lowest = std::min(lowest, left == 0 ? pg : lowest);
       }
+      std::fill(row, row + n, -1);
+      n_free_ += freed;
+      first_free_ = lowest;
       e->spans.push_back({(int)(row - table_.data()), n, Kv4Span::kNone});
       count_[seqs[i]] -= n;
     }
@@ -230,28 +240,49 @@ class Kv4Pages {
   // in ascending order, to the free ones below.  Returns used.
   int compact(Kv4Edits *e) {
     const int used = n_pages() - n_free_;
-    std::vector<int> to(refs_.size(), -1);
-    int hole = 0;
-    for (int pg = used; pg < n_pages(); ++pg) {
-      if (!refs_[pg]) continue;
-      while (refs_[hole]) ++hole;
-      to[pg] = hole;
-      refs_[hole] = refs_[pg];
-      refs_[pg] = 0;
-      e->copies.push_back({pg, hole});
-      ++hole;
+    // Which pages are used follows no pattern: lists without branches.  The i-th hole
+    // takes the i-th mover; to[] is where a page ends up.
+    std::vector<int> to(refs_.size()), hole(used + 1);
+    int holes = 0, moves = 0;
+    for (int pg = 0; pg < used; ++pg) {
+      to[pg] = pg;
+      hole[holes] = pg;
+      holes += refs_[pg] == 0;
     }
-    if (!e->copies.empty())
-      for (int s = 0; s < n_seqs_; ++s)
-        for (int p = 0; p < count_[s]; ++p) {
-          const int pg = table_[at(s, p)];
-          if (to[pg] >= 0) put(s, p, to[pg], e);
-        }
-    first_free_ = used;
-    return used;
+    e->copies.resize(holes + 1);
+    for (int pg = used; pg < n_pages(); ++pg) {
+      to[pg] = hole[moves];
+      e->copies[moves] = {pg, hole[moves]};
+      moves += refs_[pg] != 0;
+    }
+    e->copies.resize(moves);
+    if (!moves) return finish_compact(used);
+    size_t entries = 0;
+    for (int s = 0; s < n_seqs_; ++s) entries += count_[s];
+    e->table.resize(entries + 1);
+    for (const auto &c : e->copies) {
+      refs_[c.second] = refs_[c.first];
+      refs_[c.first] = 0;
+    }
+    size_t edits = 0;
+    for (int s = 0; s < n_seqs_; ++s) {
+      int *row = table_.data() + at(s, 0);
+      for (int p = 0; p < count_[s]; ++p) {
+        const int pg = row[p];
+        row[p] = to[pg];
+        e->table[edits] = {(int)at(s, p), to[pg]};
+        edits += to[pg] != pg;
+      }
+    }
+    e->table.resize(edits);
+    return finish_compact(used);
   }
 
  private:
+  int finish_compact(int used) {
+    first_free_ = used;
+    return used;
+  }
   size_t at(int seq, int p) const { return (size_t)seq * max_pages_ + p; }
   int last_page(const Kv4Run &x) const {
     return (int)(((int64_t)x.pos + x.count - 1) / page_len_);
