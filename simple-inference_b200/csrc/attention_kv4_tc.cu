@@ -30,7 +30,7 @@
 //               left operand from there, which halves its shared-memory reads
 //   O += P.V    TMEM: O and O_lo; finished windows in the softmax warps' registers,
 //               half of the dims in each group
-// Warp roles (384 threads): warp 0 loads Q and K, warp 2 V (TMA), warp 1 issues
+// Warp roles (384 threads): warp 0 loads K (and Q at the start), warp 2 V (TMA), warp 1 issues
 // the MMAs of the scores, warp 3 those of P.V (a thread's wait on a barrier takes
 // some 300 cycles even when it is open, during which the other one's MMAs run),
 // warps 4-7 and 8-11 are two softmax groups, one for each tile of a pair.  The
@@ -194,12 +194,36 @@ __global__ void __launch_bounds__(THREADS, 1)
       reinterpret_cast<volatile unsigned long long *>(smem + S::OFF_M);
   float *l_s = reinterpret_cast<float *>(smem + S::OFF_L);
 
+  // K comes in units of a pair's lo, then its hi, through a ring of three: the next lo
+  // is there when a pair's scores begin, its hi follows into the place of the present
+  // lo, which the first third of the MMAs has read.
+  auto load_k = [&](int u) {
+    const uint32_t dst = smem_u32(smem + S::OFF_K) + u % 3 * S::K_BYTES;
+    mbar_expect_tx(bar(B_KF + u % 3), S::K_BYTES);
+    // (rows past this head's are read with an odd last tile, and not used)
+    const int krow = g * p.Lp + (kt0 + (u & ~1)) * BK;
+    for (int c = 0; c < S::NC; ++c)
+      tma_load_2d(dst + c * S::K_CHUNK, u & 1 ? &tmKh : &tmKl, c * 64, krow, bar(B_KF + u % 3));
+  };
+  const int k_first = min(2 * npair, 3);  // units that find the ring empty
+
   if (threadIdx.x < ROWS) m_s[threadIdx.x] = ~0ull;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NBAR; ++i)
       mbar_init(bar(i), i == B_SE || i == B_FL ? 8 : i >= B_PF && i < B_OD ? 4 : 1);  // warps
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async();
+    // Q and the first of K are on their way while TMEM is allocated.
+    pdl_wait();
+    const uint32_t qb = smem_u32(smem + S::OFF_Q);
+    mbar_expect_tx(bar(B_Q), 2 * S::NC * 128 * rows);
+    for (int c = 0; c < S::NC; ++c)
+      tma_load_3d(qb + c * S::Q_CHUNK, &tmQh, c * 64, g * p.G, t0, bar(B_Q));
+    load_k(0);
+    for (int c = 0; c < S::NC; ++c)
+      tma_load_3d(qb + S::Q_BYTES + c * S::Q_CHUNK, &tmQl, c * 64, g * p.G, t0, bar(B_Q));
+    for (int u = 1; u < k_first; ++u) load_k(u);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -220,33 +244,16 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
     if (warp == 0) {
-      // ---------------- Q and K producer ----------------
+      // ---------------- K producer ----------------
       if (lane == 0) {
-        const uint32_t qb = smem_u32(smem + S::OFF_Q), kb = smem_u32(smem + S::OFF_K);
-        mbar_expect_tx(bar(B_Q), 2 * S::NC * 128 * rows);
-        for (int c = 0; c < S::NC; ++c) {
-          tma_load_3d(qb + c * S::Q_CHUNK, &tmQh, c * 64, g * p.G, t0, bar(B_Q));
-          tma_load_3d(qb + S::Q_BYTES + c * S::Q_CHUNK, &tmQl, c * 64, g * p.G, t0, bar(B_Q));
-        }
-        // K in units of a pair's lo, then its hi, through a ring of three: the next
-        // lo is there when a pair's scores begin, its hi follows into the place of
-        // the present lo, which the first third of the MMAs has read.
-        int u = 0;
+        int u = k_first;
         for (; u < 2 * npair; ++u) {
-          const int s = u % 3;
-          if (!mbar_wait(bar(B_KE + s), ((u / 3) & 1) ^ 1, abort_flag)) break;
-          mbar_expect_tx(bar(B_KF + s), S::K_BYTES);
-          // (rows past this head's are read with an odd last tile, and not used)
-          const int krow = g * p.Lp + (kt0 + (u & ~1)) * BK;
-          for (int c = 0; c < S::NC; ++c)
-            tma_load_2d(kb + s * S::K_BYTES + c * S::K_CHUNK, u & 1 ? &tmKh : &tmKl, c * 64, krow,
-                        bar(B_KF + s));
+          if (!mbar_wait(bar(B_KE + u % 3), ((u / 3) & 1) ^ 1, abort_flag)) break;
+          load_k(u);
         }
-        if (u < 2 * npair) {
-          fail();
-          mbar_drain(bar(B_Q), 0);
-          for (int k = u > 3 ? u - 3 : 0; k < u; ++k) mbar_drain(bar(B_KF + k % 3), (k / 3) & 1);
-        }
+        if (u < 2 * npair) fail();
+        mbar_drain(bar(B_Q), 0);  // no copy outlives the CTA
+        for (int k = max(u - 3, 0); k < u; ++k) mbar_drain(bar(B_KF + k % 3), (k / 3) & 1);
       }
       __syncwarp();
     } else if (warp == 2) {
@@ -261,10 +268,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           tma_load_2d(vb, &tmVh, (kt0 + i) * BK, g * D, bar(B_VF + s));
           tma_load_2d(vb + S::V_BYTES, &tmVl, (kt0 + i) * BK, g * D, bar(B_VF + s));
         }
-        if (i < nkt) {
-          fail();
-          for (int k = i > 2 ? i - 2 : 0; k < i; ++k) mbar_drain(bar(B_VF + (k & 1)), (k >> 1) & 1);
-        }
+        if (i < nkt) fail();
+        for (int k = max(i - 2, 0); k < i; ++k) mbar_drain(bar(B_VF + (k & 1)), (k >> 1) & 1);
       }
       __syncwarp();
     } else if (warp == 1) {
