@@ -892,13 +892,24 @@ static Scratch carve(const Kv4PromptArgs &a) {
   s.pieces = s.bits + up(2 * Hkv * sizeof(int));
   s.rowf = s.pieces + up(Hkv * ((L + 255) / 256) * sizeof(uint2));
   s.part = s.rowf + up((size_t)a.T * a.n_q_heads * sizeof(float));
-  // Splits of the keys where the row tiles alone leave SMs idle; a split has
-  // four tiles at least (72B, 64 tokens on 1436: 33 us, with eight 37, with two 33).
+  // Splits of the keys where the row tiles alone leave SMs idle, as many as take the
+  // least time by this count: some 1 us a tile, for the merge 3.5 us and its sums
+  // written and read at 4 TB/s.  (7B, 64 tokens on 4136: 84, 56, 41, 34 us in 1, 2, 4
+  // and 9; 300 on 400: 26 us, 29 in two; 72B, 64 on 1436: 39, 35, 30 in 1, 2 and 4.)
   const int TQ = ROWS / G;
   const long long ctas = (long long)((a.T + TQ - 1) / TQ) * Hkv;
   const long long tiles = (long long)(Lp / BK);
-  s.nsplit = (int)std::max<long long>(
-      1, std::min<long long>({148 / ctas, tiles / 4, (long long)kMaxSplits}));
+  const int most = (int)std::min<long long>({148 / ctas, tiles, (long long)kMaxSplits});
+  double best = tiles;
+  s.nsplit = 1;
+  for (int n = 2; n <= most; ++n) {
+    const double t = (double)((tiles + n - 1) / n) + 3.5 +
+                     (double)a.T * a.n_q_heads * n * (D + 2) * 8 / 4e6;
+    if (t < best) {
+      best = t;
+      s.nsplit = n;
+    }
+  }
   s.bytes = s.part + (s.nsplit > 1 ? (size_t)a.T * a.n_q_heads * s.nsplit * (D + 2) * 4 : 0);
   return s;
 }
