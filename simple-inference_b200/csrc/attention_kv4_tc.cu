@@ -1,9 +1,10 @@
 // attention_kv4_tc.cu -- prompt attention over the paged KV cache in 4 bits, on
 // the tcgen05 tensor cores.
 //
-// The function of attention_kv4.cu for a run of consecutive tokens of one
-// sequence: token t of the run, at position prefix + t, attends positions 0 ..
-// prefix + t.
+// The function of attention_kv4.cu for runs of consecutive tokens: token t of a
+// run, at position prefix + t of its sequence, attends positions 0 .. prefix + t.
+// Up to eight runs go through one launch of each kernel (7B, four of 300 tokens on
+// 400: 49 us, one after the other 100; eight of 64 on 836: 38 and 83).
 //
 // Arithmetic.  Both contractions are sums of three fp16 MMAs with fp32
 // accumulators, over operands split in two:
@@ -21,9 +22,10 @@
 // its bits.
 //
 // Layout.  Pre-passes write the split operands: Q [T][Hq][D], K [Hkv][Lp][D], V
-// transposed [Hkv][D][Lp] (Lp = the context rounded up to 64 keys).  A CTA takes
-// 128 query rows -- TQ tokens x the G heads of a KV group -- and a split of
-// their keys, in tiles of 64:
+// transposed [Hkv][D][Lp], the runs one after the other, each one's keys rounded up
+// to 64.  A CTA takes 128 query rows of a run -- TQ tokens x the G heads of a KV
+// group -- and a split of their keys, in tiles of 64 (rows and keys of the next run
+// that a copy takes in are not used):
 //   S = Q.K^T   TMEM, two tiles by one MMA of 128 columns (one of 64 columns takes
 //               the tensor pipe as long)
 //   P           TMEM, hi and lo, a buffer for each tile of a pair: the MMA takes its
@@ -91,13 +93,36 @@ struct Shape {
 };
 static_assert(Shape<128>::SMEM <= 232448, "shared memory budget");
 
+// The runs of a launch and where their parts of the operands begin; the last one's
+// end stands behind it.
+struct Run {
+  int seq, prefix, T;
+  int row;     // first row of q and out
+  int nsplit;  // splits of the keys
+  int tok0;    // first token of the Q operand
+  int tile0;   // first row tile
+  int key0;    // first key of the K and V operands
+  int piece0;  // first piece of 256 keys
+};
+struct Runs {
+  int n;
+  Run r[kKv4MaxPrompts + 1];
+};
+// The run that item i of those counted by `first` belongs to.
+__device__ __forceinline__ const Run &run_of(const Runs &runs, int Run::*first, int i) {
+  int k = 0;
+  while (k + 1 < runs.n && runs.r[k + 1].*first <= i) ++k;
+  return runs.r[k];
+}
+
 struct Params {
-  int T, Hq, G, TQ, prefix, Lp, ntiles_rows, nsplit;
-  float *out;   // rows [T][Hq][D]
+  Runs run;
+  int T, Hq, G, TQ, Lp, nsplit;  // tokens, keys and most splits of all runs
+  float *out;   // rows [.][Hq][D]
   float *part;  // with splits: (m, l) [T][Hq][nsplit], then O [T][Hq][nsplit][D]
   int *err;
   const float *rowf;  // [T][Hq]: with K's power of two takes a row's scores to log2 units
-  const int *bits;    // [Hkv][2]: largest |scale| of K and V as fp16 bits
+  const int *bits;    // [run][Hkv][2]: largest |scale| of K and V as fp16 bits
 };
 
 // The power of two by which a KV head's K or V operands are scaled: |scale| <
@@ -163,19 +188,20 @@ __global__ void __launch_bounds__(THREADS, 1)
     k_attn_kv4_tc(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__ CUtensorMap tmQl,
                   const __grid_constant__ CUtensorMap tmKh, const __grid_constant__ CUtensorMap tmKl,
                   const __grid_constant__ CUtensorMap tmVh, const __grid_constant__ CUtensorMap tmVl,
-                  const Params p) {
+                  const __grid_constant__ Params p) {
   using S = Shape<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_align<1024>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = blockIdx.y;
-  const int rt = p.ntiles_rows - 1 - (int)blockIdx.x;  // longest row tiles first
+  const Run &run = run_of(p.run, &Run::tile0, blockIdx.x);
+  const int rt = (&run)[1].tile0 - 1 - (int)blockIdx.x;  // longest row tiles first
   const int t0 = rt * p.TQ;
   const int rows = p.G * p.TQ;
-  const int last_tok = min(p.T, t0 + p.TQ) - 1;
+  const int last_tok = min(run.T, t0 + p.TQ) - 1;
   // This split's key tiles [kt0, kt0 + nkt) of the row tile's.
-  const int all_kt = (p.prefix + last_tok + 1 + BK - 1) / BK;
-  const int per = (all_kt + p.nsplit - 1) / p.nsplit;
+  const int all_kt = (run.prefix + last_tok + 1 + BK - 1) / BK;
+  const int per = (all_kt + run.nsplit - 1) / run.nsplit;
   const int kt0 = (int)blockIdx.z * per;
   const int nkt = min(all_kt - kt0, per);
   const int nsplits = (all_kt + per - 1) / per;
@@ -200,8 +226,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   auto load_k = [&](int u) {
     const uint32_t dst = smem_u32(smem + S::OFF_K) + u % 3 * S::K_BYTES;
     mbar_expect_tx(bar(B_KF + u % 3), S::K_BYTES);
-    // (rows past this head's are read with an odd last tile, and not used)
-    const int krow = g * p.Lp + (kt0 + (u & ~1)) * BK;
+    // (rows past this run's are read with an odd last tile, and not used)
+    const int krow = g * p.Lp + run.key0 + (kt0 + (u & ~1)) * BK;
     for (int c = 0; c < S::NC; ++c)
       tma_load_2d(dst + c * S::K_CHUNK, u & 1 ? &tmKh : &tmKl, c * 64, krow, bar(B_KF + u % 3));
   };
@@ -219,10 +245,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t qb = smem_u32(smem + S::OFF_Q);
     mbar_expect_tx(bar(B_Q), 2 * S::NC * 128 * rows);
     for (int c = 0; c < S::NC; ++c)
-      tma_load_3d(qb + c * S::Q_CHUNK, &tmQh, c * 64, g * p.G, t0, bar(B_Q));
+      tma_load_3d(qb + c * S::Q_CHUNK, &tmQh, c * 64, g * p.G, run.tok0 + t0, bar(B_Q));
     load_k(0);
     for (int c = 0; c < S::NC; ++c)
-      tma_load_3d(qb + S::Q_BYTES + c * S::Q_CHUNK, &tmQl, c * 64, g * p.G, t0, bar(B_Q));
+      tma_load_3d(qb + S::Q_BYTES + c * S::Q_CHUNK, &tmQl, c * 64, g * p.G, run.tok0 + t0, bar(B_Q));
     for (int u = 1; u < k_first; ++u) load_k(u);
   }
   if (warp == 1) {
@@ -265,8 +291,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (!mbar_wait(bar(B_VE + s), ((i >> 1) & 1) ^ 1, abort_flag)) break;
           const uint32_t vb = smem_u32(smem + S::OFF_V + s * 2 * S::V_BYTES);
           mbar_expect_tx(bar(B_VF + s), 2 * S::V_BYTES);
-          tma_load_2d(vb, &tmVh, (kt0 + i) * BK, g * D, bar(B_VF + s));
-          tma_load_2d(vb + S::V_BYTES, &tmVl, (kt0 + i) * BK, g * D, bar(B_VF + s));
+          const int key = run.key0 + (kt0 + i) * BK;
+          tma_load_2d(vb, &tmVh, key, g * D, bar(B_VF + s));
+          tma_load_2d(vb + S::V_BYTES, &tmVl, key, g * D, bar(B_VF + s));
         }
         if (i < nkt) fail();
         for (int k = max(i - 2, 0); k < i; ++k) mbar_drain(bar(B_VF + (k & 1)), (k >> 1) & 1);
@@ -360,12 +387,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int r = q * 32 + lane;
     const int tl = r / p.G, hh = r - tl * p.G;
     const int tok = t0 + tl;
-    const bool valid = r < rows && tok < p.T;
-    const int pos = valid ? p.prefix + tok : -1;  // a padding row attends nothing
-    const int kshift = operand_shift(p.bits[2 * g]), vshift = operand_shift(p.bits[2 * g + 1]);
+    const bool valid = r < rows && tok < run.T;
+    const int pos = valid ? run.prefix + tok : -1;  // a padding row attends nothing
+    const int *bits = p.bits + 2 * ((int)(&run - p.run.r) * (int)gridDim.y + g);
+    const int kshift = operand_shift(bits[0]), vshift = operand_shift(bits[1]);
     // (kept above zero: a masked score times it stays -inf)
     const float rf =
-        valid ? fmaxf(ldexpf(p.rowf[(size_t)tok * p.Hq + (size_t)g * p.G + hh], -kshift), 1.2e-38f)
+        valid ? fmaxf(ldexpf(p.rowf[(size_t)(run.tok0 + tok) * p.Hq + (size_t)g * p.G + hh], -kshift), 1.2e-38f)
               : 0.0f;
     const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16);
     constexpr int H = D / 2;   // this group keeps dims [grp * H, grp * H + H) of the sums
@@ -552,12 +580,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       l = l_s[r] + l_s[ROWS + r];
       const float back = ldexpf(1.0f, -vshift);
       const size_t head = (size_t)g * p.G + hh;
-      float *orow = p.out + ((size_t)tok * p.Hq + head) * D;
+      float *orow = p.out + ((size_t)(run.row + tok) * p.Hq + head) * D;
       float f = back;
       if (nsplits == 1) {
         f = l == 0.0f ? 0.0f : back / l;
       } else if (valid) {
-        const size_t slot = ((size_t)tok * p.Hq + head) * p.nsplit + blockIdx.z;
+        const size_t slot = ((size_t)(run.tok0 + tok) * p.Hq + head) * p.nsplit + blockIdx.z;
         orow = p.part + (size_t)p.T * p.Hq * p.nsplit * 2 + slot * D;
         if (grp == 0) reinterpret_cast<float2 *>(p.part)[slot] = make_float2(m, l);
       }
@@ -583,20 +611,20 @@ __global__ void __launch_bounds__(THREADS, 1)
 // are known.
 static_assert(kMaxSplits <= 32, "a split per lane");
 template <int D>
-__global__ void __launch_bounds__(256) k_kv4_tc_combine(const Params p) {
+__global__ void __launch_bounds__(256) k_kv4_tc_combine(const __grid_constant__ Params p) {
   pdl_trigger();
   pdl_wait();
   constexpr int N = D / 32, AHEAD = 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const size_t row = (size_t)blockIdx.x * 8 + warp;
-  const int t = (int)(row / p.Hq);
-  if (t >= p.T) return;
-  const int last_tok = min(p.T, (t / p.TQ + 1) * p.TQ) - 1;
-  const int all_kt = (p.prefix + last_tok + 1 + BK - 1) / BK;
-  const int per = (all_kt + p.nsplit - 1) / p.nsplit;
+  const int row = blockIdx.x * 8 + warp, tt = row / p.Hq;
+  if (tt >= p.T) return;
+  const Run &run = run_of(p.run, &Run::tok0, tt);
+  const int last_tok = min(run.T, ((tt - run.tok0) / p.TQ + 1) * p.TQ) - 1;
+  const int all_kt = (run.prefix + last_tok + 1 + BK - 1) / BK;
+  const int per = (all_kt + run.nsplit - 1) / run.nsplit;
   const int ns = (all_kt + per - 1) / per;
   if (ns == 1) return;  // already written
-  const size_t slot = row * p.nsplit;
+  const size_t slot = (size_t)row * p.nsplit;
   const float *po = p.part + (size_t)p.T * p.Hq * p.nsplit * 2 + slot * D + lane * N;
   float v[AHEAD][N], o[N] = {};
   auto load = [&](int i0) {
@@ -635,24 +663,27 @@ __global__ void __launch_bounds__(256) k_kv4_tc_combine(const Params p) {
   }
 #pragma unroll
   for (int k = 0; k < N; ++k) o[k] = L == 0.0f ? 0.0f : o[k] / L;
-  float *dst = p.out + row * D + lane * N;
+  float *dst = p.out + ((size_t)(run.row - run.tok0) * p.Hq + row) * D + lane * N;
   if constexpr (N == 4) *reinterpret_cast<float4 *>(dst) = make_float4(o[0], o[1], o[2], o[3]);
   else *reinterpret_cast<float2 *>(dst) = make_float2(o[0], o[1]);
 }
 
 // ---- operands from the cache (layout in kv4.cu) ----------------------------
-// Largest |scale| of K and of V of each piece of 256 positions below L of each KV
+// Largest |scale| of K and of V of each piece of 256 positions of a run and each KV
 // head, as fp16 bits: grid (pieces, Hkv), part [Hkv][pieces].
 template <int D>
-__global__ void __launch_bounds__(256) k_kv4_absmax(const __grid_constant__ Kv4View kv, int seq,
-                                                    int L, uint2 *__restrict__ part) {
+__global__ void __launch_bounds__(256) k_kv4_absmax(const __grid_constant__ Kv4View kv,
+                                                    const __grid_constant__ Runs runs,
+                                                    uint2 *__restrict__ part) {
   pdl_trigger();
   pdl_wait();
   constexpr int NB = D / 32, GB = kv4_group_bytes(D);
   const int head = blockIdx.y, gpp = kv.gpp;
-  const int *table = kv.tables + (size_t)seq * kv.max_pages;
+  const Run &run = run_of(runs, &Run::piece0, blockIdx.x);
+  const int L = run.prefix + run.T;
+  const int *table = kv.tables + (size_t)run.seq * kv.max_pages;
   uint32_t mk = 0, mv = 0;
-  const int pos = blockIdx.x * 256 + threadIdx.x;
+  const int pos = ((int)blockIdx.x - run.piece0) * 256 + threadIdx.x;
   const int gi = pos / kKv4Group, pi = kv.page_of(gi), page = pos < L ? table[pi] : -1;
   if (page >= 0 && page < kv.n_pages) {
     const uint8_t *g = kv.pool + (((size_t)page * kv.n_kv_heads + head) * gpp + gi - pi * gpp) * GB +
@@ -687,8 +718,8 @@ __global__ void __launch_bounds__(256) k_kv4_absmax(const __grid_constant__ Kv4V
 // below 2^14, split; rowf undoes it.  A warp takes rows one by one, the loads of
 // four ahead of their arithmetic.
 // K as [Hkv][Lp][D] and V transposed as [Hkv][D][Lp], hi and lo halves, zero
-// past L: every CTA first finds its head's largest scales among the pieces' (a
-// head's first one writes them down for the attention).  A thread takes 16 bytes of
+// past a run's end: every CTA first finds its run's and head's largest scales among
+// the pieces' (the first one writes them down for the attention).  A thread takes 16 bytes of
 // codes, four times eight neighbouring dims, by packed fp16 arithmetic: the rounded
 // product is hi, its exact remainder lo.  (The scale times the head's power of two
 // is an fp16 number again; of scales 2^-25 of the largest and less it loses bits
@@ -698,11 +729,12 @@ __global__ void __launch_bounds__(256) k_kv4_absmax(const __grid_constant__ Kv4V
 constexpr int kQRows = 32;
 struct SplitArgs {
   Kv4View kv;
-  int seq, L, Lp, pieces, q_rows;
+  Runs run;
+  int Hq, Lp, pieces, q_rows;  // keys, pieces and query rows of all runs
   float scale;
   const float *q;
   const uint2 *part;  // [Hkv][pieces] largest |scale| of K and V, as fp16 bits
-  int *bits;          // [Hkv][2]
+  int *bits;          // [run][Hkv][2]
   __half *qh, *ql, *kh, *kl, *vh, *vl;
   float *rowf;
   int *err;
@@ -720,8 +752,10 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
     float x[R][N];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float *src = a.q + (size_t)(row0 + r) * D + lane * N;
       if (row0 + r >= a.q_rows) break;
+      const Run &run = run_of(a.run, &Run::tok0, (row0 + r) / a.Hq);
+      const int to_q = (run.row - run.tok0) * a.Hq;  // from the operand's rows to those of q
+      const float *src = a.q + (size_t)(row0 + r + to_q) * D + lane * N;
       if constexpr (N == 4) {
         const float4 v = *reinterpret_cast<const float4 *>(src);
         x[r][0] = v.x; x[r][1] = v.y; x[r][2] = v.z; x[r][3] = v.w;
@@ -763,12 +797,13 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
     }
     return;
   }
-  const int head = blockIdx.x / (a.Lp / BK), p0 = blockIdx.x % (a.Lp / BK) * BK;
-  const int gpp = a.kv.gpp;
-  const int *table = a.kv.tables + (size_t)a.seq * a.kv.max_pages;
+  const int head = blockIdx.x / (a.Lp / BK), at0 = blockIdx.x % (a.Lp / BK) * BK;
+  const Run &run = run_of(a.run, &Run::key0, at0);
+  const int p0 = at0 - run.key0, L = run.prefix + run.T, gpp = a.kv.gpp;
+  const int *table = a.kv.tables + (size_t)run.seq * a.kv.max_pages;
   __shared__ uint2 w_s[8];
   uint2 mx = make_uint2(0, 0);
-  for (int i = threadIdx.x; i < a.pieces; i += blockDim.x) {
+  for (int i = run.piece0 + threadIdx.x; i < (&run)[1].piece0; i += blockDim.x) {
     const uint2 x = a.part[(size_t)head * a.pieces + i];
     mx = make_uint2(max(mx.x, x.x), max(mx.y, x.y));
   }
@@ -779,8 +814,9 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
 #pragma unroll
   for (int i = 0; i < 8; ++i) mx = make_uint2(max(mx.x, w_s[i].x), max(mx.y, w_s[i].y));
   if (p0 == 0 && threadIdx.x == 0) {
-    a.bits[2 * head] = (int)mx.x;
-    a.bits[2 * head + 1] = (int)mx.y;
+    int *bits = a.bits + 2 * ((int)(&run - a.run.r) * a.kv.n_kv_heads + head);
+    bits[0] = (int)mx.x;
+    bits[1] = (int)mx.y;
   }
   const float ck = ldexpf(1.0f, operand_shift((int)mx.x));
   const float cv = ldexpf(1.0f, operand_shift((int)mx.y));
@@ -792,7 +828,7 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
     uint4 w = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
     uint32_t sc[NB / 2] = {};
     bool bad[NB] = {};
-    if (pos < a.L) {
+    if (pos < L) {
       const int gi = pos / kKv4Group, pi = a.kv.page_of(gi), page = table[pi], r = pos % kKv4Group;
       if (page >= 0 && page < a.kv.n_pages) {
         const uint8_t *g =
@@ -843,7 +879,7 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
         *reinterpret_cast<uint4 *>(sh + at) = hi;
         *reinterpret_cast<uint4 *>(sl + at) = lo;
       } else {
-        const size_t kd = ((size_t)head * a.Lp + pos) * D + d;
+        const size_t kd = ((size_t)head * a.Lp + at0 + pp) * D + d;
         *reinterpret_cast<uint4 *>(a.kh + kd) = hi;
         *reinterpret_cast<uint4 *>(a.kl + kd) = lo;
       }
@@ -859,7 +895,7 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         x[j] = *reinterpret_cast<const uint32_t *>(src + (8 * o + j) * D + (d ^ (8 * (o ^ ((j & 1) << 2)))));
-      const size_t vd = ((size_t)head * D + d) * a.Lp + p0 + 8 * o;
+      const size_t vd = ((size_t)head * D + d) * a.Lp + at0 + 8 * o;
       __half *dst = part ? a.vl : a.vh;
       *reinterpret_cast<uint4 *>(dst + vd) =
           make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410),
@@ -871,17 +907,34 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
   }
 }
 
-// Where the pieces of the scratch lie.
+// The runs' places, and those of the pieces of the scratch.
 struct Scratch {
-  size_t qh, ql, kh, kl, vh, vl, bits, pieces, rowf, part, bytes;
-  int nsplit;
+  Runs run;
+  int T, Lp, pieces, tiles, nsplit;  // of all runs; most splits
+  size_t qh, ql, kh, kl, vh, vl, bits, part_max, rowf, part, bytes;
 };
 static Scratch carve(const Kv4PromptArgs &a) {
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-  const int D = a.kv.head_dim, Hkv = a.kv.n_kv_heads, G = a.n_q_heads / Hkv;
-  const size_t L = (size_t)a.prefix + a.T, Lp = (L + BK - 1) / BK * BK;
-  const size_t q = up((size_t)a.T * a.n_q_heads * D * 2), kv = up(Hkv * Lp * D * 2);
-  Scratch s;
+  const int D = a.kv.head_dim, Hkv = a.kv.n_kv_heads, TQ = ROWS / (a.n_q_heads / Hkv);
+  Scratch s{};
+  Run *r = s.run.r;
+  s.run.n = a.n;
+  int longest = 0;
+  for (int i = 0; i < a.n; ++i) {
+    const Kv4Prompt &x = a.run[i];
+    const int L = x.prefix + x.T, keys = (L + BK - 1) / BK * BK;
+    r[i].seq = x.seq; r[i].prefix = x.prefix; r[i].T = x.T; r[i].row = x.row;
+    r[i + 1].tok0 = r[i].tok0 + x.T;
+    r[i + 1].tile0 = r[i].tile0 + (x.T + TQ - 1) / TQ;
+    r[i + 1].key0 = r[i].key0 + keys;
+    r[i + 1].piece0 = r[i].piece0 + (L + 255) / 256;
+    longest = std::max(longest, keys / BK);
+  }
+  s.T = r[a.n].tok0;
+  s.tiles = r[a.n].tile0;
+  s.Lp = r[a.n].key0;
+  s.pieces = r[a.n].piece0;
+  const size_t rows = (size_t)s.T * a.n_q_heads, q = up(rows * D * 2), kv = up((size_t)Hkv * s.Lp * D * 2);
   s.qh = 0;
   s.ql = s.qh + q;
   s.kh = s.ql + q;
@@ -889,28 +942,33 @@ static Scratch carve(const Kv4PromptArgs &a) {
   s.vh = s.kl + kv;
   s.vl = s.vh + kv;
   s.bits = s.vl + kv;
-  s.pieces = s.bits + up(2 * Hkv * sizeof(int));
-  s.rowf = s.pieces + up(Hkv * ((L + 255) / 256) * sizeof(uint2));
-  s.part = s.rowf + up((size_t)a.T * a.n_q_heads * sizeof(float));
-  // Splits of the keys where the row tiles alone leave SMs idle, as many as take the
-  // least time by this count: some 1 us a tile, for the merge 3.5 us and its sums
-  // written and read at 4 TB/s.  (7B, 64 tokens on 4136: 84, 56, 41, 34 us in 1, 2, 4
-  // and 9; 300 on 400: 26 us, 29 in two; 72B, 64 on 1436: 39, 35, 30 in 1, 2 and 4.)
-  const int TQ = ROWS / G;
-  const long long ctas = (long long)((a.T + TQ - 1) / TQ) * Hkv;
-  const long long tiles = (long long)(Lp / BK);
-  const int most = (int)std::min<long long>({148 / ctas, tiles, (long long)kMaxSplits});
-  double best = tiles;
+  s.part_max = s.bits + up((size_t)a.n * 2 * Hkv * sizeof(int));
+  s.rowf = s.part_max + up((size_t)Hkv * s.pieces * sizeof(uint2));
+  s.part = s.rowf + up(rows * sizeof(float));
+  // Splits of the keys, into about as many tiles each, where the row tiles alone
+  // leave SMs idle, as many as take the least time by this count: some 1 us a tile,
+  // for the merge 3.5 us and its sums written and read at 4 TB/s.  (7B, 64 tokens on
+  // 4136: 84, 56, 41, 34 us in 1, 2, 4 and 9; 300 on 400: 26 us, 29 in two; 72B, 64 on
+  // 1436: 39, 35, 30 in 1, 2 and 4.)
+  auto splits = [&](int i, int n) {  // of run i, where the longest has n
+    const int per = (longest + n - 1) / n, tiles = (r[i + 1].key0 - r[i].key0) / BK;
+    return (tiles + per - 1) / per;
+  };
+  double best = longest;
   s.nsplit = 1;
-  for (int n = 2; n <= most; ++n) {
-    const double t = (double)((tiles + n - 1) / n) + 3.5 +
-                     (double)a.T * a.n_q_heads * n * (D + 2) * 8 / 4e6;
+  for (int n = 2; n <= std::min(longest, kMaxSplits); ++n) {
+    long long ctas = 0;
+    for (int i = 0; i < a.n; ++i)
+      ctas += (long long)(r[i + 1].tile0 - r[i].tile0) * Hkv * splits(i, n);
+    if (ctas > 148) break;
+    const double t = (double)((longest + n - 1) / n) + 3.5 + (double)rows * n * (D + 2) * 8 / 4e6;
     if (t < best) {
       best = t;
       s.nsplit = n;
     }
   }
-  s.bytes = s.part + (s.nsplit > 1 ? (size_t)a.T * a.n_q_heads * s.nsplit * (D + 2) * 4 : 0);
+  for (int i = 0; i < a.n; ++i) r[i].nsplit = s.nsplit > 1 ? splits(i, s.nsplit) : 1;
+  s.bytes = s.part + (s.nsplit > 1 ? rows * s.nsplit * (D + 2) * 4 : 0);
   return s;
 }
 
@@ -918,26 +976,25 @@ template <int D>
 cudaError_t launch(const Kv4PromptArgs &a, char *base, const Scratch &sc, cudaStream_t s) {
   using S = Shape<D>;
   const int Hkv = a.kv.n_kv_heads, Hq = a.n_q_heads, G = Hq / Hkv, TQ = ROWS / G;
-  const int L = a.prefix + a.T, Lp = (L + BK - 1) / BK * BK;
+  const int Lp = sc.Lp;
   __half *qh = reinterpret_cast<__half *>(base + sc.qh), *ql = reinterpret_cast<__half *>(base + sc.ql);
   __half *kh = reinterpret_cast<__half *>(base + sc.kh), *kl = reinterpret_cast<__half *>(base + sc.kl);
   __half *vh = reinterpret_cast<__half *>(base + sc.vh), *vl = reinterpret_cast<__half *>(base + sc.vl);
   int *bits = reinterpret_cast<int *>(base + sc.bits);
   float *rowf = reinterpret_cast<float *>(base + sc.rowf);
   const float scale = 1.4426950408889634f / sqrtf((float)D);
-  const int rows = a.T * Hq;
-  uint2 *part = reinterpret_cast<uint2 *>(base + sc.pieces);
-  const int pieces = (L + 255) / 256;
-  cudaError_t e = launch_pdl(k_kv4_absmax<D>, dim3(pieces, Hkv), dim3(256), 0, s, a.kv, a.seq, L,
+  const int rows = sc.T * Hq;
+  uint2 *part = reinterpret_cast<uint2 *>(base + sc.part_max);
+  cudaError_t e = launch_pdl(k_kv4_absmax<D>, dim3(sc.pieces, Hkv), dim3(256), 0, s, a.kv, sc.run,
                              part);
   if (e != cudaSuccess) return e;
-  SplitArgs sa{a.kv, a.seq, L, Lp, pieces, rows, scale, a.q, part, bits, qh, ql, kh, kl, vh, vl, rowf,
-               a.err};
+  SplitArgs sa{a.kv, sc.run, Hq, Lp, sc.pieces, rows, scale, a.q, part, bits, qh, ql, kh, kl, vh, vl,
+               rowf, a.err};
   e = launch_pdl(k_split<D>, dim3(Lp / BK * Hkv + (rows + kQRows - 1) / kQRows), dim3(256), 0, s, sa);
   if (e != cudaSuccess) return e;
 
   CUtensorMap mQh, mQl, mKh, mKl, mVh, mVl;
-  cuuint64_t dQ[3] = {(cuuint64_t)D, (cuuint64_t)Hq, (cuuint64_t)a.T};
+  cuuint64_t dQ[3] = {(cuuint64_t)D, (cuuint64_t)Hq, (cuuint64_t)sc.T};
   cuuint64_t sQ[2] = {(cuuint64_t)D * 2, (cuuint64_t)Hq * D * 2};
   cuuint32_t bQ[3] = {64, (cuuint32_t)G, (cuuint32_t)TQ};
   cuuint64_t dK[2] = {(cuuint64_t)D, (cuuint64_t)Hkv * Lp};
@@ -953,8 +1010,8 @@ cudaError_t launch(const Kv4PromptArgs &a, char *base, const Scratch &sc, cudaSt
       !tma_encode(&mVh, F16, 2, vh, dV, sV, bV, SW) || !tma_encode(&mVl, F16, 2, vl, dV, sV, bV, SW))
     return cudaErrorInvalidValue;
   Params p{};
-  p.T = a.T; p.Hq = Hq; p.G = G; p.TQ = TQ; p.prefix = a.prefix; p.Lp = Lp;
-  p.ntiles_rows = (a.T + TQ - 1) / TQ; p.nsplit = sc.nsplit; p.out = a.out;
+  p.run = sc.run;
+  p.T = sc.T; p.Hq = Hq; p.G = G; p.TQ = TQ; p.Lp = Lp; p.nsplit = sc.nsplit; p.out = a.out;
   p.part = reinterpret_cast<float *>(base + sc.part);
   p.err = a.err; p.rowf = rowf; p.bits = bits;
   e = cudaFuncSetAttribute(k_attn_kv4_tc<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
@@ -965,7 +1022,7 @@ cudaError_t launch(const Kv4PromptArgs &a, char *base, const Scratch &sc, cudaSt
     return cudaFuncGetAttributes(&fa, k_attn_kv4_tc<D>) == cudaSuccess ? fa.numRegs : 0;
   }();
   if (regs < kRegs) return cudaErrorInvalidConfiguration;
-  e = launch_pdl(k_attn_kv4_tc<D>, dim3(p.ntiles_rows, Hkv, p.nsplit), dim3(THREADS), S::SMEM, s, mQh,
+  e = launch_pdl(k_attn_kv4_tc<D>, dim3(sc.tiles, Hkv, p.nsplit), dim3(THREADS), S::SMEM, s, mQh,
                  mQl, mKh, mKl, mVh, mVl, p);
   if (e != cudaSuccess || p.nsplit == 1) return e;
   return launch_pdl(k_kv4_tc_combine<D>, dim3((rows + 7) / 8), dim3(256), 0, s, p);
@@ -977,7 +1034,7 @@ size_t kv4_prompt_scratch_bytes(const Kv4PromptArgs &a) { return k4tc::carve(a).
 
 cudaError_t launch_attention_kv4_prompt(const Kv4PromptArgs &a, void *scratch, size_t scratch_bytes,
                                         cudaStream_t s) {
-  if (a.T <= 0) return cudaSuccess;
+  if (a.n <= 0) return cudaSuccess;
   const k4tc::Scratch sc = k4tc::carve(a);
   if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 255) || scratch_bytes < sc.bytes ||
       !tma_encode_fn() || a.n_q_heads / a.kv.n_kv_heads > 8)

@@ -1106,18 +1106,20 @@ static const si::Kv4Run *as_runs(const si_kv4_run *r) {
   return reinterpret_cast<const si::Kv4Run *>(r);
 }
 
-// Whether a run's attention goes through the prompt kernel.  That costs some 20 us
-// a run before it starts (its operands are made first, over all keys) and then a
-// fifth of what the decode kernel takes per token and key; measured at 16 to 128
-// tokens on 500 to 8000 positions, the two meet near (tokens - 8) * keys * KV heads =
-// 330,000 at head_dim 128 (7B, 2000 positions: 32 tokens 18 against 27 us, 64 34
-// against 29 us; 72B, 2000: 16 tokens 18 against 27 us, 32 34 against 28 us), a
-// half more at 64, whose decode tiles take two thirds of the time (0.5B, 2000: 64
-// tokens 13 against 20 us, 128 24.5 against 23.7 us).
-static bool kv4_prompt_run(const si_kv4 *kv, const si_kv4_run &r) {
-  if (r.pos < 0 || r.count < 16) return false;
-  const double keys = r.pos + 0.5 * r.count;
-  return (r.count - 8) * keys * kv->d.n_kv_heads * (kv->d.head_dim + 64) / 192 >= 3.3e5;
+// Whether the runs of 16 tokens and more go through the prompt kernel, together.
+// That costs some 20 us before it starts (its operands are made first, over all
+// keys) and then a fifth of what the decode kernel takes per token and key; measured
+// on one run of 16 to 128 tokens on 500 to 8000 positions, the two meet near
+// (tokens - 8) * keys * KV heads = 330,000 at head_dim 128 (7B, 2000 positions: 32
+// tokens 18 against 27 us, 64 34 against 29 us; 72B, 2000: 16 tokens 18 against 27 us,
+// 32 34 against 28 us), a half more at 64, whose decode tiles take two thirds of the
+// time (0.5B, 2000: 64 tokens 13 against 20 us, 128 24.5 against 23.7 us).
+static bool kv4_prompt_run(const si_kv4_run &r) { return r.pos >= 0 && r.count >= 16; }
+static bool kv4_prompts_pay(const si_kv4 *kv, const si_kv4_run *runs, int n) {
+  double work = 0;
+  for (int i = 0; i < n; ++i)
+    if (kv4_prompt_run(runs[i])) work += (runs[i].count - 8) * (runs[i].pos + 0.5 * runs[i].count);
+  return work * kv->d.n_kv_heads * (kv->d.head_dim + 64) / 192 >= 3.3e5;
 }
 
 extern "C" SI_API size_t si_kv4_page_bytes(const si_dims *d, int page_len) {
@@ -1511,6 +1513,31 @@ static si_status kv4_rope_append(si_ctx *ctx, si_kv4 *kv, const si_dims &d, cons
   });
 }
 
+// Prompts through their kernel, as many in a launch as fit kKv4MaxPrompts and half a
+// gigabyte of operands (one at least), the longest first: its CTAs start first.
+static si_status kv4_prompts(si_ctx *ctx, si::Kv4PromptArgs &pa, std::vector<si::Kv4Prompt> &runs) {
+  constexpr size_t kBytes = (size_t)512 << 20;
+  std::sort(runs.begin(), runs.end(), [](const si::Kv4Prompt &a, const si::Kv4Prompt &b) {
+    return (int64_t)a.prefix + a.T != (int64_t)b.prefix + b.T ? a.prefix + a.T > b.prefix + b.T
+                                                               : a.row < b.row;
+  });
+  for (size_t i = 0; i < runs.size();) {
+    size_t bytes = 0;
+    for (pa.n = 0; pa.n < si::kKv4MaxPrompts && i < runs.size(); ++i) {
+      pa.run[pa.n++] = runs[i];
+      const size_t need = si::kv4_prompt_scratch_bytes(pa);
+      if (pa.n > 1 && need > kBytes) {
+        --pa.n;
+        break;
+      }
+      bytes = need;
+    }
+    SI_TRY(ctx->attn.reserve(bytes));
+    SI_CUDA(si::launch_attention_kv4_prompt(pa, ctx->attn.p, ctx->attn.bytes, ctx->stream));
+  }
+  return SI_OK;
+}
+
 // The attention of a list of runs (checked by the caller), or with tok_ctx of
 // token t at position tok_ctx[t] - 1 of sequence t.
 static si_status kv4_attend(si_ctx *ctx, si_kv4 *kv, int n_q_heads, const float *q,
@@ -1534,13 +1561,19 @@ static si_status kv4_attend(si_ctx *ctx, si_kv4 *kv, int n_q_heads, const float 
   }
   const std::vector<int> rows = kv4_rows(runs, n);
   // Decode tokens, short and early prompts: one token at a time.
+  const bool tiles = kv4_prompts_pay(kv, runs, n);
   std::vector<si_kv4_run> few;
   std::vector<int> few_rows;
-  for (int i = 0; i < n; ++i)
-    if (runs[i].count > 0 && !kv4_prompt_run(kv, runs[i])) {
+  std::vector<si::Kv4Prompt> prompts;
+  for (int i = 0; i < n; ++i) {
+    if (runs[i].count <= 0) continue;
+    if (tiles && kv4_prompt_run(runs[i])) {
+      prompts.push_back({runs[i].seq, runs[i].pos, runs[i].count, rows[i]});
+    } else {
       few.push_back(runs[i]);
       few_rows.push_back(rows[i]);
     }
+  }
   SI_TRY(kv4_pieces(
       few.data(), few_rows.data(), (int)few.size(),
       [&](const si::Kv4Runs &p, int tokens) -> si_status {
@@ -1552,41 +1585,35 @@ static si_status kv4_attend(si_ctx *ctx, si_kv4 *kv, int n_q_heads, const float 
         SI_CUDA(si::launch_attention_kv4(a, ctx->stream));
         return SI_OK;
       }));
-  for (int i = 0; i < n; ++i) {
-    if (!kv4_prompt_run(kv, runs[i])) continue;
-    if (!ctx->exact_attention) {
-      si::Kv4PromptArgs pa{};
-      pa.kv = a.kv;
-      pa.seq = runs[i].seq;
-      pa.prefix = runs[i].pos;
-      pa.T = runs[i].count;
-      pa.n_q_heads = n_q_heads;
-      pa.q = q + rows[i] * row;
-      pa.out = out + rows[i] * row;
-      pa.err = ctx->err;
-      SI_TRY(ctx->attn.reserve(si::kv4_prompt_scratch_bytes(pa)));
-      SI_CUDA(si::launch_attention_kv4_prompt(pa, ctx->attn.p, ctx->attn.bytes, ctx->stream));
-      continue;
-    }
+  if (!ctx->exact_attention) {
+    si::Kv4PromptArgs pa{};
+    pa.kv = a.kv;
+    pa.n_q_heads = n_q_heads;
+    pa.q = q;
+    pa.out = out;
+    pa.err = ctx->err;
+    return kv4_prompts(ctx, pa, prompts);
+  }
+  for (const si::Kv4Prompt &x : prompts) {
     // The fp32 kernel over the run's keys unpacked to an fp32 cache.
-    const int L = runs[i].pos + runs[i].count;
+    const int L = x.prefix + x.T;
     const size_t kvd = (size_t)kv->d.n_kv_heads * D;
     SI_TRY(ctx->kv4.reserve(2 * L * kvd * sizeof(float)));
     float *kf = static_cast<float *>(ctx->kv4.p), *vf = kf + L * kvd;
-    const si_kv4_run all{runs[i].seq, 0, L};
+    const si_kv4_run all{x.seq, 0, L};
     SI_TRY(kv4_read(ctx, kv, &all, 1, kf, vf));
     si::AttnArgs aa{};
-    aa.q = q + rows[i] * row;
+    aa.q = q + x.row * row;
     aa.kc = kf;
     aa.vc = vf;
     aa.kv_f32 = 1;
-    aa.T = runs[i].count;
+    aa.T = x.T;
     aa.n_q_heads = n_q_heads;
     aa.n_kv_heads = kv->d.n_kv_heads;
     aa.head_dim = D;
     aa.max_ctx = L;
-    aa.ctx0 = runs[i].pos + 1;
-    aa.out = out + rows[i] * row;
+    aa.ctx0 = x.prefix + 1;
+    aa.out = out + x.row * row;
     aa.err = ctx->err;
     aa.nsplit = 1;
     SI_CUDA(si::launch_attention(aa, ctx->stream));

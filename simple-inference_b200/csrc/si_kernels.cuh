@@ -289,13 +289,18 @@ struct Kv4AttnArgs {
 void kv4_pick_splits(Kv4AttnArgs &a);
 size_t kv4_part_floats(const Kv4AttnArgs &a);
 cudaError_t launch_attention_kv4(const Kv4AttnArgs &a, cudaStream_t s);
-// A run of T consecutive tokens of sequence seq from position prefix on, on the
-// tensor cores (attention_kv4_tc.cu).
+// Runs of consecutive tokens on the tensor cores (attention_kv4_tc.cu): run i is T
+// tokens of sequence seq from position prefix on, rows row, row + 1, ... of q and out.
+constexpr int kKv4MaxPrompts = 8;
+struct Kv4Prompt {
+  int seq, prefix, T, row;
+};
 struct Kv4PromptArgs {
   Kv4View kv;
-  int seq, prefix, T, n_q_heads;
-  const float *q;  // [T][Hq][D], 16-byte aligned
-  float *out;      // [T][Hq][D], 16-byte aligned
+  int n, n_q_heads;
+  Kv4Prompt run[kKv4MaxPrompts];
+  const float *q;  // [.][Hq][D], 16-byte aligned
+  float *out;      // [.][Hq][D], 16-byte aligned
   int *err;
 };
 size_t kv4_prompt_scratch_bytes(const Kv4PromptArgs &a);

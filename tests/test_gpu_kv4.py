@@ -383,6 +383,44 @@ def test_mixed_batch_of_prompts_and_tokens(si_ctx):
     c.kv.free()
 
 
+@pytest.mark.parametrize("heads", [(12, 2, 128), (14, 2, 64), (3, 3, 128)])
+def test_many_prompts_in_one_call(si_ctx, heads):
+    """More prompts than one launch takes, of odd lengths, several of one sequence,
+    between single tokens; a NaN in one sequence stays in its own rows."""
+    c = Cache(si_ctx, heads, 12, 1000, 48, seed=26)
+    lens = [900, 64, 333, 1000, 17, 640, 512, 129, 777, 48, 801, 96]
+    c.shuffle(lens)
+    c.random([(s, 0, n) for s, n in enumerate(lens)])
+    bad = np.full((1, heads[1], heads[2]), np.nan, np.float32)
+    c.append([(6, 0, 1)], bad, bad)
+    runs = []
+    for s, n in enumerate(lens):
+        for count in (16 + 7 * s, 16 + s, 1):
+            if count <= n:
+                runs.append((s, n - count, count))
+    runs += [(3, 500, 131), (0, 0, 64), (0, 0, 16)]
+    assert sum(r[2] >= 16 for r in runs) > 16
+    q = c.rng.standard_normal((sum(r[2] for r in runs), heads[0], heads[2]))
+    got = c.attend(q, runs)
+    at, good = 0, np.ones(len(q), bool)
+    for s, p, count in runs:
+        good[at:at + count] = s != 6
+        at += count
+    assert np.isnan(got[~good]).all()
+    c.check(got[good], q[good], [r for r in runs if r[0] != 6], every=11)
+    c.kv.free()
+
+
+def test_prompts_with_too_many_keys_for_one_launch(si_ctx):
+    """Operands of three prompts that would take a gigabyte together."""
+    c = Cache(si_ctx, (8, 8, 128), 1, 40000, 128, seed=27)
+    c.random([(0, 0, 40000)])
+    runs = [(0, 33000, 16), (0, 39980, 20), (0, 100, 40), (0, 36000, 17)]
+    q = c.rng.standard_normal((sum(r[2] for r in runs), 8, 128))
+    c.check(c.attend(q, runs), q, runs, every=50)
+    c.kv.free()
+
+
 # ------------------------------------------------------------------- pages --
 def test_fork_write_and_compact(si_ctx):
     c = Cache(si_ctx, (12, 2, 128), 4, 200, 32, seed=11, spare=10)
