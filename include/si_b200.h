@@ -522,7 +522,7 @@ SI_API si_status si_kv4_read_dev(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs
 /* Attention of queries q [T][Hq][D] (RoPE applied; 16-byte aligned, as out)
  * over the cache: the token at position p attends positions 0 .. p of its
  * sequence, whose pages must cover it.  A run at pos -1 begins with a token
- * that attends nothing; its row of out is zeros (padding of a batch).  Runs of 16
+ * that attends nothing; its row of out is zeros (padding of a batch).  Runs of 13
  * tokens and more, where they have enough work together, go through a prompt kernel
  * on the tensor cores (with si_ctx_set_exact_attention the fp32 one over their keys
  * unpacked), the others read the packed cache token by token.  fp32 in and out, within about 1e-6 of

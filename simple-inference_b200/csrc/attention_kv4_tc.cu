@@ -49,7 +49,7 @@
 // 4 KB with P from TMEM; a pair of tiles takes about 3900 cycles, 3100 of them MMAs.
 // 72B heads, 509 tokens on 7680 positions: P through shared memory and one issuing
 // warp 417 us, P from TMEM 362, windows taken at the next pair 337, keys a third
-// ahead 322, operands by packed arithmetic 305 (three MMAs a product: 430 TFLOP/s are
+// ahead 322, operands by packed arithmetic 305, now 302 (three MMAs a product: 430 TFLOP/s are
 // 1290); 7B, a prompt of 2048: 101.
 #include <algorithm>
 

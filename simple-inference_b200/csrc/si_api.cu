@@ -1106,15 +1106,17 @@ static const si::Kv4Run *as_runs(const si_kv4_run *r) {
   return reinterpret_cast<const si::Kv4Run *>(r);
 }
 
-// Whether the runs of 16 tokens and more go through the prompt kernel, together.
+// Whether the runs of 13 tokens and more go through the prompt kernel, together.
 // That costs some 20 us before it starts (its operands are made first, over all
 // keys) and then a fifth of what the decode kernel takes per token and key; measured
 // on one run of 16 to 128 tokens on 500 to 8000 positions, the two meet near
 // (tokens - 8) * keys * KV heads = 330,000 at head_dim 128 (7B, 2000 positions: 32
 // tokens 18 against 27 us, 64 34 against 29 us; 72B, 2000: 16 tokens 18 against 27 us,
 // 32 34 against 28 us), a half more at 64, whose decode tiles take two thirds of the
-// time (0.5B, 2000: 64 tokens 13 against 20 us, 128 24.5 against 23.7 us).
-static bool kv4_prompt_run(const si_kv4_run &r) { return r.pos >= 0 && r.count >= 16; }
+// time (0.5B, 2000: 64 tokens 13 against 20 us, 128 24.5 against 23.7 us).  Runs of
+// fewer tokens fill too little of a row tile, however many they are (7B, 2000
+// positions: 16 runs of 8 53 against 74 us, of 12 73 against 76, 8 of 15 52 against 39).
+static bool kv4_prompt_run(const si_kv4_run &r) { return r.pos >= 0 && r.count >= 13; }
 static bool kv4_prompts_pay(const si_kv4 *kv, const si_kv4_run *runs, int n) {
   double work = 0;
   for (int i = 0; i < n; ++i)

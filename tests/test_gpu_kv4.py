@@ -398,7 +398,7 @@ def test_many_prompts_in_one_call(si_ctx, heads):
         for count in (16 + 7 * s, 16 + s, 1):
             if count <= n:
                 runs.append((s, n - count, count))
-    runs += [(3, 500, 131), (0, 0, 64), (0, 0, 16)]
+    runs += [(3, 500, 131), (0, 0, 64), (0, 0, 16), (8, 700, 13), (10, 5, 14), (8, 600, 12)]
     assert sum(r[2] >= 16 for r in runs) > 16
     q = c.rng.standard_normal((sum(r[2] for r in runs), heads[0], heads[2]))
     got = c.attend(q, runs)
