@@ -392,9 +392,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int *bits = p.bits + 2 * ((int)(&run - p.run.r) * (int)gridDim.y + g);
     const int kshift = operand_shift(bits[0]), vshift = operand_shift(bits[1]);
     // (kept above zero: a masked score times it stays -inf)
-    const float rf =
-        valid ? fmaxf(ldexpf(p.rowf[(size_t)(run.tok0 + tok) * p.Hq + (size_t)g * p.G + hh], -kshift), 1.2e-38f)
-              : 0.0f;
+    const size_t frow = (size_t)(run.tok0 + tok) * p.Hq + (size_t)g * p.G + hh;
+    const float rf = valid ? fmaxf(ldexpf(p.rowf[frow], -kshift), 1.2e-38f) : 0.0f;
     const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16);
     constexpr int H = D / 2;   // this group keeps dims [grp * H, grp * H + H) of the sums
     const uint32_t t_o = t_row + S::COL_O + grp * H, t_ol = t_row + S::COL_OL + grp * H;

@@ -17,6 +17,8 @@
 // dims 32b + 4g .. 32b + 4g + 3 is half-word g * (D/32) + b, so that the 2*D/32
 // bytes of one g hold the same four dims of every block -- what one lane of a
 // matrix instruction's operand takes, in one load.
+#include <type_traits>
+
 #include "si_common.cuh"
 #include "si_kernels.cuh"
 
@@ -111,19 +113,19 @@ __device__ __forceinline__ void kv4_store_rows(const float4 (&x)[N], int j, int 
 // latency of the loads and the warps that an SM holds: rows written and read back,
 // 4099 tokens of 72B, 28 us with four warps of four rows, 31 with two rows each or
 // in eight warps, 30 with two warps of eight, 35 with a whole token per warp (their
-// bytes alone would take 12).  With tables the K rows and queries are rotated first
-// (rope_kv.cu's arithmetic).  A position without a page, or whose page other
+// bytes alone would take 12).  In a layer step (STEP) the K rows and queries are
+// rotated first (rope_kv.cu's arithmetic).  A position without a page, or whose page other
 // sequences hold too, is not written and recorded as SI_ERR_INVALID.
 constexpr int kWarps = 4, kRows = 4, kUnits = kWarps * kRows;
 
-template <int D, bool VEC>
+template <int D, bool VEC, bool STEP>
 __global__ void __launch_bounds__(32 * kWarps) k_kv4_append(const __grid_constant__ Kv4AppendArgs a) {
   pdl_trigger();
   pdl_wait();
   constexpr int HALF = D / 2, LPR = D / 4, RPW = 32 / LPR;  // lanes per row, rows per warp
   constexpr int N = kRows / RPW;
   const int t = blockIdx.x, lane = threadIdx.x & 31, j = lane % LPR;
-  const int nq = a.q_out ? a.n_q_heads : 0, Hkv = a.kv.n_kv_heads, units = nq + 2 * Hkv;
+  const int nq = STEP ? a.n_q_heads : 0, Hkv = a.kv.n_kv_heads, units = nq + 2 * Hkv;
   int seq, pos, row = t;
   if (a.tok_ctx) {
     seq = t;
@@ -135,16 +137,16 @@ __global__ void __launch_bounds__(32 * kWarps) k_kv4_append(const __grid_constan
     pos = a.runs.pos[r] + row - a.runs.row0[r];
   }
   const int u0 = blockIdx.y * kUnits + (threadIdx.x >> 5) * (N * RPW) + lane / LPR;
-  const float *qr = nq ? a.q + (size_t)row * a.ldq + 4 * j : nullptr;
-  const float *kr = a.k + (size_t)row * a.ldkv + 4 * j, *vr = a.v + (size_t)row * a.ldkv + 4 * j;
+  const size_t qat = STEP ? (size_t)row * a.ldq + 4 * j : 0, at = (size_t)row * a.ldkv + 4 * j;
   float4 x[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const int u = u0 + k * RPW;
     x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (u < units) {
-      const float *src = u < nq ? qr + u * D : u < nq + Hkv ? kr + (u - nq) * D
-                                                            : vr + (u - nq - Hkv) * D;
+      const bool is_q = STEP && u < nq, is_v = u >= nq + Hkv;
+      const float *src = (is_q ? a.q : is_v ? a.v : a.k) + (is_q ? qat : at) +
+                         (is_q ? u : is_v ? u - nq - Hkv : u - nq) * D;
       if constexpr (VEC) x[k] = *reinterpret_cast<const float4 *>(src);
       else x[k] = make_float4(src[0], src[1], src[2], src[3]);
     }
@@ -153,25 +155,20 @@ __global__ void __launch_bounds__(32 * kWarps) k_kv4_append(const __grid_constan
   uint8_t *grp = kv4_group(a.kv, seq, pos, &page);
   if (grp && a.kv.refs[page] != 1) grp = nullptr;
   if (!grp && threadIdx.x == 0 && blockIdx.y == 0) raise_error(a.err, 1);
-  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (a.cos_tab) {
+  if constexpr (STEP) {
     if (pos < 0 || pos >= a.max_positions) return;  // never read outside the tables
     const int i = (4 * j) % HALF;
-    c = *reinterpret_cast<const float4 *>(a.cos_tab + (size_t)pos * HALF + i);
-    s = *reinterpret_cast<const float4 *>(a.sin_tab + (size_t)pos * HALF + i);
-  }
-  const size_t head_bytes = (size_t)a.kv.gpp * kv4_group_bytes(D);
+    const float4 c = *reinterpret_cast<const float4 *>(a.cos_tab + (size_t)pos * HALF + i);
+    const float4 s = *reinterpret_cast<const float4 *>(a.sin_tab + (size_t)pos * HALF + i);
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int u = u0 + k * RPW;
-    const bool is_v = u >= nq + Hkv;
-    if (a.cos_tab) {
+    for (int k = 0; k < N; ++k) {
+      const int u = u0 + k * RPW;
       float4 y;  // the other half of the pair
       y.x = __shfl_xor_sync(0xffffffffu, x[k].x, LPR / 2);
       y.y = __shfl_xor_sync(0xffffffffu, x[k].y, LPR / 2);
       y.z = __shfl_xor_sync(0xffffffffu, x[k].z, LPR / 2);
       y.w = __shfl_xor_sync(0xffffffffu, x[k].w, LPR / 2);
-      if (!is_v) {
+      if (u < nq + Hkv) {
         auto rot = [&](float own, float other, float c, float s) {
           return j < LPR / 2 ? __fsub_rn(__fmul_rn(own, c), __fmul_rn(other, s))
                              : __fadd_rn(__fmul_rn(own, c), __fmul_rn(other, s));
@@ -179,15 +176,16 @@ __global__ void __launch_bounds__(32 * kWarps) k_kv4_append(const __grid_constan
         x[k] = make_float4(rot(x[k].x, y.x, c.x, s.x), rot(x[k].y, y.y, c.y, s.y),
                            rot(x[k].z, y.z, c.z, s.z), rot(x[k].w, y.w, c.w, s.w));
       }
+      if (u < nq)
+        *reinterpret_cast<float4 *>(a.q_out + ((size_t)row * a.n_q_heads + u) * D + 4 * j) = x[k];
     }
-    if (u < nq)
-      *reinterpret_cast<float4 *>(a.q_out + ((size_t)row * a.n_q_heads + u) * D + 4 * j) = x[k];
+    if (!__any_sync(0xffffffffu, u0 + (N - 1) * RPW >= nq)) return;  // queries alone
   }
-  if (!__any_sync(0xffffffffu, u0 + (N - 1) * RPW >= nq)) return;  // queries alone
+  const uint32_t head_bytes = (uint32_t)a.kv.gpp * kv4_group_bytes(D);  // below 2^20
   kv4_store_rows<D, N>(x, j, pos & 15, [&](int k) -> uint8_t * {
     const int h = u0 + k * RPW - nq;
     if (!grp || h < 0 || h >= 2 * Hkv) return nullptr;
-    return h < Hkv ? grp + h * head_bytes : grp + (h - Hkv) * head_bytes + kv4_group_bytes(D) / 2;
+    return grp + (h < Hkv ? h * head_bytes : (h - Hkv) * head_bytes + kv4_group_bytes(D) / 2);
   });
 }
 
@@ -209,7 +207,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_kv4_read(const __grid_constant_
   int page;
   const uint8_t *grp = kv4_group(a.kv, a.runs.seq[r], pos, &page);
   if (!grp && threadIdx.x == 0 && blockIdx.y == 0) raise_error(a.err, 1);
-  const size_t head_bytes = (size_t)a.kv.gpp * kv4_group_bytes(D);
+  const uint32_t head_bytes = (uint32_t)a.kv.gpp * kv4_group_bytes(D);
   const int r16 = pos & 15, b = j >> 3, g = j & 7;
   const int u0 = blockIdx.y * kUnits + (threadIdx.x >> 5) * (N * RPW) + lane / LPR;
   uint32_t w[N];
@@ -221,7 +219,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_kv4_read(const __grid_constant_
     sc[k] = 0.0f;
     if (grp && u < 2 * Hkv) {
       const uint8_t *p =
-          u < Hkv ? grp + u * head_bytes : grp + (u - Hkv) * head_bytes + kv4_group_bytes(D) / 2;
+          grp + (u < Hkv ? u * head_bytes : (u - Hkv) * head_bytes + kv4_group_bytes(D) / 2);
       w[k] = reinterpret_cast<const uint16_t *>(p + r16 * (D / 2))[g * NB + b];
       sc[k] = f16_to_f32(reinterpret_cast<const uint16_t *>(p + kKv4Group * (D / 2))[r16 * NB + b]);
     }
@@ -299,8 +297,13 @@ cudaError_t launch_kv4_append(const Kv4AppendArgs &a, cudaStream_t s) {
   const dim3 grid(a.T, (units + kUnits - 1) / kUnits);
   const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
             reinterpret_cast<uintptr_t>(a.v) | 4 * a.ldq | 4 * a.ldkv) & 15) == 0;
-  auto *kern = a.kv.head_dim == 128 ? (vec ? k_kv4_append<128, true> : k_kv4_append<128, false>)
-                                    : (vec ? k_kv4_append<64, true> : k_kv4_append<64, false>);
+  auto pick = [&](auto d, auto step) {
+    return vec ? k_kv4_append<d.value, true, step.value> : k_kv4_append<d.value, false, step.value>;
+  };
+  const std::integral_constant<int, 64> d64;
+  const std::integral_constant<int, 128> d128;
+  auto *kern = a.kv.head_dim == 128 ? (a.q_out ? pick(d128, std::true_type()) : pick(d128, std::false_type()))
+                                    : (a.q_out ? pick(d64, std::true_type()) : pick(d64, std::false_type()));
   return launch_pdl(kern, grid, dim3(32 * kWarps), 0, s, a);
 }
 
