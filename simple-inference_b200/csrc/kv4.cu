@@ -61,8 +61,8 @@ __device__ __forceinline__ float larger(float first, float later) {
 // rows at once.  The N rows of a lane are quantised together: the eight lanes of a
 // block halve the rows they hold at each exchange, so that lane g ends with the
 // extreme of row g % N, divides once and stores one scale (one row after the
-// other, with everything in every lane: 19 us for 4099 tokens of 72B; together
-// 17).  Row k is row r16 of the half-group dst(k), null for one that is not stored.
+// other, with everything in every lane: 2.5 us more of 17 for 4099 tokens of 72B).
+// Row k is row r16 of the half-group dst(k), null for one that is not stored.
 template <int D, int N, typename Dst>
 __device__ __forceinline__ void kv4_store_rows(const float4 (&x)[N], int j, int r16, Dst dst) {
   static_assert(N == 2 || N == 4, "rows of a lane");
@@ -111,9 +111,9 @@ __device__ __forceinline__ void kv4_store_rows(const float4 (&x)[N], int j, int 
 // (rotated into q_out; none without q_out), then the K rows, then the V rows of
 // the token; a warp loads its kRows units before it works on them.  Bound by the
 // latency of the loads and the warps that an SM holds: rows written and read back,
-// 4099 tokens of 72B, 28 us with four warps of four rows, 31 with two rows each or
-// in eight warps, 30 with two warps of eight, 35 with a whole token per warp (their
-// bytes alone would take 12).  In a layer step (STEP) the K rows and queries are
+// 4099 tokens of 72B, 24 us with four warps of four rows, 27 with two rows each, 31
+// in eight warps, 29 with eight rows each, 24 in two warps of eight (their bytes alone
+// would take 12).  In a layer step (STEP) the K rows and queries are
 // rotated first (rope_kv.cu's arithmetic).  A position without a page, or whose page other
 // sequences hold too, is not written and recorded as SI_ERR_INVALID.
 constexpr int kWarps = 4, kRows = 4, kUnits = kWarps * kRows;
