@@ -575,10 +575,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
       if (c == 0) cta_ml[h] = make_float2(M, L);
     } else {
       const size_t slot = ((size_t)blockIdx.z * a.n_q_heads + head) * a.nsplit + split;
-      float2 *pml = reinterpret_cast<float2 *>(a.part);
-      float *po = a.part + (size_t)gridDim.z * a.n_q_heads * a.nsplit * 2;
-      if (c == 0) pml[slot] = make_float2(M, L);
-      *reinterpret_cast<float4 *>(po + slot * D + 4 * c) = o;
+      const size_t slots = (size_t)gridDim.z * a.n_q_heads * a.nsplit;
+      if (c == 0)
+        *reinterpret_cast<float2 *>(a.part + kv4_part_ml(slots, slot, D)) = make_float2(M, L);
+      *reinterpret_cast<float4 *>(a.part + kv4_part_out(slot, D) + 4 * c) = o;
     }
   }
   if (ns == 1 || !a.cluster) return;
@@ -630,8 +630,9 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
   const int ns = tk.len > 0 ? (tk.len + per - 1) / per : 1;
   if (ns == 1) return;  // already written
   const size_t slot = ((size_t)blockIdx.y * a.n_q_heads + blockIdx.x) * a.nsplit;
-  const float2 *ml = reinterpret_cast<const float2 *>(a.part) + slot;
-  const float *po = a.part + (size_t)gridDim.y * a.n_q_heads * a.nsplit * 2 + slot * D;
+  const size_t slots = (size_t)gridDim.y * a.n_q_heads * a.nsplit;
+  const float2 *ml = reinterpret_cast<const float2 *>(a.part + kv4_part_ml(slots, slot, D));
+  const float *po = a.part + kv4_part_out(slot, D);
   const int grp = threadIdx.x / LPR, c = threadIdx.x % LPR;
   float M = -INFINITY;
   for (int i = threadIdx.x; i < ns; i += blockDim.x) M = fmaxf(M, ml[i].x);
@@ -757,7 +758,8 @@ void kv4_pick_splits(Kv4AttnArgs &a) {
 }
 
 size_t kv4_part_floats(const Kv4AttnArgs &a) {
-  return a.nsplit > kMaxCluster ? (size_t)a.T * a.n_q_heads * a.nsplit * (a.kv.head_dim + 2) : 0;
+  return a.nsplit > kMaxCluster
+             ? kv4_part_size((size_t)a.T * a.n_q_heads * a.nsplit, a.kv.head_dim) : 0;
 }
 
 cudaError_t launch_attention_kv4(const Kv4AttnArgs &a, cudaStream_t s) {

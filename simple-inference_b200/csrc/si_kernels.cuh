@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "si_kv4_split.hpp"
+
 namespace si {
 
 // Row-parallel tensor parallelism: where a GEMV's partial sums go instead of

@@ -1,0 +1,58 @@
+"""GPU tests of the 4-bit cache's attention at odd numbers of heads, where the partial
+sums of split keys have an odd number of slots."""
+import numpy as np
+import pytest
+
+import sib200
+from test_gpu_kv4 import Cache
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("heads", [(7, 1, 128), (7, 1, 64), (1, 1, 128), (5, 1, 64), (9, 3, 128)])
+def test_odd_heads_decode_with_many_splits(si_ctx, heads):
+    """Lengths whose split counts lie above eight, odd and even ones, alone and in threes."""
+    lens = [6200, 7000, 8200, 20000]
+    c = Cache(si_ctx, heads, len(lens), 20000, 64, seed=31)
+    c.random([(s, 0, n) for s, n in enumerate(lens)])
+    calls = [[(s, n - 1, 1)] for s, n in enumerate(lens)]
+    calls += [[(0, 6198, 1), (1, 6998, 1), (2, 8000, 1)]]
+    for runs in calls:
+        q = c.rng.standard_normal((len(runs), heads[0], heads[2]))
+        c.check(c.attend(q, runs), q, runs)
+    c.kv.free()
+
+
+@pytest.mark.parametrize("B", [7, 5, 1])
+def test_odd_batch_with_device_lengths(B):
+    """A captured-form step over a long cache (up to 63 splits) against the step with
+    host runs: one flipped Q8 code of the attention output moves a row by about 1 / 127
+    of one input's share, the bar of the other step tests."""
+    D = 128
+    dims = dict(hidden=7 * D, n_q_heads=7, n_kv_heads=1, head_dim=D, intermediate=0,
+                rope_theta=1e6, rms_eps=1e-6)
+    L = 8192
+    ctx = sib200.Context(0, max_positions=L, rope_theta=1e6, head_dim=D)
+    layer = ctx.layer_synth(dims, 33)
+    rng = np.random.default_rng(34)
+    lens = [int(n) for n in rng.integers(1, L - 1, B)]
+    lens[0] = L - 1
+    T = sum(lens)
+    g = torch.Generator("cuda").manual_seed(35)
+    k, v = (torch.randn(T, 1, D, device="cuda", generator=g) for _ in range(2))
+    x = torch.randn(B, 7 * D, device="cuda", generator=g)
+    ya, yb = torch.zeros_like(x), torch.zeros_like(x)
+    torch.cuda.synchronize()
+    kvs = [ctx.kv4(dims, B, L, B * L // 64, 64) for _ in range(2)]
+    for kv in kvs:
+        kv.append(k, v, [(s, 0, n) for s, n in enumerate(lens)])
+    layer.step_dev(kvs[0], x, [(s, n, 1) for s, n in enumerate(lens)], ya)
+    kvs[1].reserve([(s, n, 1) for s, n in enumerate(lens)])
+    st = ctx.decode_state([n + 1 for n in lens], L)
+    layer.decode_state_dev(kvs[1], x, st, yb)
+    ctx.status()
+    a, b = ya.cpu().numpy(), yb.cpu().numpy()
+    for t in range(B):
+        assert np.linalg.norm(a[t] - b[t]) <= 1e-2 * np.linalg.norm(a[t]), (t, lens[t])
+    ctx.close()
