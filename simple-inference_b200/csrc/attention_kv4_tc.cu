@@ -119,7 +119,7 @@ struct Params {
   Runs run;
   int T, Hq, G, TQ, Lp, nsplit;  // tokens, keys and most splits of all runs
   float *out;   // rows [.][Hq][D]
-  float *part;  // with splits: (m, l) [T][Hq][nsplit], then O [T][Hq][nsplit][D]
+  float *part;  // with splits: O [T][Hq][nsplit][D], then (m, l) [T][Hq][nsplit]
   int *err;
   const float *rowf;  // [T][Hq]: with K's power of two takes a row's scores to log2 units
   const int *bits;    // [run][Hkv][2]: largest |scale| of K and V as fp16 bits
@@ -585,8 +585,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         f = l == 0.0f ? 0.0f : back / l;
       } else if (valid) {
         const size_t slot = ((size_t)(run.tok0 + tok) * p.Hq + head) * p.nsplit + blockIdx.z;
-        orow = p.part + (size_t)p.T * p.Hq * p.nsplit * 2 + slot * D;
-        if (grp == 0) reinterpret_cast<float2 *>(p.part)[slot] = make_float2(m, l);
+        orow = p.part + kv4_part_out(slot, D);
+        if (grp == 0)
+          *reinterpret_cast<float2 *>(
+              p.part + kv4_part_ml((size_t)p.T * p.Hq * p.nsplit, slot, D)) = make_float2(m, l);
       }
       take_window(1.0f, f);
       if (valid) {
@@ -624,7 +626,7 @@ __global__ void __launch_bounds__(256) k_kv4_tc_combine(const __grid_constant__ 
   const int ns = (all_kt + per - 1) / per;
   if (ns == 1) return;  // already written
   const size_t slot = (size_t)row * p.nsplit;
-  const float *po = p.part + (size_t)p.T * p.Hq * p.nsplit * 2 + slot * D + lane * N;
+  const float *po = p.part + kv4_part_out(slot, D) + lane * N;
   float v[AHEAD][N], o[N] = {};
   auto load = [&](int i0) {
 #pragma unroll
@@ -642,7 +644,9 @@ __global__ void __launch_bounds__(256) k_kv4_tc_combine(const __grid_constant__ 
   };
   load(0);
   float2 ml = make_float2(-INFINITY, 0.0f);
-  if (lane < ns) ml = reinterpret_cast<const float2 *>(p.part)[slot + lane];
+  if (lane < ns)
+    ml = *reinterpret_cast<const float2 *>(
+        p.part + kv4_part_ml((size_t)p.T * p.Hq * p.nsplit, slot + lane, D));
   float M = ml.x;
 #pragma unroll
   for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
@@ -967,7 +971,7 @@ static Scratch carve(const Kv4PromptArgs &a) {
     }
   }
   for (int i = 0; i < a.n; ++i) r[i].nsplit = s.nsplit > 1 ? splits(i, s.nsplit) : 1;
-  s.bytes = s.part + (s.nsplit > 1 ? rows * s.nsplit * (D + 2) * 4 : 0);
+  s.bytes = s.part + (s.nsplit > 1 ? kv4_part_size(rows * s.nsplit, D) * sizeof(float) : 0);
   return s;
 }
 

@@ -56,3 +56,16 @@ def test_odd_batch_with_device_lengths(B):
     for t in range(B):
         assert np.linalg.norm(a[t] - b[t]) <= 1e-2 * np.linalg.norm(a[t]), (t, lens[t])
     ctx.close()
+
+
+@pytest.mark.parametrize("heads", [(7, 1, 128), (7, 1, 64), (5, 1, 128), (9, 3, 64)])
+@pytest.mark.parametrize("prefix,count", [(2000, 201), (3000, 255), (4000, 129), (1000, 501)])
+def test_odd_heads_prompts_with_splits(si_ctx, heads, prefix, count):
+    """Prompts of few row tiles, whose keys are split, odd in tokens and heads; with a
+    second prompt of another length in the same call."""
+    c = Cache(si_ctx, heads, 2, prefix + count, 48, seed=32)
+    c.random([(0, 0, prefix + count), (1, 0, 331)])
+    for runs in ([(0, prefix, count)], [(1, 200, 131), (0, prefix, count)]):
+        q = c.rng.standard_normal((sum(r[2] for r in runs), heads[0], heads[2]))
+        c.check(c.attend(q, runs), q, runs, every=29)
+    c.kv.free()
