@@ -39,9 +39,9 @@
 // scores of pair n + 1 follow as soon as both groups have read those of pair n, so
 // the tensor pipe has work while the softmax of pair n runs.  The running maximum
 // is handed from tile to tile through shared memory, by a tagged word per row (a
-// barrier's wait took 300 to 800 cycles there); it is only raised by a score more
-// than 2^8 above it.  Every wait is bounded (about 2 s; SI_ERR_TIMEOUT in the
-// context's error word); on expiry every role stops, the CTA's own copies and MMAs
+// barrier's wait took 300 to 800 cycles there); the reference of the probabilities is
+// only raised by a score more than 2^6 above the maximum that set it.  Every wait is
+// bounded (about 2 s; SI_ERR_TIMEOUT in the context's error word); on expiry every role stops, the CTA's own copies and MMAs
 // in flight are waited for (bounded) and TMEM is freed.
 //
 // Bound by the tensor pipe and shared memory together: an MMA of 128 x 128 x 16
@@ -70,7 +70,13 @@ constexpr int THREADS = 384;
 // softmax warps take (the sums match, else the kernel would wait for good).
 constexpr int kRegs = 168, kRegsControl = 56, kRegsSoftmax = 224;
 static_assert(THREADS * kRegs >= 128 * kRegsControl + 256 * kRegsSoftmax, "register split");
-constexpr float kRescaleLog2 = 8.0f;
+// Probabilities are 2^(score - reference), at most 2^kTopLog2; a score above that sets
+// its row's reference kLiftLog2 below itself.  fp16 has no step finer than 2^-24: with
+// the maximum itself as the reference, keys of 2^-17 of the largest one's weight, which
+// together may make the whole output, kept 8 bits (a first key 10 nats above 40000
+// others: 8e-5 of the row, now 2e-6).  A higher lift makes the reference rise more
+// often (11: 7B, a prompt of 2048 tokens 100.7 -> 106.0 us; 7 and 9 cost nothing).
+constexpr float kTopLog2 = 15.0f, kLiftLog2 = 9.0f;
 constexpr int kWindow = 6;  // tiles per window
 constexpr int kMaxSplits = 32;
 
@@ -474,10 +480,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         ok = false;
         break;
       }
-      const bool resc = mt > m + kRescaleLog2;
-      const float alpha = resc ? ex2(m - mt) : 1.0f;  // 0 from no keys yet
+      const bool resc = mt > m + kTopLog2;
+      const float raised = mt - kLiftLog2;
+      const float alpha = resc ? ex2(m - raised) : 1.0f;  // 0 from no keys yet
       const float sync = m != mine ? ex2(mine - m) : 1.0f;  // 0 from no keys yet
-      if (resc) m = mt;
+      if (resc) m = raised;
       m_s[r] = ((unsigned long long)(uint32_t)i << 32) | __float_as_uint(m);
       mine = m;
       l *= sync * alpha;

@@ -1,5 +1,6 @@
-"""GPU tests of the 4-bit cache's attention at odd numbers of heads, where the partial
-sums of split keys have an odd number of slots."""
+"""GPU tests of the 4-bit cache's attention: odd numbers of heads, where the partial
+sums of split keys have an odd number of slots, and scores of which one lies far above
+the others."""
 import numpy as np
 import pytest
 
@@ -68,4 +69,27 @@ def test_odd_heads_prompts_with_splits(si_ctx, heads, prefix, count):
     for runs in ([(0, prefix, count)], [(1, 200, 131), (0, prefix, count)]):
         q = c.rng.standard_normal((sum(r[2] for r in runs), heads[0], heads[2]))
         c.check(c.attend(q, runs), q, runs, every=29)
+    c.kv.free()
+
+
+@pytest.mark.parametrize("nats", [8, 10, 12, 17])
+@pytest.mark.parametrize("heads,prefix,count", [
+    ((28, 4, 128), 0, 2048), ((16, 2, 128), 7580, 612), ((16, 2, 64), 7580, 612),
+    ((16, 2, 128), 40000, 612), ((12, 2, 128), 7900, 131), ((12, 2, 128), 8000, 2)])
+def test_a_first_key_far_above_the_others(si_ctx, heads, prefix, count, nats):
+    """Position 0 takes much of every row's weight and holds small values, as the first
+    token of a text does: the others, each of 2^-12 to 2^-25 of its weight, make the
+    output.  In one split of the keys, in many, and token by token."""
+    hq, hkv, D = heads
+    n = prefix + count
+    c = Cache(si_ctx, heads, 1, n, 64, seed=36)
+    k, v = (c.rng.standard_normal((n, hkv, D)) for _ in range(2))
+    u = np.sign(c.rng.standard_normal(D))
+    k[0] = u
+    v[0] *= 0.05
+    c.append([(0, 0, n)], k, v)
+    # u.q / sqrt(D) is the sink's score: noise of one nat about the given number
+    q = c.rng.standard_normal((count, hq, D)) + nats / np.sqrt(D) * u
+    runs = [(0, prefix, count)]
+    c.check(c.attend(q, runs), q, runs, every=199)
     c.kv.free()
