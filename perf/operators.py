@@ -16,16 +16,19 @@ import torch
 
 own = False
 
-_CTX = {}
+_CTX = []
 
 
-def _ctx(head_dim):
-    """The framework's context (one stream), kept for the process as a serving program keeps it."""
-    if head_dim not in _CTX:
+def _ctx():
+    """The framework's context, kept for the process as a serving program keeps it.  Its stream
+    becomes torch's current one, so that torch's work on inputs and outputs and the framework's calls
+    are in order."""
+    if not _CTX:
         sys.path.insert(0, os.path.join(os.getcwd(), "simple-inference_b200"))
         import sib200
-        _CTX[head_dim] = sib200.Context(0, max_positions=1024, head_dim=head_dim)
-    return _CTX[head_dim]
+        _CTX.append(sib200.Context(0, max_positions=1024))
+    torch.cuda.set_stream(torch.cuda.ExternalStream(_CTX[0].stream))
+    return _CTX[0]
 
 
 class _Wrapped:
@@ -203,7 +206,7 @@ def prepare(case, seed):
         state["from"] = torch.arange(R).repeat_interleave(C)
     if own:
         import numpy as np
-        ctx = _ctx(D)
+        ctx = _ctx()
         kv = ctx.kv4(_dims(case["model"]), n_seqs, wide * P, n_pages, P, pool=pool)
         seqs = [i for i, n in enumerate(need) if n]
         kv.assign(seqs, [need[i] for i in seqs], ids.numpy().astype(np.int32))
