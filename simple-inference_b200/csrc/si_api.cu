@@ -237,6 +237,10 @@ struct si_kv4 {
   int *tables = nullptr, *refs = nullptr;
   si::Kv4Pages *pages = nullptr;
   si::Kv4Edits edits;  // of the call in progress
+  si::Kv4Edits *new_edits() {  // (a call that threw may have left some)
+    edits.clear();
+    return &edits;
+  }
   si::Kv4View view() const {
     si::Kv4View v;
     v.pool = pool;
@@ -1304,7 +1308,7 @@ static si_status kv4_writable(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs, i
   }
   if (kv->pages->writable(as_runs(runs), n)) return SI_OK;
   SI_TRY(kv4_not_capturing(ctx));
-  SI_PAGES(kv, reserve(as_runs(runs), n, &kv->edits));
+  SI_PAGES(kv, reserve(as_runs(runs), n, kv->new_edits()));
   return kv4_flush(ctx, kv);
 }
 
@@ -1317,7 +1321,7 @@ extern "C" SI_API si_status si_kv4_reserve(si_ctx *ctx, si_kv4 *kv, const si_kv4
     for (int i = 0; i < n; ++i)
       SI_CHECK((int64_t)runs[i].pos + runs[i].count <= kv->max_ctx, "positions past max_ctx %d",
                kv->max_ctx);
-    SI_PAGES(kv, reserve(as_runs(runs), n, &kv->edits));
+    SI_PAGES(kv, reserve(as_runs(runs), n, kv->new_edits()));
     return kv4_flush(ctx, kv);
   });
 }
@@ -1328,7 +1332,7 @@ extern "C" SI_API si_status si_kv4_assign(si_ctx *ctx, si_kv4 *kv, const int *se
     SI_TRY(kv4_check(ctx, kv));
     SI_CHECK(n >= 0 && (n == 0 || (seqs && counts && pages)), "null argument");
     SI_TRY(kv4_not_capturing(ctx));
-    SI_PAGES(kv, assign(seqs, counts, n, pages, &kv->edits));
+    SI_PAGES(kv, assign(seqs, counts, n, pages, kv->new_edits()));
     return kv4_flush(ctx, kv);
   });
 }
@@ -1339,7 +1343,7 @@ extern "C" SI_API si_status si_kv4_fork(si_ctx *ctx, si_kv4 *kv, const int *src,
     SI_TRY(kv4_check(ctx, kv));
     SI_CHECK(n >= 0 && (n == 0 || (src && dst && lens)), "null argument");
     SI_TRY(kv4_not_capturing(ctx));
-    SI_PAGES(kv, fork(src, dst, lens, n, &kv->edits));
+    SI_PAGES(kv, fork(src, dst, lens, n, kv->new_edits()));
     return kv4_flush(ctx, kv);
   });
 }
@@ -1350,7 +1354,7 @@ extern "C" SI_API si_status si_kv4_release(si_ctx *ctx, si_kv4 *kv, const int *s
     SI_TRY(kv4_check(ctx, kv));
     SI_CHECK(n >= 0 && (n == 0 || seqs), "null argument");
     SI_TRY(kv4_not_capturing(ctx));
-    SI_PAGES(kv, release(seqs, keep, n, &kv->edits));
+    SI_PAGES(kv, release(seqs, keep, n, kv->new_edits()));
     return kv4_flush(ctx, kv);
   });
 }
@@ -1359,7 +1363,7 @@ extern "C" SI_API si_status si_kv4_compact(si_ctx *ctx, si_kv4 *kv, int *used) {
   return kv4_entry([&]() -> si_status {
     SI_TRY(kv4_check(ctx, kv));
     SI_TRY(kv4_not_capturing(ctx));
-    const int n = kv->pages->compact(&kv->edits);
+    const int n = kv->pages->compact(kv->new_edits());
     SI_TRY(kv4_flush(ctx, kv));
     if (used) *used = n;
     return SI_OK;

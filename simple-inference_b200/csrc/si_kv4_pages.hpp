@@ -4,8 +4,9 @@
 // each change asks of the device (table entries, reference counts, page
 // copies) on the context's stream.
 //
-// Every change is checked in full before anything is touched, so a refused
-// call leaves the tables as they were.  Free pages are handed out lowest first.
+// Every change is checked in full, and the room for what it asks of the device is
+// taken, before anything is touched: a call that is refused or throws (host memory
+// has run out) leaves the tables as they were.  Free pages are handed out lowest first.
 #pragma once
 #include <stdint.h>
 
@@ -36,6 +37,13 @@ struct Kv4Edits {
   std::vector<int> literal;
   std::vector<std::pair<int, int>> table;  // (entry, page)
   std::vector<std::pair<int, int>> copies; // (from page, to page)
+  // Room for as many more of each, so that adding them does not throw.
+  void room(size_t n_spans, size_t n_literal, size_t n_table, size_t n_copies) {
+    spans.reserve(spans.size() + n_spans);
+    literal.reserve(literal.size() + n_literal);
+    table.reserve(table.size() + n_table);
+    copies.reserve(copies.size() + n_copies);
+  }
   void clear() {
     spans.clear();
     literal.clear();
@@ -101,7 +109,7 @@ class Kv4Pages {
     // A dry run that counts the pages taken.  Of a page's holders the ones that
     // write get copies, except that the last holder left keeps the page.
     std::vector<int> have(count_);
-    int64_t need = 0;
+    int64_t grown = 0, copied = 0;
     std::vector<std::pair<int, int>> shared;  // (page, table entry), each pair once
     for (const Kv4Run &x : r) {
       const int p0 = x.pos / page_len_, p1 = last_page(x);
@@ -110,7 +118,7 @@ class Kv4Pages {
         if (refs_[pg] > 1) shared.push_back({pg, (int)at(x.seq, p)});
       }
       if (p1 + 1 > have[x.seq]) {
-        need += p1 + 1 - have[x.seq];
+        grown += p1 + 1 - have[x.seq];
         have[x.seq] = p1 + 1;
       }
     }
@@ -119,10 +127,11 @@ class Kv4Pages {
     for (size_t i = 0; i < shared.size();) {
       size_t j = i;
       while (j < shared.size() && shared[j].first == shared[i].first) ++j;
-      need += std::min((int64_t)(j - i), (int64_t)refs_[shared[i].first] - 1);
+      copied += std::min((int64_t)(j - i), (int64_t)refs_[shared[i].first] - 1);
       i = j;
     }
-    if (need > n_free_) return no("not enough free pages");
+    if (grown + copied > n_free_) return no("not enough free pages");
+    e->room(r.size(), grown, copied, copied);
     for (const Kv4Run &x : r) {
       const int p0 = x.pos / page_len_, p1 = last_page(x);
       for (int p = p0; p < std::min(p1 + 1, count_[x.seq]); ++p) {
@@ -160,8 +169,7 @@ class Kv4Pages {
     bool bad = false;
     for (int64_t i = 0; i < total; ++i) bad |= (unsigned)pages[i] >= limit;
     if (bad) return no("page out of range");
-    e->literal.reserve(e->literal.size() + total);
-    e->spans.reserve(e->spans.size() + n);
+    e->room(n, total, 0, 0);
     int *__restrict refs = refs_.data();
     int taken = 0;
     for (int64_t i = 0; i < total; ++i) taken += refs[pages[i]]++ == 0;
@@ -191,6 +199,7 @@ class Kv4Pages {
       need += lens[i] % page_len_ != 0;
     }
     if (need > n_free_) return no("not enough free pages");
+    e->room(n, 0, need, need);
     for (int i = 0; i < n; ++i) {
       const int whole = lens[i] / page_len_;
       const int *from = table_.data() + at(src[i], 0);
@@ -214,6 +223,7 @@ class Kv4Pages {
       if (!seq_ok(seqs[i])) return false;
       if (keep && keep[i] < 0) return no("negative length");
     }
+    e->room(n, 0, 0, 0);
     for (int i = 0; i < n; ++i) {
       const int64_t len = keep ? keep[i] : 0;
       const int64_t stay = (len + page_len_ - 1) / page_len_;
