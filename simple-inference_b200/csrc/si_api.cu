@@ -1265,7 +1265,8 @@ static si_status kv4_push(si_ctx *ctx, si_kv4 *kv) {
   return SI_OK;
 }
 
-// Queues a change of the pages on the context's stream.
+// Queues a change of the pages on the context's stream.  Where a launch fails, the
+// host's tables are ahead of the device's: the cache refuses all further calls.
 static si_status kv4_flush(si_ctx *ctx, si_kv4 *kv) {
   si::Kv4Edits &e = kv->edits;
   const size_t n = 3 * e.spans.size() + e.literal.size() + 2 * (e.table.size() + e.copies.size());
@@ -1275,6 +1276,7 @@ static si_status kv4_flush(si_ctx *ctx, si_kv4 *kv) {
          : n <= si::kKv4MediumWords ? kv4_push<si::kKv4MediumWords>(ctx, kv)
                                     : kv4_push<si::kKv4LargeWords>(ctx, kv);
   e.clear();
+  if (st != SI_OK) kv->pages->lose();
   return st;
 }
 
@@ -1284,6 +1286,8 @@ static si_status kv4_flush(si_ctx *ctx, si_kv4 *kv) {
 static si_status kv4_check(si_ctx *ctx, const si_kv4 *kv) {
   SI_TRY(set_device(ctx));
   SI_CHECK(kv && kv->ctx == ctx, "null KV cache, or one of another context");
+  if (kv->pages->lost())
+    return fail(SI_ERR_CUDA, "an earlier change of the cache's pages did not reach the device");
   return SI_OK;
 }
 
@@ -2198,8 +2202,8 @@ static si_status run_rows(const si_kv4_run *runs, int n, int *T) {
 extern "C" SI_API si_status si_step_kv4_dev(si_ctx *ctx, si_layer *l, si_kv4 *kv, const float *x,
                                             const si_kv4_run *runs, int n, float *y, int mode) {
   return kv4_entry([&]() -> si_status {
-    SI_TRY(set_device(ctx));
-    SI_CHECK(l && kv && kv->ctx == ctx, "null argument, or a cache of another context");
+    SI_TRY(kv4_check(ctx, kv));
+    SI_CHECK(l, "null layer");
     int T = 0;
     SI_TRY(run_rows(runs, n, &T));
     return run_step(ctx, l, nullptr, x, T, nullptr, nullptr, 0, 0, y, mode, nullptr, false,
@@ -2211,8 +2215,8 @@ extern "C" SI_API si_status si_decode_step_state_kv4_dev(si_ctx *ctx, si_layer *
                                                          const float *x, si_decode_state *st,
                                                          float *y, int mode) {
   return kv4_entry([&]() -> si_status {
-    SI_TRY(set_device(ctx));
-    SI_CHECK(l && kv && kv->ctx == ctx && st, "null argument, or a cache of another context");
+    SI_TRY(kv4_check(ctx, kv));
+    SI_CHECK(l && st, "null layer or state");
     SI_CHECK(st->batch <= kv->pages->n_seqs(), "batch %d exceeds the cache's %d sequences",
              st->batch, kv->pages->n_seqs());
     return run_step(ctx, l, nullptr, x, st->batch, nullptr, nullptr, 0, 0, y, mode, nullptr, false,

@@ -71,8 +71,14 @@ class Kv4Pages {
   // Positions of seq that its pages cover.
   int64_t covered(int seq) const { return (int64_t)count_[seq] * page_len_; }
 
+  // A change did not reach the device in full, whose tables are no longer these:
+  // from now on every call is refused.
+  void lose() { lost_ = true; }
+  bool lost() const { return lost_; }
+
   // Runs within the cache's sequences and positions.
   bool runs_ok(const Kv4Run *runs, int n) {
+    if (!usable()) return false;
     for (int i = 0; i < n; ++i) {
       if (!seq_ok(runs[i].seq)) return false;
       if (runs[i].pos < 0 || runs[i].count < 0 ||
@@ -84,6 +90,7 @@ class Kv4Pages {
 
   // Every page that the runs write to is there and held by their sequence alone.
   bool writable(const Kv4Run *runs, int n) const {
+    if (lost_) return false;
     for (int i = 0; i < n; ++i) {
       const Kv4Run &x = runs[i];
       if (x.count <= 0) continue;
@@ -95,7 +102,9 @@ class Kv4Pages {
     return true;
   }
 
-  bool seq_ok(int seq) { return (seq >= 0 && seq < n_seqs_) || no("sequence out of range"); }
+  bool seq_ok(int seq) {
+    return usable() && ((seq >= 0 && seq < n_seqs_) || no("sequence out of range"));
+  }
 
   // Positions [pos, pos + count) of every run get pages that no other
   // sequence holds: missing pages (from the sequence's first missing one) are
@@ -156,6 +165,7 @@ class Kv4Pages {
   // Sequence seqs[i] (empty until now) holds the next counts[i] pages of the
   // list, each of which may be held by others already.
   bool assign(const int *seqs, const int *counts, int n, const int *pages, Kv4Edits *e) {
+    if (!usable()) return false;
     std::vector<char> seen(n_seqs_, 0);
     int64_t total = 0;
     for (int i = 0; i < n; ++i) {
@@ -188,6 +198,7 @@ class Kv4Pages {
   // dst[i] (empty until now) begins with the first lens[i] positions of
   // src[i]: whole pages are shared, the page that lens[i] ends in is copied.
   bool fork(const int *src, const int *dst, const int *lens, int n, Kv4Edits *e) {
+    if (!usable()) return false;
     std::vector<char> seen(n_seqs_, 0);
     int64_t need = 0;
     for (int i = 0; i < n; ++i) {
@@ -219,6 +230,7 @@ class Kv4Pages {
 
   // seqs[i] keeps the pages of its first keep[i] positions (keep null: none).
   bool release(const int *seqs, const int *keep, int n, Kv4Edits *e) {
+    if (!usable()) return false;
     for (int i = 0; i < n; ++i) {
       if (!seq_ok(seqs[i])) return false;
       if (keep && keep[i] < 0) return no("negative length");
@@ -247,8 +259,9 @@ class Kv4Pages {
   }
 
   // The used pages become pages [0, used): the used pages from `used` on move,
-  // in ascending order, to the free ones below.  Returns used.
+  // in ascending order, to the free ones below.  Returns used, -1 where refused.
   int compact(Kv4Edits *e) {
+    if (!usable()) return -1;
     const int used = n_pages() - n_free_;
     // Which pages are used follows no pattern: lists without branches.  The i-th hole
     // takes the i-th mover; to[] is where a page ends up.
@@ -297,6 +310,9 @@ class Kv4Pages {
   int last_page(const Kv4Run &x) const {
     return (int)(((int64_t)x.pos + x.count - 1) / page_len_);
   }
+  bool usable() {
+    return !lost_ || no("an earlier change of the pages did not reach the device");
+  }
   bool no(const char *why) {
     why_ = why;
     return false;
@@ -331,6 +347,7 @@ class Kv4Pages {
 
   int n_seqs_, max_pages_, page_len_, n_free_;
   int first_free_ = 0;  // no free page lies below
+  bool lost_ = false;
   std::vector<int> count_, refs_, table_;
   std::string why_;
 };

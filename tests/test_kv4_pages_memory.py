@@ -1,5 +1,6 @@
 """CPU tests of the 4-bit cache's page bookkeeping (csrc/si_kv4_pages.hpp) when the host
-runs out of memory: a call that throws has changed nothing."""
+runs out of memory, and after a change that did not reach the device: a call that
+throws has changed nothing, and lost pages refuse every call."""
 import os
 import subprocess
 
@@ -99,7 +100,28 @@ int main() {
 }
 """
 
-@pytest.mark.parametrize("name", ["MEMORY"])
+LOST = HEAD + r"""
+int main() {
+  Kv4Pages k(3, 4, 8, 16);
+  Kv4Edits e;
+  const Kv4Run run[1] = {{0, 0, 20}};
+  const int a[1] = {0}, b[1] = {1}, c[1] = {1}, d[1] = {7};
+  if (!k.reserve(run, 1, &e) || k.lost()) return 1;
+  k.lose();
+  if (!k.lost()) return 2;
+  e.clear();
+  if (k.runs_ok(run, 1) || k.seq_ok(0) || k.writable(run, 1)) return 3;
+  if (k.reserve(run, 1, &e) || k.assign(b, c, 1, d, &e) || k.fork(a, b, c, 1, &e) ||
+      k.release(a, nullptr, 1, &e) || k.compact(&e) >= 0)
+    return 4;
+  if (!e.spans.empty() || !e.table.empty() || !e.copies.empty() || k.why().empty()) return 5;
+  if (k.count(0) != 2 || k.free_pages() != 6) return 6;
+  return 0;
+}
+"""
+
+
+@pytest.mark.parametrize("name", ["MEMORY", "LOST"])
 def test_pages(name, tmp_path):
     (tmp_path / "t.cpp").write_text(globals()[name])
     exe = str(tmp_path / "t")
