@@ -463,9 +463,10 @@ SI_API si_status si_attention_prefill_dev(si_ctx *ctx, si_kv *kv, const si_dims 
 /* The page tables are kept on the host and mirrored on the device; calls that  */
 /* change them are refused (SI_ERR_INVALID) during a graph capture, take their  */
 /* arguments at once, and queue the device's part on the context's stream.  A   */
-/* refused call changes nothing.  If the device's part cannot be queued          */
-/* (SI_ERR_CUDA), the cache refuses every later call.  Free pages are handed out */
-/* lowest first.                                                                 */
+/* refused call changes nothing; a step that lacks memory only for its attention */
+/* has taken its pages and written its positions, and may be made again.  If the  */
+/* device's part cannot be queued (SI_ERR_CUDA), the cache refuses every later    */
+/* call.  Free pages are handed out lowest first.                                 */
 /* Calls on one cache come from one thread at a time, like all calls of one     */
 /* context.                                                                     */
 /* ------------------------------------------------------------------------ */

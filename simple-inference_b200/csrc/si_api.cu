@@ -1880,7 +1880,6 @@ static si_status run_step(si_ctx *ctx, si_layer *l, si_kv *kv, const float *x, i
       SI_CHECK(runs[i].count <= 0 ||
                    (int64_t)runs[i].pos + runs[i].count <= ctx->max_positions,
                "positions past the context's %d", ctx->max_positions);
-    if (!st) SI_TRY(kv4_writable(ctx, kv4, runs, n_runs));
   } else if (st) {
     // Lengths are on the device: the kernels bound every position by the
     // cache (rope_kv appends nothing past it, attention clamps), and the
@@ -1905,6 +1904,8 @@ static si_status run_step(si_ctx *ctx, si_layer *l, si_kv *kv, const float *x, i
   const bool decode_form = ctx_host != nullptr || st != nullptr;
   const int nsplit = kv4 ? 1 : si::attn_pick_splits(T, decode_form, max_len);
   SI_TRY(ctx->work.reserve(step_bytes(d, T, nsplit, true)));
+  // (after the memory of the step: one that is refused for want of it takes no pages)
+  if (kv4 && !st) SI_TRY(kv4_writable(ctx, kv4, runs, n_runs));
   StepBuffers b = carve(ctx->work.p, d, T, nsplit);
   cudaStream_t s = ctx->stream;
 

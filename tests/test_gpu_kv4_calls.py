@@ -1,0 +1,26 @@
+"""GPU tests of calls on the 4-bit cache that are refused."""
+import pytest
+
+import sib200
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def test_a_step_that_lacks_memory_takes_no_pages():
+    """Two million tokens of the 72B dims want 375 GB of workspace."""
+    dims = dict(hidden=8192, n_q_heads=64, n_kv_heads=8, head_dim=128, intermediate=0,
+                rope_theta=1e6, rms_eps=1e-6)
+    ctx = sib200.Context(0, max_positions=8192, rope_theta=1e6, head_dim=128)
+    layer = ctx.layer_synth(dims, 2)
+    kv = ctx.kv4(dims, 256, 8192, 512, 4096)
+    x, y = torch.randn(1, 8192, device="cuda"), torch.zeros(1, 8192, device="cuda")
+    torch.cuda.synchronize()
+    with pytest.raises(sib200.SiError) as e:
+        layer.step_dev(kv, x, [(s, 0, 8192) for s in range(256)], y)
+    assert e.value.status == sib200.SI_ERR_OOM
+    assert kv.free_pages() == 512 and kv.pages(0) == []
+    layer.step_dev(kv, x, [(3, 0, 1)], y)
+    ctx.status()
+    assert kv.free_pages() == 511 and torch.isfinite(y).all()
+    ctx.close()
