@@ -527,8 +527,8 @@ SI_API si_status si_kv4_read_dev(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs
  * sequence, whose pages must cover it.  A run at pos -1 begins with a token
  * that attends nothing; its row of out is zeros (padding of a batch).  Runs of 13
  * tokens and more, where they have enough work together, go through a prompt kernel
- * on the tensor cores (with si_ctx_set_exact_attention the fp32 one over their keys
- * unpacked), the others read the packed cache token by token.  fp32 in and out, within about 1e-6 of
+ * on the tensor cores (with si_ctx_set_exact_attention those of 16 and more through the
+ * fp32 one over their keys unpacked), the others read the packed cache token by token.  fp32 in and out, within about 1e-6 of
  * the 64-bit result.  Sums follow the split of the work, so a token's result may
  * differ in its last bits between calls with other runs.  A position whose V
  * holds infinities or NaN makes whole rows NaN that attend it in the prompt

@@ -48,7 +48,6 @@ constexpr int kSplitKeys = 128;    // keys per split
 constexpr int kSubPerSplit = kSplitKeys / kSub;
 constexpr int kPrefillRows = 64;   // query rows (token x head) per prefill CTA
 constexpr int kPrefillThreads = 256;
-constexpr int kPrefillMinTokens = 16;
 
 __host__ __device__ __forceinline__ int splits_for(int L) {
   const int s = (L + kSplitKeys - 1) / kSplitKeys;

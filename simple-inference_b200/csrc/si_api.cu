@@ -1120,11 +1120,15 @@ static const si::Kv4Run *as_runs(const si_kv4_run *r) {
 // time (0.5B, 2000: 64 tokens 13 against 20 us, 128 24.5 against 23.7 us).  Runs of
 // fewer tokens fill too little of a row tile, however many they are (7B, 2000
 // positions: 16 runs of 8 53 against 74 us, of 12 73 against 76, 8 of 15 52 against 39).
-static bool kv4_prompt_run(const si_kv4_run &r) { return r.pos >= 0 && r.count >= 13; }
-static bool kv4_prompts_pay(const si_kv4 *kv, const si_kv4_run *runs, int n) {
+// The fp32 prefill kernel takes kPrefillMinTokens and more.
+static bool kv4_prompt_run(const si_ctx *ctx, const si_kv4_run &r) {
+  return r.pos >= 0 && r.count >= (ctx->exact_attention ? si::kPrefillMinTokens : 13);
+}
+static bool kv4_prompts_pay(const si_ctx *ctx, const si_kv4 *kv, const si_kv4_run *runs, int n) {
   double work = 0;
   for (int i = 0; i < n; ++i)
-    if (kv4_prompt_run(runs[i])) work += (runs[i].count - 8) * (runs[i].pos + 0.5 * runs[i].count);
+    if (kv4_prompt_run(ctx, runs[i]))
+      work += (runs[i].count - 8) * (runs[i].pos + 0.5 * runs[i].count);
   return work * kv->d.n_kv_heads * (kv->d.head_dim + 64) / 192 >= 3.3e5;
 }
 
@@ -1571,13 +1575,13 @@ static si_status kv4_attend(si_ctx *ctx, si_kv4 *kv, int n_q_heads, const float 
   }
   const std::vector<int> rows = kv4_rows(runs, n);
   // Decode tokens, short and early prompts: one token at a time.
-  const bool tiles = kv4_prompts_pay(kv, runs, n);
+  const bool tiles = kv4_prompts_pay(ctx, kv, runs, n);
   std::vector<si_kv4_run> few;
   std::vector<int> few_rows;
   std::vector<si::Kv4Prompt> prompts;
   for (int i = 0; i < n; ++i) {
     if (runs[i].count <= 0) continue;
-    if (tiles && kv4_prompt_run(runs[i])) {
+    if (tiles && kv4_prompt_run(ctx, runs[i])) {
       prompts.push_back({runs[i].seq, runs[i].pos, runs[i].count, rows[i]});
     } else {
       few.push_back(runs[i]);

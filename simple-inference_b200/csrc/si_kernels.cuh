@@ -189,6 +189,7 @@ struct AttnArgs {
   const float *qkv;
   const float *cos_tab, *sin_tab;  // [positions][D/2]
 };
+constexpr int kPrefillMinTokens = 16;  // of the prefill kernel
 size_t attn_part_floats(int T, int n_q_heads, int head_dim, int nsplit);
 // Splits the launch needs: 1 when the prefill kernel runs (contiguous tokens
 // of one sequence, T >= 16), else ceil(max_len / 128).

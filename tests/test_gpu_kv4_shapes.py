@@ -93,3 +93,21 @@ def test_a_first_key_far_above_the_others(si_ctx, heads, prefix, count, nats):
     runs = [(0, prefix, count)]
     c.check(c.attend(q, runs), q, runs, every=199)
     c.kv.free()
+
+
+@pytest.mark.parametrize("exact", [False, True])
+@pytest.mark.parametrize("count", [12, 13, 15, 16, 17])
+def test_short_runs_on_many_positions(si_ctx, count, exact):
+    """Runs on both sides of the fewest tokens of either prompt kernel, with enough work
+    for them, alone and beside a longer one."""
+    heads = (64, 8, 128)
+    c = Cache(si_ctx, heads, 2, 6100, 64, seed=37)
+    c.random([(0, 0, 6100), (1, 0, 2000)])
+    si_ctx.set_exact_attention(exact)
+    try:
+        for runs in ([(0, 6100 - count, count)], [(0, 6001, count), (1, 1900, 40), (0, 3000, 13)]):
+            q = c.rng.standard_normal((sum(r[2] for r in runs), heads[0], heads[2]))
+            c.check(c.attend(q, runs), q, runs, every=6)
+    finally:
+        si_ctx.set_exact_attention(False)
+    c.kv.free()
