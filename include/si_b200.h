@@ -532,7 +532,8 @@ SI_API si_status si_kv4_read_dev(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs
  * the 64-bit result.  Sums follow the split of the work, so a token's result may
  * differ in its last bits between calls with other runs.  A position whose V
  * holds infinities or NaN makes whole rows NaN that attend it in the prompt
- * kernel, the affected dims in the other. */
+ * kernels, the affected dims in the other; rows that do not attend it keep their
+ * results. */
 SI_API si_status si_attention_kv4_dev(si_ctx *ctx, si_kv4 *kv, const si_dims *dims,
                                       const float *q_dev, const si_kv4_run *runs, int n,
                                       float *out_dev);

@@ -195,8 +195,10 @@ __device__ __forceinline__ float code_at(uint32_t w, int i) {
 }
 
 // Rows back to fp32, laid out as above: grid (tokens, ceil(2 Hkv / kUnits)).  A
-// position without a page reads as zeros and is recorded.
-template <int D>
+// position without a page reads as zeros and is recorded.  MARK, for an attention whose
+// probability 0 would not mask a V that is no number from the queries before it: its key's
+// scores become NaN instead, and with them the rows that attend it.
+template <int D, bool MARK>
 __global__ void __launch_bounds__(32 * kWarps) k_kv4_read(const __grid_constant__ Kv4ReadArgs a) {
   pdl_trigger();
   pdl_wait();
@@ -221,7 +223,12 @@ __global__ void __launch_bounds__(32 * kWarps) k_kv4_read(const __grid_constant_
       const uint8_t *p =
           grp + (u < Hkv ? u * head_bytes : (u - Hkv) * head_bytes + kv4_group_bytes(D) / 2);
       w[k] = reinterpret_cast<const uint16_t *>(p + r16 * (D / 2))[g * NB + b];
-      sc[k] = f16_to_f32(reinterpret_cast<const uint16_t *>(p + kKv4Group * (D / 2))[r16 * NB + b]);
+      const uint16_t *scale = reinterpret_cast<const uint16_t *>(p + kKv4Group * (D / 2)) + r16 * NB + b;
+      sc[k] = f16_to_f32(*scale);
+      if constexpr (MARK) {
+        const uint16_t v = u < Hkv ? scale[kv4_group_bytes(D) / 4] : *scale;  // the V half's
+        if ((v & 0x7c00u) == 0x7c00u) sc[k] = u < Hkv ? __int_as_float(0x7fffffff) : 0.0f;
+      }
     }
   }
 #pragma unroll
@@ -310,8 +317,9 @@ cudaError_t launch_kv4_append(const Kv4AppendArgs &a, cudaStream_t s) {
 cudaError_t launch_kv4_read(const Kv4ReadArgs &a, cudaStream_t s) {
   if (a.T <= 0) return cudaSuccess;
   const dim3 grid(a.T, (2 * a.kv.n_kv_heads + kUnits - 1) / kUnits);
-  return a.kv.head_dim == 128 ? launch_pdl(k_kv4_read<128>, grid, dim3(32 * kWarps), 0, s, a)
-                              : launch_pdl(k_kv4_read<64>, grid, dim3(32 * kWarps), 0, s, a);
+  auto *kern = a.kv.head_dim == 128 ? (a.mark ? k_kv4_read<128, true> : k_kv4_read<128, false>)
+                                    : (a.mark ? k_kv4_read<64, true> : k_kv4_read<64, false>);
+  return launch_pdl(kern, grid, dim3(32 * kWarps), 0, s, a);
 }
 
 template <int WORDS>

@@ -1467,9 +1467,10 @@ static si_status kv4_covered(const si_kv4 *kv, const si_kv4_run *runs, int n, in
 }
 
 static si_status kv4_read(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs, int n, float *k,
-                          float *v) {
+                          float *v, bool mark) {
   const std::vector<int> rows = kv4_rows(runs, n);
   si::Kv4ReadArgs a{};
+  a.mark = mark;
   a.kv = kv->view();
   a.k = k;
   a.v = v;
@@ -1491,7 +1492,7 @@ extern "C" SI_API si_status si_kv4_read_dev(si_ctx *ctx, si_kv4 *kv, const si_kv
     SI_TRY(kv4_covered(kv, runs, n, 0));
     SI_CHECK(((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0,
              "K and V rows must be 16-byte aligned");
-    return kv4_read(ctx, kv, runs, n, k, v);
+    return kv4_read(ctx, kv, runs, n, k, v, false);
   });
 }
 
@@ -1615,7 +1616,7 @@ static si_status kv4_attend(si_ctx *ctx, si_kv4 *kv, int n_q_heads, const float 
     SI_TRY(ctx->kv4.reserve(2 * L * kvd * sizeof(float)));
     float *kf = static_cast<float *>(ctx->kv4.p), *vf = kf + L * kvd;
     const si_kv4_run all{x.seq, 0, L};
-    SI_TRY(kv4_read(ctx, kv, &all, 1, kf, vf));
+    SI_TRY(kv4_read(ctx, kv, &all, 1, kf, vf, true));
     si::AttnArgs aa{};
     aa.q = q + x.row * row;
     aa.kc = kf;

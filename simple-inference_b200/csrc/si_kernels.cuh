@@ -255,6 +255,7 @@ struct Kv4ReadArgs {
   int T;
   float *k, *v;  // [.][Hkv][D] fp32, either may be null
   int *err;
+  bool mark;     // blocks of V that are no numbers become zeros, and NaN in K
 };
 cudaError_t launch_kv4_read(const Kv4ReadArgs &a, cudaStream_t s);
 // word: n_spans triples (to, n, from) of table entries that become the entries

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import sib200
-from test_gpu_kv4 import Cache
+from test_gpu_kv4 import Cache, up
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -111,3 +111,32 @@ def test_short_runs_on_many_positions(si_ctx, count, exact):
     finally:
         si_ctx.set_exact_attention(False)
     c.kv.free()
+
+
+@pytest.mark.parametrize("exact", [False, True])
+@pytest.mark.parametrize("heads", [(12, 2, 128), (14, 2, 64)])
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("prefix,where", [(4100, 57), (4100, 0), (20, 57)])
+def test_values_that_are_no_numbers_reach_only_later_rows(si_ctx, heads, prefix, where, what, exact):
+    """One block of one head's V of position prefix + where is no number: the rows before it
+    and the other KV head's keep their results, in every kernel."""
+    hq, hkv, D = heads
+    c = Cache(si_ctx, heads, 1, prefix + 100, 32, seed=38)
+    c.random([(0, 0, prefix + 100)])
+    one = np.ones((1, hkv, D), np.float32)
+    bad = one.copy()
+    bad[0, 1, 32:64] = what
+    kd, vd = up(one), up(bad)
+    torch.cuda.synchronize()
+    c.kv.append(kd, vd, [(0, prefix + where, 1)])
+    q = c.rng.standard_normal((100, hq, D))
+    si_ctx.set_exact_attention(exact)
+    try:
+        got = c.attend(q, [(0, prefix, 100)])
+    finally:
+        si_ctx.set_exact_attention(False)
+    assert np.isfinite(got[:where]).all()
+    if where:
+        c.check(got[:where], q[:where], [(0, prefix, where)], every=19)
+    assert np.isfinite(got[:, :hq // 2]).all()
+    assert np.isnan(got[where:, hq // 2:, 32:64]).all()
