@@ -1644,6 +1644,7 @@ extern "C" SI_API si_status si_attention_kv4_dev(si_ctx *ctx, si_kv4 *kv, const 
     SI_TRY(check_dims(d));
     SI_CHECK(kv->d.n_kv_heads == d->n_kv_heads && kv->d.head_dim == d->head_dim,
              "KV cache dims do not match");
+    SI_CHECK(d->n_q_heads > 0, "no query heads");
     int T = 0;
     SI_TRY(kv4_count(runs, n, &T));
     if (T == 0) return SI_OK;

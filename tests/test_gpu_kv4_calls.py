@@ -24,3 +24,20 @@ def test_a_step_that_lacks_memory_takes_no_pages():
     ctx.status()
     assert kv.free_pages() == 511 and torch.isfinite(y).all()
     ctx.close()
+
+
+@pytest.mark.parametrize("n_q_heads", [0, -8])
+def test_attention_without_query_heads_is_refused(si_ctx, n_q_heads):
+    dims = dict(hidden=1024, n_q_heads=8, n_kv_heads=8, head_dim=128, intermediate=0)
+    kv = si_ctx.kv4(dims, 1, 4096, 64, 64)
+    kv.reserve([(0, 0, 4096)])
+    q, out = torch.randn(64, 1024, device="cuda"), torch.zeros(64, 1024, device="cuda")
+    torch.cuda.synchronize()
+    for runs in ([(0, 300, 1)], [(0, 4032, 64)]):
+        with pytest.raises(sib200.SiError) as e:
+            si_ctx.attention_kv4(kv, dict(dims, n_q_heads=n_q_heads), q, runs, out)
+        assert e.value.status == sib200.SI_ERR_INVALID
+    si_ctx.attention_kv4(kv, dims, q, [(0, 4032, 64)], out)
+    si_ctx.status()
+    assert torch.isfinite(out).all()
+    kv.free()
