@@ -482,7 +482,8 @@ typedef struct {
 SI_API size_t si_kv4_page_bytes(const si_dims *dims, int page_len);
 /* pool_dev NULL: the pool is allocated and zeroed; else n_pages *
  * si_kv4_page_bytes of the caller's device memory, 16-byte aligned, used as it
- * is and left to the caller, who keeps it until si_kv4_free. */
+ * is and left to the caller, who keeps it until si_kv4_free.  A page has fewer
+ * than 2^32 bytes. */
 SI_API si_status si_kv4_create(si_ctx *ctx, const si_dims *dims, int n_seqs, int max_ctx,
                                int n_pages, int page_len, void *pool_dev, si_kv4 **out);
 SI_API void si_kv4_free(si_kv4 *kv);

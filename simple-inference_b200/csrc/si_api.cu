@@ -1152,6 +1152,8 @@ extern "C" SI_API si_status si_kv4_create(si_ctx *ctx, const si_dims *d, int n_s
     SI_CHECK(max_pages * n_seqs < (1ll << 30), "too many table entries");
     SI_CHECK((int64_t)n_pages * d->n_kv_heads * (page_len / si::kKv4Group) < (1ll << 31),
              "too many pages");
+    // (the kernels find a head's part of a page by a product of 32 bits)
+    SI_CHECK(si_kv4_page_bytes(d, page_len) < (1ull << 32), "pages of 4 GB and more");
     SI_CHECK((reinterpret_cast<uintptr_t>(pool_dev) & 15) == 0, "pool must be 16-byte aligned");
     si_kv4 *kv = new si_kv4();
     kv->ctx = ctx;

@@ -41,3 +41,14 @@ def test_attention_without_query_heads_is_refused(si_ctx, n_q_heads):
     si_ctx.status()
     assert torch.isfinite(out).all()
     kv.free()
+
+
+def test_pages_of_four_gigabytes_are_refused(si_ctx):
+    """Whose heads lie at offsets past 32 bits; the page length below is taken."""
+    dims = dict(hidden=1024, n_q_heads=8192, n_kv_heads=8192, head_dim=128, intermediate=0)
+    assert sib200.kv4_page_bytes(dims, 4096) > 1 << 32
+    small = torch.zeros(1024, dtype=torch.uint8, device="cuda")  # not touched by the creation
+    with pytest.raises(sib200.SiError) as e:
+        si_ctx.kv4(dims, 1, 4096, 1, 4096, small.data_ptr())
+    assert e.value.status == sib200.SI_ERR_INVALID
+    si_ctx.kv4(dims, 1, 4096, 1, 2048, small.data_ptr()).free()
