@@ -1155,6 +1155,11 @@ extern "C" SI_API si_status si_kv4_create(si_ctx *ctx, const si_dims *d, int n_s
     // (the kernels find a head's part of a page by a product of 32 bits)
     SI_CHECK(si_kv4_page_bytes(d, page_len) < (1ull << 32), "pages of 4 GB and more");
     SI_CHECK((reinterpret_cast<uintptr_t>(pool_dev) & 15) == 0, "pool must be 16-byte aligned");
+    if (pool_dev) {
+      cudaPointerAttributes at{};
+      SI_CUDA(cudaPointerGetAttributes(&at, pool_dev));
+      SI_CHECK(at.type != cudaMemoryTypeUnregistered, "pool is not memory of a device");
+    }
     si_kv4 *kv = new si_kv4();
     kv->ctx = ctx;
     kv->d = *d;

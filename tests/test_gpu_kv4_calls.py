@@ -52,3 +52,13 @@ def test_pages_of_four_gigabytes_are_refused(si_ctx):
         si_ctx.kv4(dims, 1, 4096, 1, 4096, small.data_ptr())
     assert e.value.status == sib200.SI_ERR_INVALID
     si_ctx.kv4(dims, 1, 4096, 1, 2048, small.data_ptr()).free()
+
+
+def test_a_pool_in_host_memory_is_refused(si_ctx):
+    dims = dict(hidden=1024, n_q_heads=8, n_kv_heads=8, head_dim=128, intermediate=0)
+    pool = torch.zeros(4 * sib200.kv4_page_bytes(dims, 16), dtype=torch.uint8)
+    for p in (pool, pool.numpy(), pool.data_ptr()):
+        with pytest.raises(sib200.SiError) as e:
+            si_ctx.kv4(dims, 1, 64, 4, 16, p)
+        assert e.value.status == sib200.SI_ERR_INVALID
+    si_ctx.kv4(dims, 1, 64, 4, 16, pool.cuda()).free()
