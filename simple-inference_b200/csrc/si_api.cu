@@ -95,7 +95,11 @@ struct DevBuf {
   si_status reserve(size_t n) {
     if (n <= bytes) return SI_OK;
     if (p && held) {
-      kept.push_back(p);
+      try {
+        kept.push_back(p);
+      } catch (...) {  // (nothing changed; no exception leaves a C entry)
+        return SI_ERR_OOM;
+      }
       kept_bytes += bytes;
     } else if (p) {
       cudaFree(p);
@@ -1102,7 +1106,11 @@ static si_status kv4_entry(F f) {
   try {
     return f();
   } catch (...) {
+  }
+  try {
     return fail(SI_ERR_OOM, "out of host memory");
+  } catch (...) {  // not even for the message
+    return SI_ERR_OOM;
   }
 }
 
