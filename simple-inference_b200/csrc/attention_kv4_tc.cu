@@ -52,6 +52,7 @@
 // ahead 322, operands by packed arithmetic 305, now 302 (three MMAs a product: 430 TFLOP/s are
 // 1290); 7B, a prompt of 2048: 101.
 #include <algorithm>
+#include <atomic>
 
 #include "si_common.cuh"
 #include "si_kernels.cuh"
@@ -1026,12 +1027,16 @@ cudaError_t launch(const Kv4PromptArgs &a, char *base, const Scratch &sc, cudaSt
   p.err = a.err; p.rowf = rowf; p.bits = bits;
   e = cudaFuncSetAttribute(k_attn_kv4_tc<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
   if (e != cudaSuccess) return e;
-  // The register split needs the count that the kernel was to be compiled to.
-  static const int regs = [] {
+  // The register split needs the count that the kernel was to be compiled to.  (A query
+  // that fails is asked again by the next call.)
+  static std::atomic<int> regs{0};
+  if (regs.load() == 0) {
     cudaFuncAttributes fa;
-    return cudaFuncGetAttributes(&fa, k_attn_kv4_tc<D>) == cudaSuccess ? fa.numRegs : 0;
-  }();
-  if (regs < kRegs) return cudaErrorInvalidConfiguration;
+    e = cudaFuncGetAttributes(&fa, k_attn_kv4_tc<D>);
+    if (e != cudaSuccess) return e;
+    regs.store(fa.numRegs);
+  }
+  if (regs.load() < kRegs) return cudaErrorInvalidConfiguration;
   e = launch_pdl(k_attn_kv4_tc<D>, dim3(sc.tiles, Hkv, p.nsplit), dim3(THREADS), S::SMEM, s, mQh,
                  mQl, mKh, mKl, mVh, mVl, p);
   if (e != cudaSuccess || p.nsplit == 1) return e;
