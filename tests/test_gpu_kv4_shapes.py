@@ -140,3 +140,15 @@ def test_values_that_are_no_numbers_reach_only_later_rows(si_ctx, heads, prefix,
         c.check(got[:where], q[:where], [(0, prefix, where)], every=19)
     assert np.isfinite(got[:, :hq // 2]).all()
     assert np.isnan(got[where:, hq // 2:, 32:64]).all()
+
+
+@pytest.mark.parametrize("heads,prefix,count", [((28, 4, 128), 500, 200), ((14, 2, 64), 3200, 211),
+                                                ((16, 2, 128), 7580, 612)])
+@pytest.mark.parametrize("qscale", [0.0, 1e-3, 6.0, 30.0])
+def test_sharp_and_flat_softmax_of_prompts(si_ctx, heads, prefix, count, qscale):
+    c = Cache(si_ctx, heads, 1, prefix + count, 64, seed=39)
+    c.random([(0, 0, prefix + count)])
+    runs = [(0, prefix, count)]
+    q = c.rng.standard_normal((count, heads[0], heads[2])) * qscale
+    c.check(c.attend(q, runs), q, runs, every=37)
+    c.kv.free()
