@@ -336,9 +336,17 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
   float m = -INFINITY, l = 0.0f;
-  // P.V operands are (p 2^sp) (d_v 2^dexp) for |d_v| < 2^(eR + 1); both factors
-  // and the product stay below 2^15.
-  int eR = -1000, sp = 0, dexp = 0;
+  // P.V operands are (p 2^p_shift) (d_v 2^d_shift) for |d_v| < 2^(eR + 1); both factors
+  // and the product stay below 2^15 (p below 2^4).  fp16 has no step finer than 2^-24,
+  // so that keys far below the maximum keep their bits p and the products both have to
+  // lie high: the largest d_v goes to 2^-3 to 2.  (Unscaled from 2^-8 to 2^8, with p
+  // making room for it, a first key 12 nats above 2100 others of size 300 or 0.01 cost
+  // those 1e-4 of their sum, now 2e-6.)  Only eR is kept: with the shifts in registers
+  // of their own 131071 keys took 53.6 us instead of 52.9.
+  int eR = -1000;
+  auto scaled = [](int e) { return e < -2 || e > 0; };  // values outside 1 to 8
+  auto d_shift = [&](int e) { return scaled(e) ? -e : 0; };
+  auto p_shift = [&](int e) { return scaled(e) || e == 0 ? 10 : 11; };
 
   for (int n = 0; n < mine; ++n) {
     if (n + kStages - 1 < mine) issue(n + kStages - 1);
@@ -449,11 +457,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
       }
       const uint32_t vm = __reduce_max_sync(0xffffffffu, vmax);
       if ((int)(vm >> 10) - 15 > eR) {
-        const int old = sp + dexp;
+        const int old = p_shift(eR) + d_shift(eR);
         eR = (int)(vm >> 10) - 15 + 1;  // one binade ahead
-        dexp = eR < -8 ? 10 : eR > 8 ? -8 : 0;
-        sp = min(11, 10 - (eR + dexp));
-        f *= pow2(sp + dexp - old);
+        f *= pow2(p_shift(eR) + d_shift(eR) - old);  // (the sums are 0 at the first tile)
       }
 #pragma unroll
       for (int i = 0; i < NB * 4; ++i)
@@ -483,17 +489,26 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
           dv[e][0] = *reinterpret_cast<const uint32_t *>(dp);
         }
       }
-      if (dexp) {  // uncommon sizes of V: scales below 2^-8 or from 2^8 on
-        const __half2 c = __float2half2_rn(pow2(dexp));
+      const float up = p_shift(eR) == 11 ? 2048.0f : 1024.0f;
+      float ps[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e) ps[e] = s[grp * 4 + e] * up;
+      if (scaled(eR)) {  // (3 to 4 % of the call)
 #pragma unroll
-          for (int i = 0; i < NB / 2; ++i) dv[e][i] = h2bits(__hmul2(as_h2(dv[e][i]), c));
+        for (int e = 0; e < 4; ++e) {
+          // Scaling d down would cost the small d of a key that dominates: there p, which
+          // has bits to spare, takes the factor.
+          const float c = pow2(-eR);
+          const bool by_p = eR > 0 && s[grp * 4 + e] >= 0.5f;
+          if (by_p) ps[e] *= c;
+          const __half2 c2 = __float2half2_rn(by_p ? 1.0f : c);
+#pragma unroll
+          for (int i = 0; i < NB / 2; ++i) dv[e][i] = h2bits(__hmul2(as_h2(dv[e][i]), c2));
+        }
       }
-      const float up = pow2(sp);
       uint32_t ph01, pl01, ph23, pl23;
-      split2(s[grp * 4] * up, s[grp * 4 + 1] * up, ph01, pl01);
-      split2(s[grp * 4 + 2] * up, s[grp * 4 + 3] * up, ph23, pl23);
+      split2(ps[0], ps[1], ph01, pl01);
+      split2(ps[2], ps[3], ph23, pl23);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const uint32_t sel = (b & 1) ? 0x7632 : 0x5410;
@@ -531,7 +546,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
   float2 *ml = reinterpret_cast<float2 *>(smem + kWarps * kHeads * S::OROW * 4);
   float2 *cta_ml = reinterpret_cast<float2 *>(amax_s);  // [8 heads]
   {
-    const float f0 = mine ? ldexpf(1.0f, -(sp + dexp)) : 0.0f, f1 = f0 * 0.0625f;
+    const float f0 = mine ? ldexpf(1.0f, -(p_shift(eR) + d_shift(eR))) : 0.0f, f1 = f0 * 0.0625f;
     float *o = ow + (warp * kHeads + g) * S::OROW + 8 * t;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {

@@ -152,3 +152,28 @@ def test_sharp_and_flat_softmax_of_prompts(si_ctx, heads, prefix, count, qscale)
     q = c.rng.standard_normal((count, heads[0], heads[2])) * qscale
     c.check(c.attend(q, runs), q, runs, every=37)
     c.kv.free()
+
+
+@pytest.mark.parametrize("vscale", [1e-5, 1e-3, 0.01, 0.1, 1.0, 4.0, 30.0, 300.0, 3000.0, 4e4])
+@pytest.mark.parametrize("heads,prefix,count,times", [
+    ((12, 2, 128), 8000, 2, 1), ((12, 2, 128), 7900, 131, 1),
+    ((64, 8, 128), 2100, 12, 6), ((56, 8, 64), 2100, 12, 6)])
+def test_a_first_key_far_above_values_of_any_size(si_ctx, heads, prefix, count, times, vscale):
+    """As above, with values of other sizes, whose scales must not take the bits of the
+    small probabilities: in many splits, in a prompt, and in a batch that fills the GPU
+    with a split or two of each token."""
+    hq, hkv, D = heads
+    n = prefix + count
+    c = Cache(si_ctx, heads, 1, n, 64, seed=40)
+    k, v = (c.rng.standard_normal((n, hkv, D)) for _ in range(2))
+    u = np.sign(c.rng.standard_normal(D))
+    k[0] = u
+    v *= vscale
+    v[0] *= 1e-6
+    c.append([(0, 0, n)], k, v)
+    q = c.rng.standard_normal((count * times, hq, D)) + 13 / np.sqrt(D) * u
+    runs = [(0, prefix, count)] * times
+    got = c.attend(q, runs)
+    c.check(got[:count], q[:count], runs[:1], every=29)
+    c.check(got[-count:], q[-count:], runs[:1], every=29)
+    c.kv.free()
