@@ -41,10 +41,12 @@
 // thread-block cluster and merge through distributed shared memory (72B, 8 x 4096
 // keys: 23.2 -> 19.7 us); more go through scratch and a second kernel.
 //
-// Bound by instruction issue, not by the cache's bytes: a tile of 4608 bytes takes
-// 818 instructions, some 350 of them to bring the codes into the operands, at 2.3 to
-// 2.6 a cycle and SM.  72B heads on B200: 131071 keys 52.5 us (2.9 TB/s; the copies
-// alone 35.5 us), 8 x 4096 keys 19.3 us.
+// Not bound by the cache's bytes: a tile of 4608 bytes takes 823 instructions, some 350
+// of them to bring the codes into the operands, at 2.3 of 4 a cycle and SM.  Three warps
+// a scheduler are too few to fill the rest: of the stalls the fixed latencies of
+// dependent instructions come first (0.99 of an issue), then full math pipes (0.79; the
+// fullest, the ALU, is busy 45 % of the time).  72B heads on B200: 131071 keys 53.0 us
+// (2.8 TB/s; the copies alone 35.5 us), 8 x 4096 keys 19.4 us.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -738,7 +740,9 @@ constexpr int kCtaKeys = 300, kMergeKeys = 600;
 void kv4_pick_splits(Kv4AttnArgs &a) {
   const int Hkv = a.kv.n_kv_heads;
   if (a.tok_ctx) {
-    // Lengths up to the cache's are possible: enough splits for one wave.
+    // Lengths up to the cache's are possible: enough splits for one wave.  (The lengths
+    // themselves are not known here: long ragged batches get fewer splits than above,
+    // short tokens of a long cache a second kernel that they do not need.)
     const int most = a.kv.max_pages * a.kv.page_len;
     a.nsplit = std::max(1, std::min(kSlots / (a.T * Hkv), (most + kMinSplit - 1) / kMinSplit));
     return;

@@ -50,7 +50,8 @@
 // 72B heads, 509 tokens on 7680 positions: P through shared memory and one issuing
 // warp 417 us, P from TMEM 362, windows taken at the next pair 337, keys a third
 // ahead 322, operands by packed arithmetic 305, now 302 (three MMAs a product: 430 TFLOP/s are
-// 1290); 7B, a prompt of 2048: 101.
+// 1290); 7B, a prompt of 2048: 101.  These are runs of some milliseconds; in series of half a
+// second and more the card's power lowers the clock: 351 and 109.
 #include <algorithm>
 #include <atomic>
 
