@@ -531,7 +531,7 @@ SI_API si_status si_kv4_read_dev(si_ctx *ctx, si_kv4 *kv, const si_kv4_run *runs
  * on the tensor cores (with si_ctx_set_exact_attention those of 16 and more through the
  * fp32 one over their keys unpacked), the others read the packed cache token by token.
  * fp32 in and out, within about 1e-6 of the 64-bit result (of the norm of a call's rows;
- * a single row 3e-6; large scores add the 2^-22 of their size that fp32 costs).  Where
+ * a single row 5e-6; large scores add the 2^-22 of their size that fp32 costs).  Where
  * one key has most of a row's weight, that holds for the others down to about 2^-18 of
  * it; those of less keep fewer bits.  Sums follow the split of the work, so a token's
  * result may differ in its last bits between calls with other runs.  A position whose V
