@@ -41,8 +41,9 @@
 // is handed from tile to tile through shared memory, by a tagged word per row (a
 // barrier's wait took 300 to 800 cycles there); the reference of the probabilities is
 // only raised by a score more than 2^6 above the maximum that set it.  Every wait is
-// bounded (about 2 s; SI_ERR_TIMEOUT in the context's error word); on expiry every role stops, the CTA's own copies and MMAs
-// in flight are waited for (bounded) and TMEM is freed.
+// bounded (about 2 s; SI_ERR_TIMEOUT in the context's error word); on expiry every role
+// stops, the CTA's own copies and MMAs in flight are waited for (bounded) and TMEM is
+// freed.
 //
 // Bound by the tensor pipe and shared memory together: an MMA of 128 x 128 x 16
 // takes 64 cycles and reads 8 KB of shared memory, all that there is in that time,
